@@ -60,6 +60,22 @@ _SIGS = {
     "clm_b200_verify_speculative": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _u64, _u64, _vp, _vp, _vp]),
     "clm_b200_accept_logits": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _f, _vp, _u64, _u64, _vp, _vp, _vp]),
     "clm_b200_philox_uniforms": (_i, [_vp, _u64, _u64, _u32, _u32, _u64, _vp, _vp]),
+    "clm_b200_sample_logits": (_i, [_vp, _vp, _i, _u32, _u32, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "clm_b200_rope_frequencies": (_i, [_i, _u32] + [C.c_double] * 5 + [_vp, _vp]),
+    "clm_b200_kv_append": (_i, [_vp, _vp, _u32, _vp, _u32, _u32, _u32, _i, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp,
+                                _vp, _vp]),
+    "clm_b200_kv_attention_workspace": (_i, [_vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, C.POINTER(_u64)]),
+    "clm_b200_kv_attention": (_i, [_vp, _vp, _u32, _vp, _u32, _u32, _u32, _vp, _u64, _u32, _vp, _vp, _vp, _f, _vp, _vp,
+                                   _u64, _vp]),
+    "clm_b200_kv_fork": (_i, [_vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
+    "clm_b200_kv_copy_pages": (_i, [_vp, _vp, _u32, _vp, _vp, _vp, _u64, _vp]),
+    "clm_b200_pages_create": (_i, [_u32, C.POINTER(_vp)]),
+    "clm_b200_pages_destroy": (_i, [_vp]),
+    "clm_b200_pages_alloc": (_i, [_vp, _u32, _vp]),
+    "clm_b200_pages_retain": (_i, [_vp, _u32, _vp]),
+    "clm_b200_pages_release": (_i, [_vp, _u32, _vp]),
+    "clm_b200_pages_info": (_i, [_vp, C.c_int32, C.POINTER(_u32), C.POINTER(_u32)]),
+    "clm_b200_pages_compact": (_i, [_vp, _u32, _vp, _vp, C.POINTER(_u32)]),
     "clm_b200_llama_create": (_i, [_vp, _vp, _vp, C.POINTER(_vp)]),
     "clm_b200_fixture_create": (_i, [_vp, _vp, _vp, C.POINTER(_vp)]),
     "clm_b200_engine_set_object": (_i, [_vp, C.c_char_p, _i, _vp, _u64]),

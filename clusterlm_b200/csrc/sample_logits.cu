@@ -1,0 +1,604 @@
+// sample_logits.cu — temperature, top-k, top-p and min-p sampling straight from logits, one launch, no scratch.
+//
+// Row: d_i = l_i - max l (f32, as distribution() forms it), e_i = exp(d_i / T).  In the order (d descending, index
+// ascending) three prefixes are allowed: the first top_k entries; the shortest prefix whose mass reaches top_p of the
+// whole row's; the entries with e_i >= min_p.  The token is the first allowed index i, in index order, with
+// u W < sum of e_j over allowed j <= i (W: the allowed mass), as sample_from walks a distribution.
+//
+// Masses are integers: w_i = round(2^44 e_i), evaluated with a relative error below 1e-12, summed in 64 bits.  Sums of
+// integers do not depend on their order, so a row's result is the same whatever computed it, every comparison is
+// exact on the w_i, and an entry below 2^-45 of the largest has no mass.
+//
+// A cluster of eight CTAs holds a row in shared memory (a slice each), so the logits are read from memory once however
+// many passes the row needs:
+//   1. load, maximum (and its lowest index: greedy rows end here);
+//   2. without top-k / top-p: the masses of the CTAs' sixteen warp segments;
+//      with them: the row's whole mass and a histogram of the entries over 64 bins per octave of e, whose counts bound
+//      the cumulative mass within 1.1%: the cut falls into known bins.  Entries above these are allowed (their exact
+//      mass is summed), entries below are not, and the few in them are ranked one against the other.  Where more than
+//      kCand entries share those bins (many equal logits, as from 16-bit types, or a flat row), the key range is
+//      bisected until few enough or one key value is left; of one value the lowest indices stay.
+//   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
+#include <cooperative_groups.h>
+
+#include "kv_ops.cuh"
+#include "pdl.cuh"
+
+namespace clm {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kCl = 8;             // CTAs of a row
+constexpr int kThr = 512;
+constexpr int kWrp = kThr / 32;    // warp segments of a CTA's slice
+constexpr int kBinsOct = 64;       // histogram bins per octave
+constexpr int kBins = 44 * kBinsOct;
+constexpr int kOwn = kBins / kCl;  // bins whose row totals a CTA forms
+constexpr int kCand = 1024;        // entries ranked one against the other
+constexpr int kFrac = 44;          // fraction bits of a mass
+constexpr uint32_t kMaxVocab = 8 * 44032;  // a slice and the tables fit in 227 KB
+
+typedef unsigned long long u64;
+
+struct Cand {
+  float d;
+  uint32_t idx;
+  u64 w;
+};
+
+struct SampleArgs {
+  const void* logits;
+  long long ld;
+  uint32_t V, slice;
+  const float *temp, *top_p, *min_p;
+  const int32_t* top_k;
+  const double* u;
+  int32_t* token;
+  float* prob;
+  int vec;  // rows and slices start 16-byte aligned
+};
+
+// round(2^44 * 2^y) for y <= 0 (0 below y = -45, and for -inf and NaN): 2^y = 2^n 2^f with |f| <= 1/2 and a degree-8
+// polynomial for 2^f (least maximum relative error by weighted least squares: 7.8e-13).
+__device__ __forceinline__ u64 mass_of(double y) {
+  if (!(y > -45.0)) return 0;
+  constexpr double kShift = 0x1.8p52;
+  const double k = y + kShift;
+  const int n = (int)(unsigned)__double_as_longlong(k);
+  const double f = y - (k - kShift);
+  double p = 0x1.61afce9c47e39p-20;
+  p = fma(p, f, 0x1.00dad250307efp-16);
+  p = fma(p, f, 0x1.430acca365ca2p-13);
+  p = fma(p, f, 0x1.5d87483855d48p-10);
+  p = fma(p, f, 0x1.3b2ab5c52912fp-7);
+  p = fma(p, f, 0x1.c6b08dd46d38ep-5);
+  p = fma(p, f, 0x1.ebfbdff9319e2p-3);
+  p = fma(p, f, 0x1.62e42fef8615ep-1);
+  p = fma(p, f, 0x1.ffffffffff7a3p-1);
+  const double scale = __hiloint2double((1023 + kFrac + n) << 20, 0);
+  return (u64)(__double_as_longlong(fma(p, scale, kShift)) - __double_as_longlong(kShift));
+}
+
+// Order of floats as integers (ascending).
+__device__ __forceinline__ uint32_t ord_of(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_ord(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+
+__device__ __forceinline__ u64 warp_sum(u64 x) {
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+struct Shared {
+  u64 top[kCl];       // (ordered maximum, ~index) of each CTA's slice
+  u64 total[kCl];     // whole mass (pass 2)
+  u64 above[kCl];     // mass above the candidates
+  u64 kept[kCl];      // allowed mass
+  uint32_t ncand[kCl];
+  u64 it_mass[2][kCl];  // bisection, alternating
+  uint32_t it_cnt[2][kCl];
+  uint32_t ties[kCl];
+  u64 seg[kWrp];      // allowed mass of the warp segments
+  u64 red[kWrp];
+  uint32_t redc[kWrp];
+  double redd[kWrp];
+  uint32_t cand_n;
+  int lo, hi;
+  uint32_t cnt_above;
+};
+
+template <typename S>
+__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
+    sample_logits_kernel(const __grid_constant__ SampleArgs a) {
+  extern __shared__ __align__(16) uint8_t sl_smem[];
+  __shared__ Shared s;
+  cg::cluster_group cluster = cg::this_cluster();
+  float* key = reinterpret_cast<float*>(sl_smem);  // [slice]
+  uint32_t* hist = reinterpret_cast<uint32_t*>(key + a.slice);
+  uint32_t* tot = hist + kBins;  // the row's histogram
+  Cand* mine = reinterpret_cast<Cand*>(tot + kBins);
+  Cand* all = reinterpret_cast<Cand*>(hist);  // the row's candidates, once the histograms are read
+  static_assert(sizeof(Cand) * kCand <= 2 * kBins * sizeof(uint32_t), "the candidates fit over the histograms");
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t rank = cluster.block_rank(), row = blockIdx.x / kCl;
+  const uint32_t v0 = min(a.V, rank * a.slice), cnt = min(a.V, v0 + a.slice) - v0;
+  // a value of this CTA goes to every CTA of the row
+  auto push = [&](auto* slot, auto value) {
+    if (tid < kCl) *cluster.map_shared_rank(slot + rank, tid) = value;
+  };
+  cluster.barrier_arrive();  // waited for before the first write into another CTA's shared memory
+  griddep_wait();
+  griddep_launch();
+
+  // ---- 1. load and maximum (NaN counts as -inf; -0 as 0)
+  const S* src = static_cast<const S*>(a.logits) + (long long)row * a.ld + v0;
+  float mx = -INFINITY;
+  auto put = [&](uint32_t i, float x) {
+    x = x == x ? x + 0.0f : -INFINITY;
+    key[i] = x;
+    mx = fmaxf(mx, x);
+  };
+  if (a.vec) {
+    constexpr int N = 16 / sizeof(S);
+    const uint32_t nv = cnt / N;
+#pragma unroll 4
+    for (uint32_t i = tid; i < nv; i += kThr) {
+      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(src) + i);
+      S e[N];
+      memcpy(e, &w, 16);
+#pragma unroll
+      for (int j = 0; j < N; ++j) put(i * N + j, to_f32(e[j]));
+    }
+    for (uint32_t i = nv * N + tid; i < cnt; i += kThr) put(i, to_f32(src[i]));
+  } else {
+#pragma unroll 4
+    for (uint32_t i = tid; i < cnt; i += kThr) put(i, to_f32(src[i]));
+  }
+  for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
+  if (tid == 0) s.cand_n = 0;
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) s.redd[warp] = mx;
+  __syncthreads();
+  for (int w = 0; w < kWrp; ++w) mx = fmaxf(mx, (float)s.redd[w]);
+  const float T = a.temp ? a.temp[row] : 1.0f;
+  const bool greedy = !(T > 0.0f);
+  uint32_t first = 0xffffffffu;  // lowest index of the slice's maximum (greedy rows)
+  if (greedy)
+    for (uint32_t i = tid; i < cnt; i += kThr)
+      if (key[i] == mx) first = min(first, v0 + i);
+  for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+  if (lane == 0) s.redc[warp] = first;
+  __syncthreads();
+  for (int w = 0; w < kWrp; ++w) first = min(first, s.redc[w]);
+  cluster.barrier_wait();  // every CTA of the row runs
+  push(s.top, (u64)ord_of(mx) << 32 | (u64)(0xffffffffu - first));
+  cluster.sync();
+  u64 best = 0;
+  for (int r = 0; r < kCl; ++r) best = max(best, s.top[r]);
+  const float M = of_ord((uint32_t)(best >> 32));
+  if (greedy || M == -INFINITY) {  // the same for the whole cluster
+    if (rank == 0 && tid == 0) {
+      a.token[row] = M == -INFINITY ? -1 : (int32_t)(0xffffffffu - (uint32_t)best);
+      if (a.prob) a.prob[row] = M == -INFINITY ? 0.0f : 1.0f;
+    }
+    return;
+  }
+
+  // ---- 2. what is allowed
+  const double c = 1.4426950408889634 / (double)T;
+  const float cf = (float)c;
+  const int32_t k_in = a.top_k ? a.top_k[row] : 0;
+  const float p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f;
+  const bool need_k = k_in > 0 && (uint32_t)k_in < a.V, need_p = p_in < 1.0f;
+  const uint32_t k = need_k ? (uint32_t)k_in : 0xffffffffu;
+  const double ymin = m_in > 0.0f ? log2((double)fminf(m_in, 1.0f)) : -46.0;
+  auto d_of = [&](float x) { return x == M ? 0.0f : __fsub_rn(x, M); };
+  auto y_of = [&](float d) { return d == 0.0f ? 0.0 : (double)d * c; };
+  auto bin_of = [&](float d) {  // ascends as the order does (cf may be infinite: 0 has bin 0)
+    return d == 0.0f ? 0 : min(kBins - 1, (int)fminf(-d * cf * (float)kBinsOct, (float)kBins));
+  };
+  auto u_of = [&](float d) { return __float_as_uint(fabsf(d)); };  // ascends as the order does
+  const uint32_t seg = (a.slice + kWrp - 1) / kWrp;
+  const uint32_t s0 = min(cnt, warp * seg), s1 = min(cnt, s0 + seg);  // this warp's segment
+  int hi = kBins;                 // allowed entries: bin <= hi, u <= umax, key not struck out
+  uint32_t umax = 0x7f7fffffu;
+  u64 seg_mass = 0;
+  if (!need_k && !need_p) {
+    for (uint32_t i = s0 + lane; i < s1; i += 32) {
+      const double y = y_of(d_of(key[i]));
+      if (y >= ymin) seg_mass += mass_of(y);
+    }
+    seg_mass = warp_sum(seg_mass);
+  } else {
+    u64 sum = 0;
+    for (uint32_t i = s0 + lane; i < s1; i += 32) {
+      const float d = d_of(key[i]);
+      const double y = y_of(d);
+      if (!(y > -45.0)) continue;
+      if (need_p) sum += mass_of(y);
+      if (y >= ymin) atomicAdd(&hist[bin_of(d)], 1u);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) s.red[warp] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < kWrp; ++w) sum += s.red[w];
+    push(s.total, sum);
+    cluster.sync();
+    for (int b = tid; b < kOwn; b += kThr) {
+      const int bin = (int)rank * kOwn + b;
+      uint32_t n = 0;
+      for (int r = 0; r < kCl; ++r) n += cluster.map_shared_rank(hist, r)[bin];
+      for (int r = 0; r < kCl; ++r) cluster.map_shared_rank(tot, r)[bin] = n;
+    }
+    cluster.sync();
+    u64 total = 0;
+    for (int r = 0; r < kCl; ++r) total += s.total[r];
+    // allowed by top-p: entries with less than `thr` mass before them (p in units of 2^-40, rounded up)
+    u64 thr = ~0ull;
+    if (need_p) {
+      const u64 pi = (u64)ceil(fmax((double)p_in, 0.0) * 0x1p40);
+      const u64 ph = __umul64hi(pi, total), pl = pi * total;
+      thr = (ph << 24 | pl >> 40) + ((pl & 0xffffffffffull) != 0);
+      if (thr == 0) thr = 1;
+    }
+    // cumulative counts and (approximate) masses over the bins
+    constexpr int kPer = (kBins + kThr - 1) / kThr;
+    uint32_t n[kPer];
+    double m[kPer];
+    uint32_t nsum = 0;
+    double msum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int bin = tid * kPer + j;
+      n[j] = bin < kBins ? tot[bin] : 0u;
+      m[j] = n[j] ? (double)n[j] * (double)exp2f((float)kFrac - (float)bin / kBinsOct) : 0.0;
+      nsum += n[j];
+      msum += m[j];
+    }
+    uint32_t nx = nsum;
+    double mm = msum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t on = __shfl_up_sync(0xffffffffu, nx, o);
+      const double om = __shfl_up_sync(0xffffffffu, mm, o);
+      if (lane >= o) {
+        nx += on;
+        mm += om;
+      }
+    }
+    if (lane == 31) {
+      s.redc[warp] = nx;
+      s.redd[warp] = mm;
+    }
+    if (tid == 0) {
+      s.lo = kBins;
+      s.hi = kBins;
+    }
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) {
+      nx += s.redc[w];
+      mm += s.redd[w];
+    }
+    nx -= nsum;
+    mm -= msum;
+    // a bin's entries weigh between 2^(-1/64) and 1 times its upper edge (1e-4 covers the f32 roundings)
+    constexpr double kUp = 1.0001, kDown = 0.989228 * 0.9999;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int bin = tid * kPer + j;
+      if (bin >= kBins) break;
+      nx += n[j];
+      mm += m[j];
+      const bool by_k = nx >= k;
+      if (by_k || (need_p && mm * kUp >= (double)thr)) atomicMin(&s.lo, bin);
+      if (by_k || (need_p && mm * kDown >= (double)thr)) atomicMin(&s.hi, bin);
+    }
+    __syncthreads();
+    const int lo = s.lo;
+    hi = s.hi;
+    if (lo < kBins) {  // else every entry with mass is allowed
+      if (tid == lo / kPer) {
+        uint32_t before = nx - nsum;
+        for (int j = 0; j < lo % kPer; ++j) before += n[j];
+        s.cnt_above = before;
+      }
+    } else if (tid == 0) {
+      s.cnt_above = 0;
+    }
+    for (uint32_t i = s0 + lane; i < s1; i += 32) {
+      const float d = d_of(key[i]);
+      const double y = y_of(d);
+      if (!(y > -45.0) || y < ymin) continue;
+      const int bin = bin_of(d);
+      if (bin > hi) continue;
+      const u64 w = mass_of(y);
+      if (bin < lo) {
+        seg_mass += w;
+      } else {
+        const uint32_t at = atomicAdd(&s.cand_n, 1u);
+        if (at < kCand) mine[at] = Cand{d, v0 + i, w};
+      }
+    }
+    seg_mass = warp_sum(seg_mass);
+    if (lane == 0) s.seg[warp] = seg_mass;
+    __syncthreads();
+    {
+      u64 x = 0;
+      for (int w = 0; w < kWrp; ++w) x += s.seg[w];
+      push(s.above, x);
+      push(s.ncand, s.cand_n);
+    }
+    cluster.sync();
+    u64 above = 0;
+    uint32_t cand = 0, before = 0;
+    for (int r = 0; r < kCl; ++r) {
+      above += s.above[r];
+      if (r < (int)rank) before += s.ncand[r];
+      cand += s.ncand[r];
+    }
+    uint32_t cnt_above = s.cnt_above;
+    bool recount = false;  // the segments' masses are summed anew
+    bool struck = false;
+    if (cand > kCand) {
+      // bisect the keys of the bins [lo, hi]: entries with u < ul are allowed, entries with u > uh are not
+      uint32_t ul = 0, uh = 0x7f7fffffu;
+      int turn = 0;
+      recount = true;
+      while (ul < uh && cand > kCand) {
+        const uint32_t mid = ul + (uh - ul) / 2;
+        uint32_t cl = 0;
+        u64 ml = 0;
+        for (uint32_t i = s0 + lane; i < s1; i += 32) {
+          const float d = d_of(key[i]);
+          const uint32_t u = u_of(d);
+          if (u < ul || u > mid) continue;
+          const int bin = bin_of(d);
+          const double y = y_of(d);
+          if (bin < lo || bin > hi || !(y > -45.0) || y < ymin) continue;
+          ++cl;
+          ml += mass_of(y);
+        }
+        cl = __reduce_add_sync(0xffffffffu, cl);
+        ml = warp_sum(ml);
+        __syncthreads();
+        if (lane == 0) {
+          s.redc[warp] = cl;
+          s.red[warp] = ml;
+        }
+        __syncthreads();
+        cl = 0;
+        ml = 0;
+        for (int w = 0; w < kWrp; ++w) {
+          cl += s.redc[w];
+          ml += s.red[w];
+        }
+        push(s.it_cnt[turn], cl);
+        push(s.it_mass[turn], ml);
+        cluster.sync();
+        cl = 0;
+        ml = 0;
+        for (int r = 0; r < kCl; ++r) {
+          cl += s.it_cnt[turn][r];
+          ml += s.it_mass[turn][r];
+        }
+        turn ^= 1;
+        if (cnt_above + cl >= k || above + ml >= thr) {
+          uh = mid;
+          cand = cl;
+        } else {
+          ul = mid + 1;
+          cnt_above += cl;
+          above += ml;
+          cand -= cl;
+        }
+      }
+      umax = uh;
+      if (cand <= kCand) {
+        // collect the candidates again, from the narrowed range
+        __syncthreads();
+        if (tid == 0) s.cand_n = 0;
+        __syncthreads();
+        for (uint32_t i = s0 + lane; i < s1; i += 32) {
+          const float d = d_of(key[i]);
+          const uint32_t u = u_of(d);
+          if (u < ul || u > uh) continue;
+          const int bin = bin_of(d);
+          const double y = y_of(d);
+          if (bin < lo || bin > hi || !(y > -45.0) || y < ymin) continue;
+          mine[atomicAdd(&s.cand_n, 1u)] = Cand{d, v0 + i, mass_of(y)};
+        }
+        __syncthreads();
+        push(s.ncand, s.cand_n);
+        cluster.sync();
+        before = cand = 0;
+        for (int r = 0; r < kCl; ++r) {
+          if (r < (int)rank) before += s.ncand[r];
+          cand += s.ncand[r];
+        }
+      } else {
+        // one key value: its `stay` lowest indices are allowed
+        struck = true;
+        const float d = -__uint_as_float(ul);
+        const u64 w = mass_of(y_of(d));
+        u64 stay = ~0ull;
+        if (need_k) stay = k - cnt_above;
+        if (need_p && w > 0) stay = min(stay, (thr - above + w - 1) / w);
+        uint32_t ties = 0;
+        for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
+          const uint32_t i = i0 + lane;
+          ties += __popc(__ballot_sync(0xffffffffu, i < s1 && u_of(d_of(key[i])) == ul));
+        }
+        __syncthreads();
+        if (lane == 0) s.redc[warp] = ties;
+        __syncthreads();
+        uint32_t all_ties = 0, rank_in = 0;
+        for (int w2 = 0; w2 < kWrp; ++w2) {
+          if (w2 < warp) rank_in += s.redc[w2];
+          all_ties += s.redc[w2];
+        }
+        push(s.ties, all_ties);
+        cluster.sync();
+        for (int r = 0; r < (int)rank; ++r) rank_in += s.ties[r];
+        for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
+          const uint32_t i = i0 + lane;
+          const bool tie = i < s1 && u_of(d_of(key[i])) == ul;
+          const uint32_t bal = __ballot_sync(0xffffffffu, tie);
+          if (tie && rank_in + __popc(bal & ((1u << lane) - 1u)) >= stay) key[i] = -INFINITY;
+          rank_in += __popc(bal);
+        }
+        __syncthreads();
+      }
+    }
+    if (!struck && cand > 0) {
+      // every candidate's rank and the mass before it, against all candidates of the row
+      for (int r = 0, at = 0; r < kCl; ++r) {
+        const Cand* theirs = cluster.map_shared_rank(mine, r);
+        for (uint32_t i = tid; i < s.ncand[r]; i += kThr) all[at + i] = theirs[i];
+        at += s.ncand[r];
+      }
+      __syncthreads();
+      for (uint32_t i = tid; i < s.ncand[rank]; i += kThr) {
+        const Cand me = all[before + i];
+        uint32_t cb = cnt_above;
+        u64 mb = above;
+        for (uint32_t j = 0; j < cand; ++j) {
+          const Cand o = all[j];
+          if (o.d > me.d || (o.d == me.d && o.idx < me.idx)) {
+            ++cb;
+            mb += o.w;
+          }
+        }
+        if (cb < k && mb < thr) {
+          if (!recount) atomicAdd(&s.seg[(me.idx - v0) / seg], me.w);
+        } else {
+          key[me.idx - v0] = -INFINITY;
+        }
+      }
+      __syncthreads();
+    }
+    if (recount) {
+      seg_mass = 0;
+      for (uint32_t i = s0 + lane; i < s1; i += 32) {
+        const float d = d_of(key[i]);
+        const double y = y_of(d);
+        if (bin_of(d) <= hi && u_of(d) <= umax && y >= ymin) seg_mass += mass_of(y);
+      }
+      seg_mass = warp_sum(seg_mass);
+    } else {
+      seg_mass = s.seg[warp];
+    }
+    __syncthreads();
+  }
+
+  // ---- 3. the token
+  if (lane == 0) s.seg[warp] = seg_mass;
+  __syncthreads();
+  {
+    u64 x = 0;
+    for (int w = 0; w < kWrp; ++w) x += s.seg[w];
+    push(s.kept, x);
+  }
+  cluster.sync();
+  u64 W = 0;
+  for (int r = 0; r < kCl; ++r) W += s.kept[r];
+  // floor(u W), exactly: u = m 2^-e with a 53-bit m
+  const double u = a.u[row];
+  u64 r = 0;
+  if (u > 0x1p-64 && u < 1.0) {
+    const u64 bits = (u64)__double_as_longlong(u);
+    const int e = 1075 - (int)(bits >> 52);  // 53 .. 117
+    const u64 m = (bits & 0xfffffffffffffull) | 1ull << 52;
+    const u64 ph = __umul64hi(m, W), pl = m * W;
+    r = e < 64 ? ph << (64 - e) | pl >> e : ph >> (e - 64);
+  } else if (!(u < 1.0)) {
+    r = W - 1;  // at or past the end (and NaN): the last allowed token
+  }
+  u64 base = 0;
+  uint32_t owner = 0;
+  for (; owner + 1 < (uint32_t)kCl && base + s.kept[owner] <= r; ++owner) base += s.kept[owner];
+  if (owner != rank) return;
+  int ws = 0;
+  for (; ws + 1 < kWrp && base + s.seg[ws] <= r; ++ws) base += s.seg[ws];
+  // entries of the segment, kPerT consecutive ones a thread
+  const uint32_t g0 = min(cnt, ws * seg), g1 = min(cnt, g0 + seg), per = (seg + kThr - 1) / kThr;
+  const uint32_t e0 = min(g1, g0 + tid * per), e1 = min(g1, e0 + per);
+  auto mass_at = [&](uint32_t i) -> u64 {
+    const float d = d_of(key[i]);
+    const double y = y_of(d);
+    return bin_of(d) <= hi && u_of(d) <= umax && y >= ymin ? mass_of(y) : 0ull;
+  };
+  u64 own = 0;
+  for (uint32_t i = e0; i < e1; ++i) own += mass_at(i);
+  u64 inc = own;
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  __syncthreads();
+  if (lane == 31) s.red[warp] = inc;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) base += s.red[w];
+  base += inc - own;
+  if (own > 0 && base <= r && r < base + own) {
+    for (uint32_t i = e0; i < e1; ++i) {
+      const u64 w = mass_at(i);
+      if (w > 0 && r < base + w) {
+        a.token[row] = (int32_t)(v0 + i);
+        if (a.prob) a.prob[row] = (float)(exp2(y_of(d_of(key[i]))) / ((double)W * 0x1p-44));
+        break;
+      }
+      base += w;
+    }
+  }
+}
+
+template <typename S>
+int launch_sample_logits(SampleArgs a, uint32_t rows, cudaStream_t st) {
+  constexpr int N = 16 / sizeof(S);
+  a.slice = (uint32_t)((ceil_div(a.V, kCl) + N - 1) / N * N);
+  a.slice = (a.slice + 3) / 4 * 4;  // the tables after the keys stay 16-byte aligned
+  a.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.ld % N == 0;
+  const size_t smem = (size_t)a.slice * 4 + 2 * kBins * sizeof(uint32_t) + kCand * sizeof(Cand);
+  CLM_TRY(ensure_smem(sample_logits_kernel<S>, smem));
+  return launch_pdl(sample_logits_kernel<S>, dim3(rows * kCl), dim3(kThr), smem, st, a);
+}
+
+}  // namespace
+
+}  // namespace clm
+
+using namespace clm;
+
+extern "C" int clm_b200_sample_logits(clm_b200_ctx* ctx, const void* d_logits, int dtype, uint32_t rows, uint32_t vocab,
+                                      uint64_t ld, const float* d_temperature, const int32_t* d_top_k,
+                                      const float* d_top_p, const float* d_min_p, const double* d_uniforms,
+                                      int32_t* d_out, float* d_probs, void* stream) {
+  CLM_CHECK(ctx != nullptr, CLM_INVALID_ARGUMENT, "null context");
+  CLM_CHECK(vocab > 0, CLM_INVALID_ARGUMENT, "empty vocabulary");
+  CLM_CHECK(vocab <= kMaxVocab, CLM_OUT_OF_RANGE, "vocabulary too large for sampling");
+  CLM_CHECK(ld >= vocab && ld < (1ull << 40), CLM_INVALID_ARGUMENT, "a row stride is smaller than a row");
+  CLM_CHECK(dtype >= CLM_DTYPE_F32 && dtype <= CLM_DTYPE_BF16, CLM_INVALID_ARGUMENT, "unknown element type");
+  if (rows == 0) return CLM_OK;
+  CLM_CHECK(d_logits && d_uniforms && d_out, CLM_INVALID_ARGUMENT, "null buffer");
+  CLM_CHECK(rows <= 0x7fffffffu / kCl, CLM_OUT_OF_RANGE, "too many rows");
+  SampleArgs a{};
+  a.logits = d_logits;
+  a.ld = (long long)ld;
+  a.V = vocab;
+  a.temp = d_temperature;
+  a.top_k = d_top_k;
+  a.top_p = d_top_p;
+  a.min_p = d_min_p;
+  a.u = d_uniforms;
+  a.token = d_out;
+  a.prob = d_probs;
+  CLM_SCOPE(ctx);
+  cudaStream_t st = pick_stream(ctx, stream);
+  if (dtype == CLM_DTYPE_F32) return launch_sample_logits<float>(a, rows, st);
+  if (dtype == CLM_DTYPE_F16) return launch_sample_logits<__half>(a, rows, st);
+  return launch_sample_logits<__nv_bfloat16>(a, rows, st);
+}

@@ -39,6 +39,28 @@ def _stream() -> _vp:
     return _vp(h if h else _LEGACY_STREAM)
 
 
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _stream_on(device: int) -> _vp:
+    """torch's current stream of `device` (which need not be the current device)."""
+    h = torch.cuda.current_stream(device).cuda_stream
+    return _vp(h if h else _LEGACY_STREAM)
+
+
+def _operand(ctx: "Context", name: str, t: torch.Tensor, dtype=None, shape=None, contiguous: bool = True) -> _vp:
+    """The address of an operator's tensor, checked: on the context's device, of this type and shape."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != ctx.device:
+        raise ValueError(f"{name}: expected a tensor on cuda:{ctx.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor")
+    return _vp(t.data_ptr())
+
+
 def device_count() -> int:
     n = C.c_int(0)
     call("clm_b200_device_count", C.byref(n))
@@ -155,6 +177,41 @@ def sample_from(ctx: Context, probs: torch.Tensor, uniforms: torch.Tensor) -> to
     out = torch.empty(rows, dtype=torch.int32, device=probs.device)
     call("clm_b200_sample_rows", ctx.h, _ptr(probs), rows, vocab, _ptr(uniforms), _ptr(out), _stream())
     return out
+
+
+def sample_logits(ctx: Context, logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0, with_probs: bool = False):
+    """One token per row of logits (rows, vocab) f32 / f16 / bf16, the last dim contiguous (rows may be a view of wider
+    ones), with one float64 uniform per row.  temperature (<= 0: argmax), top_k (0: all), top_p (1: all) and min_p (0:
+    all) are numbers, or tensors (rows,) of float32 (top_k: int32).  Returns int32 tokens (rows,), -1 for a row without
+    a finite logit; with_probs: also the tokens' probabilities among the allowed entries, float32 (rows,)."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in DTYPES:
+        raise ValueError("logits: expected a (rows, vocab) tensor of float32, float16 or bfloat16")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: the last dimension must be contiguous")
+    if rows > 1 and logits.stride(0) < vocab:
+        raise ValueError("logits: rows overlap")
+    ld = logits.stride(0) if rows > 1 else vocab
+    lp = _operand(ctx, "logits", logits, contiguous=False)
+    up = _operand(ctx, "uniforms", uniforms, torch.float64, (rows,))
+    keep = []
+
+    def setting(name, value, default, dtype):
+        if not isinstance(value, torch.Tensor):
+            if value == default:
+                return None
+            value = torch.full((rows,), value, dtype=dtype, device=logits.device)
+        keep.append(value)
+        return _operand(ctx, name, value, dtype, (rows,))
+
+    settings = (setting("temperature", temperature, 1.0, torch.float32), setting("top_k", top_k, 0, torch.int32),
+                setting("top_p", top_p, 1.0, torch.float32), setting("min_p", min_p, 0.0, torch.float32))
+    out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if with_probs else None
+    call("clm_b200_sample_logits", ctx.h, lp, DTYPES[logits.dtype], rows, vocab, ld, *settings, up,
+         _vp(out.data_ptr()), _vp(probs.data_ptr()) if with_probs else None, _stream_on(ctx.device))
+    return (out, probs) if with_probs else out
 
 
 def verify_speculative(ctx: Context, target: torch.Tensor, drafts: torch.Tensor, draft_probs: torch.Tensor | None,

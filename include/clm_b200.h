@@ -53,6 +53,9 @@ enum {
  * first three; Q4_K is the ggml 256-element / 144-byte superblock, ggml_types.cpp:26). */
 enum { CLM_QUANT_F32 = 0, CLM_QUANT_Q8_FIXTURE = 1, CLM_QUANT_Q8_0 = 2, CLM_QUANT_Q4_K = 3 };
 
+/* Element types of activations, caches and logits. */
+enum { CLM_DTYPE_F32 = 0, CLM_DTYPE_F16 = 1, CLM_DTYPE_BF16 = 2 };
+
 /* ---- library / context ------------------------------------------------------------------------ */
 CLM_API int clm_b200_abi_version(void);
 CLM_API const char* clm_b200_last_error(void);
@@ -131,6 +134,22 @@ CLM_API int clm_b200_distribution_rows(clm_b200_ctx* ctx, const float* d_logits,
  * error bound proves the serial rounding cannot change it; otherwise the row is re-walked serially. */
 CLM_API int clm_b200_sample_rows(clm_b200_ctx* ctx, const float* d_probs, uint32_t rows, uint32_t vocab,
                          const double* d_uniforms, int32_t* d_out, void* stream);
+/* A token per row straight from logits (f32, f16 or bf16; row r starts ld elements after row r - 1; vocab <= 352256),
+ * every row with its own settings; a NULL array is the default for all rows.  No reference counterpart in this form
+ * (distribution() and sample_from(), sampling.cpp:51-101, with one setting; min-p is not in the reference).
+ *   d_temperature  e_i = exp((l_i - max) / T), default 1; T <= 0 (or NaN): the lowest index of the maximum
+ *   d_top_k        in the order (logit descending, index ascending), the first k; <= 0: all
+ *   d_top_p        the shortest prefix of that order whose mass reaches p of the whole row's; >= 1: all
+ *   d_min_p        the entries with e_i >= min(p, 1) (the maximum's e is 1); <= 0: all
+ * The token is the first entry i, by index, that all of them allow and for which u * W < the mass of the allowed
+ * entries up to i (W: of all of them); u = d_uniforms[row] in [0, 1).  Masses are held as integers in units of 2^-44
+ * of the largest entry's, so a row's token does not depend on the batch.  -inf and NaN logits are never drawn; a row
+ * with nothing else gives token -1.  d_probs (optional): the token's probability among the allowed ones (0 for -1).
+ * Allocates nothing and can be captured. */
+CLM_API int clm_b200_sample_logits(clm_b200_ctx* ctx, const void* d_logits, int dtype, uint32_t rows, uint32_t vocab,
+                                   uint64_t ld, const float* d_temperature, const int32_t* d_top_k,
+                                   const float* d_top_p, const float* d_min_p, const double* d_uniforms,
+                                   int32_t* d_out, float* d_probs, void* stream);
 /* verify_speculative() for `batch` sequences (sampling.cpp:103-131).
  *   d_target      [batch][k+1][vocab] target probabilities
  *   d_drafts      [batch][k] drafted tokens
@@ -175,6 +194,97 @@ CLM_API int clm_b200_shard_probs(clm_b200_ctx* ctx, const float* d_logits, uint3
 /* Philox4x32-10 uniforms: out[i] = top 53 bits of (o0:o1) * 2^-53 for counter (first+i lo, hi, c2, c3). */
 CLM_API int clm_b200_philox_uniforms(clm_b200_ctx* ctx, uint64_t seed, uint64_t first, uint32_t c2, uint32_t c3, uint64_t n,
                              double* d_out, void* stream);
+
+/* ---- paged KV cache operators: many continuations of one prompt ------------------------------------
+ * (no reference counterpart: the reference's sequence state is private to a domain, reference_domain.cpp:297-329.)
+ * The operators work on caller-owned device memory, so they serve any cache laid out like the engines' own; every
+ * call is asynchronous on `stream`, allocates nothing and can be captured into a graph.  What it reads on the device
+ * (tables, positions, frequencies, rows) is read at every replay; host arguments are baked in.
+ *
+ * A pool holds `pages` pages of 64 positions per layer, K as [layers][pages][n_kv_heads][64][head_dim] and V as
+ * [layers][pages][n_kv_heads][head_dim][64]; within a page the 16-byte chunks are permuted (clm_b200_kv_append writes
+ * them, clm_b200_kv_attention reads them): chunk c of a K row of position p lies at c ^ (c >= 8 ? 2 : 0) ^ (p & 1),
+ * chunk c of a V row of dim d at c ^ (d & 1).  head_dim 64 or 128; f16 or bf16. */
+typedef struct {
+  void* k;
+  void* v;
+  uint32_t layers, pages, n_kv_heads, head_dim;
+  int dtype;
+} clm_b200_kv_pool;
+/* Page tables [rows][max_pages] and committed positions [rows], device memory: sequence b's position j lies in page
+ * d_tables[b][j / 64].  An entry outside [0, pages) is no page: its positions are not seen and rows that would enter
+ * it are dropped.  A negative position marks an idle sequence. */
+typedef struct {
+  int32_t* d_tables;
+  int64_t* d_pos;
+  uint32_t rows, max_pages;
+} clm_b200_kv_seqs;
+
+/* Rotary positions: pair j of the leading `rot` dims of a head turns by position * d_inv_freq[j] (doubles on the
+ * device), then times `scale`.  Pairs are (2j, 2j + 1) or (j, j + rot / 2). */
+enum { CLM_ROPE_INTERLEAVED = 0, CLM_ROPE_HALF = 1 };
+typedef struct {
+  int layout;
+  uint32_t rot;
+  const double* d_inv_freq;
+  float scale;
+} clm_b200_rope;
+/* The rot / 2 frequencies theta^(-2j / rot) and the scale: as they are; all divided by `factor`; by bands (those with
+ * more than `high` turns in the `original` context kept, those with fewer than `low` divided, blended between); or
+ * YaRN (the bands blended over the pair index, scale 0.1 ln(factor) + 1).  Host arrays. */
+enum { CLM_ROPE_PLAIN = 0, CLM_ROPE_LINEAR = 1, CLM_ROPE_BANDS = 2, CLM_ROPE_YARN = 3 };
+CLM_API int clm_b200_rope_frequencies(int kind, uint32_t rot, double theta, double factor, double low, double high,
+                                      double original, double* h_inv_freq, float* h_scale);
+/* Rows enter the cache: for sequences 0..n-1, `positions` rows each, at d_pos[b] + i: k (rotated) and v go to the
+ * pages, q (optional) is rotated into d_q_out [n][positions][n_heads][head_dim] in the pool's type.  Row r of q / k / v
+ * starts ld elements after row r - 1 (slices of one fused projection).  d_parents (optional, <= 256 nodes): a tree
+ * window as in clm_b200_run_tree_window; node i is placed at d_pos[b] + i and rotated at d_pos[b] + depth(i).
+ * rope NULL: no rotation.  The positions are not advanced.  Idle sequences: nothing enters, their q rows become 0. */
+CLM_API int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t layer,
+                               const clm_b200_kv_seqs* seqs, uint32_t n, uint32_t positions, uint32_t n_heads,
+                               int src_dtype, const void* d_q, uint64_t ld_q, const void* d_k, uint64_t ld_k,
+                               const void* d_v, uint64_t ld_v, const clm_b200_rope* rope, const int32_t* d_parents,
+                               void* d_q_out, void* stream);
+/* Attention of `positions` (<= 256) rows of each of n (<= 512) sequences over the cache: row i of sequence b sees the
+ * positions below d_pos[b] and the window rows 0..i (or, with d_parents, its ancestors and itself), which
+ * clm_b200_kv_append has placed there.  Group g (of n_groups <= 64) is the next h_group_seqs[g] sequences, whose first
+ * h_group_pages[g] table entries are the same: these pages are read once for all of the group's rows.  Sequences after
+ * the last group share nothing.  Softmax statistics and sums are f32, the weights round to the pool's type for their
+ * product with v.  Rows that see nothing (idle sequences) become 0.  q rows ld_q elements apart, 16-byte aligned, like
+ * d_out; q, pool and out have one type.  d_work: clm_b200_kv_attention_workspace bytes, 16-byte aligned, used by this
+ * call alone while it runs (a captured graph keeps its own). */
+CLM_API int clm_b200_kv_attention_workspace(clm_b200_ctx* ctx, uint32_t n, uint32_t positions, uint32_t n_heads,
+                                            uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_groups,
+                                            const uint32_t* h_group_seqs, const uint32_t* h_group_pages,
+                                            uint64_t* bytes);
+CLM_API int clm_b200_kv_attention(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t layer,
+                                  const clm_b200_kv_seqs* seqs, uint32_t n, uint32_t positions, uint32_t n_heads,
+                                  const void* d_q, uint64_t ld_q, uint32_t n_groups, const uint32_t* h_group_seqs,
+                                  const uint32_t* h_group_pages, const int32_t* d_parents, float scale, void* d_out,
+                                  void* d_work, uint64_t work_bytes, void* stream);
+/* Forks: child h_children[i] takes over the full pages of h_parents[i] (the table entries), its position, and a copy,
+ * in page h_new_pages[i], of the parent's last page in every layer (no copy when the position is a multiple of 64; the
+ * entry is set all the same).  n <= 256; a child appears once and is no parent of the same call. */
+CLM_API int clm_b200_kv_fork(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, const clm_b200_kv_seqs* seqs, uint32_t n,
+                             const uint32_t* h_parents, const uint32_t* h_children, const int32_t* h_new_pages,
+                             void* stream);
+/* Copies page h_src[i] to h_dst[i] in every layer.  With d_tables (table_entries entries) the pages move: entries that
+ * name h_src[i] then name h_dst[i].  Destinations are distinct and no sources. */
+CLM_API int clm_b200_kv_copy_pages(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t n, const int32_t* h_src,
+                                   const int32_t* h_dst, int32_t* d_tables, uint64_t table_entries, void* stream);
+/* Host ledger of a pool's pages: which are free, and how many sequences hold each.  alloc takes the lowest free pages
+ * (none when fewer than n are free: CLM_RESOURCE_EXHAUSTED), retain adds a holder to each page, release drops one
+ * (CLM_NOT_FOUND, and nothing changed, when a page is not in use), compact plans the moves that pack the live pages
+ * into the lowest ones, for clm_b200_kv_copy_pages (`capacity` moves fit; *h_moves says how many there are). */
+typedef struct clm_b200_pages clm_b200_pages;
+CLM_API int clm_b200_pages_create(uint32_t pages, clm_b200_pages** out);
+CLM_API int clm_b200_pages_destroy(clm_b200_pages* p);
+CLM_API int clm_b200_pages_alloc(clm_b200_pages* p, uint32_t n, int32_t* h_ids);
+CLM_API int clm_b200_pages_retain(clm_b200_pages* p, uint32_t n, const int32_t* h_ids);
+CLM_API int clm_b200_pages_release(clm_b200_pages* p, uint32_t n, const int32_t* h_ids);
+CLM_API int clm_b200_pages_info(const clm_b200_pages* p, int32_t id, uint32_t* h_refs, uint32_t* h_free);
+CLM_API int clm_b200_pages_compact(clm_b200_pages* p, uint32_t capacity, int32_t* h_src, int32_t* h_dst,
+                                   uint32_t* h_moves);
 
 /* ---- execution engine: one stage (a contiguous layer range) of a model on one GPU ------------------
  * Replaces the CPU ReferenceDomain's compute (runtime/domain/src/reference_domain.cpp:376-585) behind

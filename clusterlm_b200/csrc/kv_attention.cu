@@ -4,15 +4,16 @@
 // its sequence shares with its group and the sequence's own pages; both parts (and any further split of them) give a
 // partial (unnormalised o, running maximum m, sum l), and partials combine by their maxima.
 //
-// Work is the list of (row tile, page) pairs.  An "entry" is a group's shared pages (rows: all query heads of a kv
-// head of all the group's window rows) or a sequence's own pages (rows: its own); an entry has one item per (kv head,
-// tile of up to 128 rows), and an item has as many work units as the entry has pages.  The line of all units is cut
-// into equal shares, one per CTA, so ragged lengths balance without any host knowledge of them; a CTA's part of an item
-// is a segment, and (item + CTA) numbers the segments without gaps to search.  A second kernel combines each row's
-// segments.
+// An "entry" is a group's shared pages (rows: all query heads of a kv head of all the group's window rows) or a sequence's
+// own pages (rows: its own).  Entries of up to kStreamRows rows per kv head are bound by reading the pages: the stream
+// kernel, whose warps load the operands of mma.sync straight from global memory.  Entries of more rows are bound by the
+// products: the tile kernel, on the tensor cores' accumulators in TMEM.  All groups of a call go to one of the two, and
+// all sequences; so a call is one or two launches and the combining one.
 //
-// A CTA streams its units' pages through a ring of page slots (one producer warp, bulk copies); eight consumer warps
-// split a page by row tiles of 16 and, when there are fewer than eight of these, by halves of the page and by pages.
+// Work of a kernel is one line of units: per entry, per item (kv head, and row tile in the tile kernel), its pages (tile
+// kernel: counted double for more than 128 rows).  The line is cut into equal shares, one per CTA (stream
+// kernel: per team of warps), so ragged lengths balance without any host knowledge of them.  A share's part of an item
+// is a segment, numbered by (item + share): both only grow along the line.
 #include <algorithm>
 #include <cfloat>
 
@@ -25,14 +26,16 @@ namespace clm {
 namespace {
 
 constexpr int kMaxEntries = kKvMaxGroups + kKvMaxSeqs;
-constexpr int kRowTile = 128;  // rows of an item: eight m16 tiles
-constexpr int kWarps = 8;      // consumer warps
+constexpr int kStreamRows = 64;  // entries of up to this many rows per kv head: the stream kernel
+constexpr int kStreamWarps = 8;  // warps of a stream CTA
+constexpr int kRowTile = 256;    // rows of an item of the tile kernel: two tiles of 128
 constexpr int kSegPad = 4;     // floats after a partial row's hd outputs: m, l, padding to 16 bytes
 
 struct Plan {
-  long long cum[kMaxEntries + 1];  // work units before entry e
-  int pages[kMaxEntries];          // pages of an item of entry e
-  int entries;
+  uint32_t cum[kMaxEntries + 1];  // work units before entry e (below 2^31, checked by the host)
+  int pages[kMaxEntries];         // pages of an item of entry e
+  uint32_t shares, q, r;          // how the line is cut (below)
+  __device__ __forceinline__ struct Shares cut() const;
 };
 
 struct Args {
@@ -44,37 +47,38 @@ struct Args {
   const int32_t* parent;
   int positions, nh, nkv, group;
   float scale_log2;
-  Plan* plan;
-  float* part_g;  // segments of group items: [group items + CTAs][kRowTile][hd + kSegPad]
-  float* part_s;  // segments of sequence items: [sequence items + CTAs][rows_s][hd + kSegPad]
-  int rows_s;     // row capacity of a sequence item (16, 32, 64 or 128)
-  int tiles_s;    // row tiles of a sequence
+  // partials of groups [0] and sequences [1]: segment x rows (tile kernel: 2 x 128, or 2 x rows, one half per stream)
+  struct Kind {
+    Plan* plan;     // of the kernel that has this kind
+    float* part;    // [segments][rows][hd + kSegPad]
+    int rows;       // row capacity of a segment, tile kernel: of half of one
+    int tiles;      // row tiles of an item (sequences)
+    int tile;       // 1: the tile kernel, 0: the stream kernel
+  } kind[2];
 };
-
-__host__ __device__ inline int tile_mt(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 
 // What entry e covers: groups first, then sequences.
 struct Entry {
-  int s0, s1;      // sequences
-  int rows;        // rows per kv head
-  int tiles;       // row tiles per kv head
-  int first_page;  // first table entry
+  int s0, s1;  // sequences
+  int kind;    // 0: group, 1: sequence
+  int rows;    // rows per kv head
+  int tiles;   // row tiles per kv head
+  int weight;  // work units of a page
 };
 __device__ __forceinline__ Entry entry_of(const Args& a, int e) {
   Entry r;
-  if (e < a.groups.n) {
+  r.kind = e >= a.groups.n;
+  if (r.kind == 0) {
     r.s0 = a.groups.start[e];
     r.s1 = a.groups.start[e + 1];
-    r.first_page = 0;
-    r.rows = (r.s1 - r.s0) * a.positions * a.group;
-    r.tiles = (r.rows + kRowTile - 1) / kRowTile;
   } else {
     r.s0 = e - a.groups.n;
     r.s1 = r.s0 + 1;
-    r.rows = a.positions * a.group;
-    r.tiles = a.tiles_s;
-    r.first_page = 0;
   }
+  r.rows = (r.s1 - r.s0) * a.positions * a.group;
+  const bool tile = a.kind[r.kind].tile;
+  r.tiles = tile ? (r.rows + kRowTile - 1) / kRowTile : 1;
+  r.weight = tile && r.rows > 128 ? 2 : 1;
   return r;
 }
 
@@ -99,46 +103,52 @@ __device__ __forceinline__ int shared_pages(const Args& a, int b) {
 
 // Items before entry e, within its kind (groups, sequences).
 __device__ __forceinline__ int items_before(const Args& a, int e) {
-  if (e >= a.groups.n) return (e - a.groups.n) * a.tiles_s * a.nkv;
+  if (e >= a.groups.n) return (e - a.groups.n) * a.kind[1].tiles * a.nkv;
+  if (!a.kind[0].tile) return e * a.nkv;
   int n = 0;
   for (int g = 0; g < e; ++g)
     n += ((a.groups.start[g + 1] - a.groups.start[g]) * a.positions * a.group + kRowTile - 1) / kRowTile * a.nkv;
   return n;
 }
 
-// The CTA whose share [c W / C, (c + 1) W / C) holds unit w.
-__device__ __forceinline__ int cta_of(long long w, long long W, int C) {
-  return (int)(((w + 1) * C + W - 1) / W) - 1;
-}
+// W units in C shares of q or q + 1: the first r have one more.
+struct Shares {
+  uint32_t C, q, r;
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * q + min(c, r); }
+  __device__ __forceinline__ uint32_t of(uint32_t w) const {  // the share that holds unit w
+    const uint32_t wide = r * (q + 1);
+    return w < wide ? w / (q + 1) : r + (w - wide) / q;
+  }
+};
 
-// Fills `plan` from the device-side positions: pages per item, then the running work of the entries.
-__device__ void make_plan(const Args& a, Plan* plan) {
+__device__ __forceinline__ Shares Plan::cut() const { return Shares{shares, q, r}; }
+
+// Fills the plan of the tile (or stream) kernel from the device-side positions: pages per item, then the running work of
+// its entries (the other kernel's have none).
+__device__ void make_plan(const Args& a, Plan* plan, int tile, uint32_t shares) {
   const int E = a.groups.n + a.seqs.n;
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    long long pages = 0, items;
+    int pages = 0;
     const Entry en = entry_of(a, e);
-    items = (long long)en.tiles * a.nkv;
     if (e < a.groups.n) {
       pages = min((int)a.groups.pages[e], a.seqs.max_pages);
     } else {
       const long long base = a.seqs.base(en.s0);
-      if (base >= 0) {
-        pages = (base + a.positions + kPageTokens - 1) / kPageTokens;
-        pages = min(pages, (long long)a.seqs.max_pages) - shared_pages(a, en.s0);
-        if (pages < 0) pages = 0;
-      }
+      if (base >= 0)
+        pages = max(0, (int)min((base + a.positions + kPageTokens - 1) / kPageTokens, (long long)a.seqs.max_pages) -
+                           shared_pages(a, en.s0));
     }
-    plan->pages[e] = (int)pages;
-    plan->cum[e + 1] = pages * items;
+    plan->pages[e] = pages;
+    plan->cum[e + 1] = a.kind[en.kind].tile == tile ? (uint32_t)pages * (uint32_t)(en.weight * en.tiles * a.nkv) : 0u;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
-    long long run = 0;
+    uint32_t run = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + threadIdx.x;
-      long long x = e < E ? plan->cum[e + 1] : 0;
+      uint32_t x = e < E ? plan->cum[e + 1] : 0;
       for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, x, d);
+        const uint32_t o = __shfl_up_sync(0xffffffffu, x, d);
         if ((int)threadIdx.x >= d) x += o;
       }
       if (e < E) plan->cum[e + 1] = run + x;
@@ -146,12 +156,699 @@ __device__ void make_plan(const Args& a, Plan* plan) {
     }
     if (threadIdx.x == 0) {
       plan->cum[0] = 0;
-      plan->entries = E;
+      plan->shares = min(shares, run);  // every share holds a unit
+      plan->q = run ? run / plan->shares : 0u;
+      plan->r = run ? run % plan->shares : 0u;
     }
   }
   __syncthreads();
 }
 
+// The combining kernel's copy of the plan.
+__device__ __forceinline__ void publish(const Args& a, const Plan& plan, int tile) {
+  Plan* to = a.kind[1].tile == tile ? a.kind[1].plan : a.kind[0].plan;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < (int)(sizeof(Plan) / 4); i += blockDim.x)
+      reinterpret_cast<int*>(to)[i] = reinterpret_cast<const int*>(&plan)[i];
+}
+
+// Ancestor sets of the tree's nodes, eight words each (an entry that is not an earlier node ends a chain).
+__device__ __forceinline__ void make_ancestors(const Args& a, uint32_t* anc) {
+  for (int i = threadIdx.x; i < a.positions; i += blockDim.x) {
+    uint32_t* bits = anc + 8 * i;
+    for (int w = 0; w < 8; ++w) bits[w] = 0;
+    for (int at = i;;) {
+      bits[at >> 5] |= 1u << (at & 31);
+      const int up = a.parent[at];
+      if (up < 0 || up >= at) break;
+      at = up;
+    }
+  }
+}
+
+// Pairs of 16-bit values with an all-ones exponent (infinities, NaN): the exponent's mask.
+template <typename T>
+constexpr uint32_t kExpMask = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+template <typename T>
+__device__ __forceinline__ bool has_nonfinite(uint32_t w) {
+  return (w & kExpMask<T>) == kExpMask<T> || ((w >> 16) & kExpMask<T>) == kExpMask<T>;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {  // 0xffff at each non-finite half
+  return ((w & kExpMask<T>) == kExpMask<T> ? 0xffffu : 0u) |
+         (((w >> 16) & kExpMask<T>) == kExpMask<T> ? 0xffff0000u : 0u);
+}
+
+// ---- tensor-core primitives (kind::f16: f16 or bf16 operands, f32 accumulators in TMEM)
+// K-major operand tiles with the 128-byte swizzle: rows of 64 elements, 8-row atoms of 1024 bytes, 16-byte chunk c of
+// row r at chunk c ^ (r % 8).
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) { return (uint32_t)row * 128u + (uint32_t)((chunk ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
+         (uint64_t)2u << 61;
+}
+template <typename T>
+__device__ constexpr uint32_t instr_desc(int n) {  // M = 128, N = n, A and B of type T, f32 result
+  return (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_smem_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 consecutive 32-bit columns of the thread's TMEM lane (complete after tc_wait_ld / tc_wait_st).
+__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+
+// 2^x (ex2.approx: 2 ulp; results below 2^-126 are 0)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// pairs of f32 (one instruction for two operations)
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float top_of(const uint32_t* x) {  // of 32 scores
+  float m[2] = {__uint_as_float(x[0]), __uint_as_float(x[1])};
+#pragma unroll
+  for (int j = 2; j < 32; j += 2) m[j / 2 % 2] = max3(m[j / 2 % 2], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+  return max3(m[0], m[1], m[1]);
+}
+
+// The weights 2^(scale x - ref) of 32 finite (or -inf) scores, as 16 columns of P, and their sum.  The special-function
+// unit makes 16 a clock, fewer than the tensor cores want: every fourth pair is computed instead, 2^y = 2^n 2^f with
+// n = round(y), |f| <= 1/2 and a degree-4 polynomial for 2^f (least maximum relative error by weighted least squares:
+// 2.7e-6, 0.6% of a weight's rounding to f16).  y is held at -125 from below: 2^-125 rounds to zero against a sum
+// of 2^-8 or more.
+template <typename T>
+__device__ __forceinline__ void weigh(const uint32_t* x, uint64_t scale2, uint64_t nref2, uint64_t (&sum)[2], uint32_t at) {
+  const float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits
+  const uint64_t magic = pair2(kMagic, kMagic), minus = pair2(-kMagic, -kMagic), neg = pair2(-1.0f, -1.0f);
+  const uint64_t c4 = pair2(0.009570102f, 0.009570102f), c3 = pair2(0.05591786f, 0.05591786f),
+                 c2 = pair2(0.24024744f, 0.24024744f), c1 = pair2(0.6931218f, 0.6931218f),
+                 c0 = pair2(0.9999993f, 0.9999993f);
+  uint32_t p[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    uint64_t y = fma2(pair2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), scale2, nref2);
+    float2 v = split2(y);
+    float2 e;
+    if (j % 4 != 3) {
+      e = make_float2(ex2(v.x), ex2(v.y));
+    } else {
+      y = pair2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
+      const uint64_t r = add2(y, magic);
+      const uint64_t f = fma2(add2(r, minus), neg, y);
+      uint64_t q = fma2(f, c4, c3);
+      q = fma2(q, f, c2);
+      q = fma2(q, f, c1);
+      q = fma2(q, f, c0);
+      const float2 n = split2(r), b = split2(q);
+      e = make_float2(__uint_as_float(__float_as_uint(b.x) + (__float_as_uint(n.x) << 23)),
+                      __uint_as_float(__float_as_uint(b.y) + (__float_as_uint(n.y) << 23)));
+    }
+    sum[j % 2] = add2(sum[j % 2], pair2(e.x, e.y));
+    p[j] = pack2<T>(e.x, e.y);
+  }
+  tc_st16(at, p);
+}
+
+// 16 bytes from global to shared memory, or 16 zero bytes
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+// arrives on the barrier once the thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+template <int HD>
+struct Tile {
+  static constexpr int kSlots = HD == 128 ? 4 : 8;         // page slots of the ring
+  static constexpr uint32_t kHalf = kPageTokens * HD * 2;  // bytes of K, or V, of a page and kv head
+  static constexpr uint32_t kQ = 128 * HD * 2;             // bytes of a query tile
+  static constexpr int kRow = HD + kSegPad;
+  static constexpr size_t kSmem = 2 * (size_t)kQ + (size_t)kSlots * 2 * kHalf;
+};
+
+constexpr int kSoftWarps = 4;  // softmax warps of a stream of the tile kernel
+constexpr int kProducers = 32;                                  // threads of the producer warp
+constexpr int kThreads = 2 * 32 * kSoftWarps + 2 * 32 + kProducers + 32;
+constexpr int kFlagRing = 16;  // flags of the last pages (the producer is at most kSlots + 1 pages ahead)
+
+// What window row i sees of its window: with ancestor sets (bits in shared memory) those, else rows 0..i.
+struct Window {
+  const uint32_t* anc;  // [positions][8], or null
+  int positions;
+  __device__ __forceinline__ bool sees(int i, int j) const {
+    return j < positions && (anc ? (anc[8 * i + (j >> 5)] >> (j & 31)) & 1u : j <= i);
+  }
+  // bits of the 32 positions from `at` = position - base on (negative ones are committed: seen)
+  __device__ __forceinline__ uint32_t word(int i, long long at) const {
+    if (at <= -32) return 0xffffffffu;
+    if (anc == nullptr) return at > i ? 0u : i - at >= 31 ? 0xffffffffu : (2u << (int)(i - at)) - 1u;
+    if (at >= 256) return 0u;
+    const int k = (int)at;
+    if (k < 0) return ((1u << -k) - 1u) | anc[8 * i] << -k;
+    const uint32_t lo = anc[8 * i + k / 32], hi = k / 32 < 7 ? anc[8 * i + k / 32 + 1] : 0u;
+    return __funnelshift_r(lo, hi, k % 32);
+  }
+};
+
+// A CTA's part of an item.
+struct Segment {
+  int item, kvh, x0, rows;   // item among its kind; kv head, first row, rows (<= kRowTile)
+  bool group, pair;          // group entry; more than 128 rows
+  int s0;                    // its (first) sequence
+  int page0, pages;          // table entry of the first page, pages
+  int streams;               // streams with work
+  __device__ __forceinline__ int stream_pages(int s) const { return pair ? pages : (pages + 1 - s) / 2; }
+  __device__ __forceinline__ int stream_rows(int s) const { return pair ? (s ? rows - 128 : 128) : rows; }
+};
+
+// The CTA's segments in order: pages whose first unit lies in its share.
+struct Walk {
+  const Args& a;
+  const Plan& plan;
+  uint32_t w, end;
+  int e;
+  __device__ __forceinline__ Walk(const Args& args, const Plan& p, uint32_t begin, uint32_t finish)
+      : a(args), plan(p), w(begin), end(finish), e(0) {
+    int lo = 0, hi = args.groups.n + args.seqs.n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (plan.cum[mid] <= begin)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    e = lo;
+  }
+  __device__ __forceinline__ bool next(Segment& s) {
+    while (w < end) {
+      while (plan.cum[e + 1] <= w) ++e;
+      const Entry en = entry_of(a, e);
+      const uint32_t pages = plan.pages[e], wt = en.weight, units = pages * wt;
+      const uint32_t tile = (w - plan.cum[e]) / units, u0 = plan.cum[e] + tile * units;
+      const uint32_t b0 = (w - u0 + wt - 1) / wt, b1 = min(pages, (end - u0 + wt - 1) / wt);
+      w = min(u0 + units, end);
+      if (b0 >= b1) continue;
+      s.item = items_before(a, e) + (int)tile;
+      s.group = e < a.groups.n;
+      s.s0 = en.s0;
+      s.kvh = (int)tile / en.tiles;
+      s.x0 = (int)tile % en.tiles * kRowTile;
+      s.rows = min(en.rows - s.x0, kRowTile);
+      s.pair = s.rows > 128;
+      s.page0 = (s.group ? 0 : shared_pages(a, en.s0)) + (int)b0;
+      s.pages = (int)(b1 - b0);
+      s.streams = s.pair || s.pages > 1 ? 2 : 1;
+      return true;
+    }
+    return false;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------
+// tile kernel: entries of more than 64 rows per kv head
+//
+// Two streams of four softmax warps each own 128 rows, one thread a row: no reductions across lanes.  With more than 128
+// rows the streams take a row tile each of every page; with fewer they take alternate pages of the same rows and give
+// two partials.  A stream has two score buffers, so the scores of its next page are computed while it weighs this one's;
+// its weights go back to TMEM as the first operand of their product with V.  O is rescaled only when a row's maximum
+// grows by more than 2^8 (weights stay below 2^8, far inside the types' range); the first maximum of a segment sets
+// the reference.
+//
+// The producer warp copies the pages with 16-byte asynchronous copies, because the cache's chunk order is not the tensor
+// cores' (128-byte swizzle): each chunk goes straight to its place, where a bulk copy would need a reordering pass.
+// ---------------------------------------------------------------------------------------------------
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_constant__ Args a) {
+  using TL = Tile<HD>;
+  constexpr int SL = TL::kSlots;
+  extern __shared__ __align__(1024) uint8_t smem[];  // [2 query tiles][slots of [K block][V block]]
+  __shared__ Plan plan;
+  __shared__ __align__(8) uint64_t copied_k[SL], copied_v[SL], free_k[SL], free_v[SL];
+  __shared__ __align__(8) uint64_t full_k[2][SL], full_v[2][SL];  // by a stream's own count of pages
+  __shared__ __align__(8) uint64_t q_ready[2], drained[2];
+  // of a stream's even and odd pages (a stream is up to two pages ahead, so that one barrier's phases could be missed)
+  __shared__ __align__(8) uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
+  __shared__ int s_real[kFlagRing];  // the page exists
+  __shared__ uint32_t s_anc[kKvMaxWindow * 8];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_dead;  // a bounded wait gave up: the others give up too
+  __shared__ volatile int s_odd;   // a value that is not finite lay in a window
+  uint8_t* ring = smem + 2 * TL::kQ;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // warps: 2 x 4 softmax, then a product warp per stream, the producer and the relay
+  constexpr int kMma = 2 * kSoftWarps, kProducer = kMma + 2, kRelay = kMma + 3;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SL; ++s) {
+      mbar_init(&copied_k[s], kProducers + 1);  // and the page flags
+      mbar_init(&copied_v[s], kProducers);
+      mbar_init(&free_k[s], 2);  // both streams' products (of a block that one stream uses: the same one twice)
+      mbar_init(&free_v[s], 2);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_ready[s], kSoftWarps);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&s_full[s][k], 1);
+        mbar_init(&p_ready[s][k], kSoftWarps);
+        mbar_init(&o_done[s][k], 1);
+      }
+      mbar_init(&drained[s], 1);
+      for (int k = 0; k < SL; ++k) {
+        mbar_init(&full_k[s][k], 1);
+        mbar_init(&full_v[s][k], 1);
+      }
+    }
+    mbar_fence_init();
+    s_dead = (smem_addr(smem) & 1023u) != 0;  // the operand tiles' alignment
+    s_odd = 0;
+  }
+  griddep_wait();
+  griddep_launch();
+  make_plan(a, &plan, 1, gridDim.x);
+  if (a.parent != nullptr) make_ancestors(a, s_anc);
+  publish(a, plan, 1);
+  const Shares shares = plan.cut();
+  if (blockIdx.x >= shares.C) return;
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  // TMEM columns of stream s: two score buffers of 64 (a page each; its weights go over the first 32), then O at
+  // 256 s + 128
+  const uint32_t tmem = s_tmem;
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    const uint32_t addr = smem_addr(bar);
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+      uint32_t done;
+      asm volatile(
+          "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+          : "=r"(done)
+          : "r"(addr), "r"(parity)
+          : "memory");
+      if (done) return true;
+      if ((i & 255) == 255 && s_dead) return false;
+    }
+    s_dead = 1;
+    return false;
+  };
+
+  Walk walk(a, plan, shares.begin(blockIdx.x), shares.begin(blockIdx.x + 1));
+  Segment g;
+  if (warp == kRelay) {
+    // ---------------- relay: copies that have landed become visible to the tensor cores (the copies are generic writes;
+    // the fence would cost a product warp its time), for the streams that use the page ----------------
+    if (lane == 0) {
+      uint32_t idx = 0, count[2] = {0, 0};
+      bool ok = true;
+      while (ok && walk.next(g))
+        for (int b = 0; b < g.pages && ok; ++b, ++idx) {
+          const int slot = (int)(idx % SL);
+          const uint32_t phase = (idx / SL) & 1u;
+          const int s_begin = g.pair ? 0 : b % 2, s_end = g.pair ? 2 : s_begin + 1;
+          if (!(ok = wait(&copied_k[slot], phase))) break;
+          fence_smem_async();
+          for (int s = s_begin; s < s_end; ++s) mbar_arrive(&full_k[s][count[s] % SL]);
+          if (!(ok = wait(&copied_v[slot], phase))) break;
+          fence_smem_async();
+          for (int s = s_begin; s < s_end; ++s) mbar_arrive(&full_v[s][count[s]++ % SL]);
+        }
+    }
+    __syncwarp();
+  } else if (warp == kProducer) {
+    // ---------------- producer: K, then V, of every page; chunks go to their swizzled places ----------------
+    // K (or V) of a page is kCopies x 32 chunks of 16 bytes; the lane's i-th one is lane + 32 i.  Its place in the
+    // swizzled tile repeats: a K row (of HD / 8 chunks) keeps its chunk and moves kStep rows, a V row keeps its chunk
+    // and moves four rows.
+    constexpr int kCopies = kPageTokens * HD / 8 / 32;
+    constexpr int kStep = 32 / (HD / 8);
+    const int kr = lane / (HD / 8), kc = kv_k_chunk(lane % (HD / 8), kr);  // (a stored chunk's place: its own inverse)
+    const int vr = lane / 8, vc = kv_v_chunk(lane % 8, vr);
+    static_assert(kStep % 2 == 0, "rows of one parity: the chunk's place repeats");
+    auto k_at = [&](int i) { return (uint32_t)(kc / 8) * (kPageTokens * 128) + sw128(kr + kStep * i, kc % 8); };
+    auto v_at = [&](int i) { return sw128(vr + 4 * i, vc); };
+    uint32_t idx = 0;
+    bool ok = true;
+    while (ok && walk.next(g)) {
+      const int32_t* table = a.seqs.table(g.s0) + g.page0;
+      // positions at or after `base` are the window's (or nobody's): their values are checked
+      const long long base = g.group ? 0x7fffffffffffffffll : a.seqs.base(g.s0);
+      int32_t page = __ldg(table);
+      for (int b = 0; b < g.pages; ++b, ++idx) {
+        const int slot = (int)(idx % SL);
+        const uint32_t phase = (idx / SL) & 1u;
+        const bool real = page >= 0 && page < a.seqs.pool_pages;
+        const size_t off = ((size_t)(real ? page : 0) * a.nkv + g.kvh) * (size_t)TL::kHalf + 16 * lane;
+        if (b + 1 < g.pages) page = __ldg(table + b + 1);
+        uint8_t* kd = ring + (size_t)slot * 2 * TL::kHalf;
+        uint8_t* vd = kd + TL::kHalf;
+        const uint32_t ka = smem_addr(kd), va = smem_addr(vd);
+        if (!(ok = wait(&free_k[slot], phase ^ 1u))) break;
+        if (lane == 0) {
+          s_real[idx % kFlagRing] = real;
+          mbar_arrive(&copied_k[slot]);
+        }
+        const uint8_t* src = static_cast<const uint8_t*>(a.k) + off;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) cp_async16(ka + k_at(i), src + 512 * i, real);
+        cp_async_arrive(&copied_k[slot]);
+        if (!(ok = wait(&free_v[slot], phase ^ 1u))) break;
+        src = static_cast<const uint8_t*>(a.v) + off;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) cp_async16(va + v_at(i), src + 512 * i, real);
+        const long long first = (long long)(g.page0 + b) * kPageTokens;
+        if (first + kPageTokens <= base) {
+          cp_async_arrive(&copied_v[slot]);
+        } else {
+          // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  In a
+          // page with positions that some row does not see, such values (from `base` on) become zero here; those of
+          // window positions reach the rows that see them at the segment's end.
+          asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+          for (int i = 0; i < kCopies; ++i) {
+            uint4* at = reinterpret_cast<uint4*>(vd + v_at(i));
+            const uint4 x = *at;
+            if (!(has_nonfinite<T>(x.x) || has_nonfinite<T>(x.y) || has_nonfinite<T>(x.z) || has_nonfinite<T>(x.w))) continue;
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t m = nonfinite_mask<T>(w[k / 2]) & (k & 1 ? 0xffff0000u : 0xffffu);
+              const long long pos = first + 8 * vc + k;
+              if (m == 0 || pos < base) continue;
+              w[k / 2] &= ~m;
+              if (pos < base + a.positions) s_odd = 1;
+            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          mbar_arrive(&copied_v[slot]);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= kMma) {
+    // ---------------- products of stream s ----------------
+    const int s = warp - kMma;
+    if (lane == 0) {
+      const uint32_t qa = smem_addr(smem) + s * TL::kQ, ra = smem_addr(ring), t0 = tmem + 256 * s;
+      uint32_t idx0 = 0, segs = 0, done = 0, asked = 0;  // pages before the segment; the stream's segments, pages, scores
+      bool ok = true;
+      for (; ok && walk.next(g); idx0 += g.pages) {
+        if (s >= g.streams) continue;
+        const int step = g.pair ? 1 : 2;
+        auto release = [&](uint64_t* bar) {  // of a page that one stream uses: for both
+          tc_commit(bar);
+          if (!g.pair) tc_commit(bar);
+        };
+        auto scores = [&](int b) {  // S = Q K^T of page b, the stream's page `asked`
+          const int slot = (int)((idx0 + b) % SL);
+          if (!wait(&full_k[s][asked % SL], (asked / SL) & 1u)) return false;
+          tc_after();
+          const uint32_t k = ra + (uint32_t)slot * 2 * TL::kHalf;
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(t0 + 64 * (asked & 1u), tile_desc(qa + c * (128 * 128) + 32 * kk),
+                     tile_desc(k + c * (kPageTokens * 128) + 32 * kk), instr_desc<T>(kPageTokens), c + kk > 0);
+          tc_commit(&s_full[s][asked & 1u]);
+          release(&free_k[slot]);
+          ++asked;
+          return true;
+        };
+        int b = g.pair ? 0 : s;
+        ok = wait(&q_ready[s], segs++ & 1u) && scores(b) && (b + step >= g.pages || scores(b + step));
+        for (bool first = true; ok && b < g.pages; b += step, first = false, ++done) {
+          const int slot = (int)((idx0 + b) % SL);
+          if (!(ok = wait(&full_v[s][done % SL], (done / SL) & 1u) && wait(&p_ready[s][done & 1u], (done >> 1) & 1u))) break;
+          tc_after();
+          const uint32_t v = ra + (uint32_t)slot * 2 * TL::kHalf + TL::kHalf;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // O (+)= P V
+            mma_ts(t0 + 128, t0 + 64 * (done & 1u) + 8 * kk, tile_desc(v + 32 * kk), instr_desc<T>(HD), !first || kk > 0);
+          tc_commit(&o_done[s][done & 1u]);
+          release(&free_v[slot]);
+          if (b + 2 * step < g.pages) ok = scores(b + 2 * step);  // over the weights that these products read
+        }
+      }
+      if (!ok) {  // products may be in flight: the accumulators are freed after them
+        tc_commit(&drained[s]);
+        mbar_wait(&drained[s], 0, nullptr);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax: stream s, one thread per row ----------------
+    const int s = warp / kSoftWarps, r = threadIdx.x % 128;
+    const Window win{a.parent ? s_anc : nullptr, a.positions};
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4) * 32 << 16);
+    const uint32_t ts = lanes + 256 * s, to = ts + 128;
+    uint8_t* qs = smem + s * TL::kQ;
+    uint32_t idx0 = 0, done = 0;  // pages before the segment, pages of the stream
+    bool ok = true;
+    for (; walk.next(g); idx0 += g.pages) {
+      if (s >= g.streams) continue;
+      const int nrows = g.stream_rows(s), x = g.x0 + (g.pair ? 128 * s : 0) + r;
+      const bool work = (warp % 4) * 32 < nrows;  // the warp has a row
+      bool valid = r < nrows;
+      int i = 0;  // window row
+      long long base = 0;
+      if (work) {
+        const int srow = valid ? x / a.group : 0, head = g.kvh * a.group + (valid ? x % a.group : 0);
+        const int b = g.s0 + srow / a.positions;
+        i = srow % a.positions;
+        base = a.seqs.base(b);
+        valid = valid && base >= 0;
+        const uint4* q = reinterpret_cast<const uint4*>(
+            static_cast<const T*>(a.q) + ((long long)b * a.positions + i) * a.ld_q + (long long)head * HD);
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c)
+          *reinterpret_cast<uint4*>(qs + (c / 8) * (128 * 128) + sw128(r, c % 8)) =
+              valid ? __ldg(q + c) : make_uint4(0u, 0u, 0u, 0u);
+        fence_smem_async();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[s]);
+      float m = -INFINITY, l = 0.0f;  // m: the reference of the weights so far (scaled scores)
+      const int np = g.stream_pages(s);
+      for (int t = 0; t < np; ++t, ++done) {
+        ok = ok && wait(&s_full[s][done & 1u], (done >> 1) & 1u);
+        if (work && ok) {
+          tc_after();
+          const int b = g.pair ? t : 2 * t + s;
+          const long long first = (long long)(g.page0 + b) * kPageTokens;
+          const uint32_t tp = ts + 64 * (done & 1u);
+          uint32_t x[64];
+          tc_ld32(tp, x);
+          tc_ld32(tp + 32, x + 32);
+          const bool real = s_real[(idx0 + b) % kFlagRing];
+          // whether some row of the warp does not see all of the page
+          const bool masked = __any_sync(0xffffffffu, valid && (!real || first + kPageTokens > base));
+          tc_wait_ld();
+          if (masked)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t see = real ? win.word(i, first + 32 * w - base) : 0u;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((see >> j) & 1u)) x[32 * w + j] = __float_as_uint(-INFINITY);
+            }
+          const float top = max3(top_of(x), top_of(x + 32), -INFINITY) * a.scale_log2;
+          if (t == 0) {
+            m = top;
+          } else {
+            const bool grow = top > m + 8.0f;
+            if (__any_sync(0xffffffffu, grow)) {
+              // the products of the page before are the last to add to O
+              ok = wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
+              tc_after();
+              const float f = grow ? ex2(m - top) : 1.0f;  // 0 for a row that had seen nothing
+              if (grow) m = top;
+              l *= f;
+#pragma unroll 1
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tc_ld16(to + 16 * c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                tc_st16(to + 16 * c, o);
+              }
+            }
+          }
+          const float ref = m == -INFINITY ? 0.0f : m;
+          if (!masked && __all_sync(0xffffffffu, fabsf(top) <= FLT_MAX)) {
+            const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), nref2 = pair2(-ref, -ref);
+            uint64_t sum[2] = {0, 0};
+            weigh<T>(x, scale2, nref2, sum, tp);
+            weigh<T>(x + 32, scale2, nref2, sum, tp + 16);
+            const float2 y = split2(add2(sum[0], sum[1]));
+            l += y.x + y.y;
+          } else {  // masked pages, and rows with infinities or NaN: the exponential itself for every score
+            float sum = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t p[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float p0 = ex2(fmaf(__uint_as_float(x[32 * h + 2 * j]), a.scale_log2, -ref));
+                const float p1 = ex2(fmaf(__uint_as_float(x[32 * h + 2 * j + 1]), a.scale_log2, -ref));
+                sum += p0 + p1;
+                p[j] = pack2<T>(p0, p1);
+              }
+              tc_st16(tp + 16 * h, p);
+            }
+            l += sum;
+          }
+          tc_wait_st();
+          tc_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[s][done & 1u]);
+      }
+      // the stream's partial rows, once its last products are complete
+      ok = ok && wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
+      if (work) {
+        tc_after();
+        const int seg = g.item + (int)blockIdx.x;
+        const Args::Kind& kind = a.kind[g.group ? 0 : 1];
+        float* dst = kind.part + ((size_t)(2 * seg + s) * kind.rows + r) * TL::kRow;
+        const bool odd = s_odd && !g.group;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tc_ld32(to + 32 * c, o);
+          tc_wait_ld();
+          if (odd && valid)  // values that are not finite, of window positions of these pages that the row sees
+            for (int j = 0; j < a.positions; ++j) {
+              const long long pos = base + j, at = pos / kPageTokens - g.page0;
+              if (!win.sees(i, j) || at < 0 || at >= g.pages) continue;
+              const int32_t page = a.seqs.table(g.s0)[pos / kPageTokens];
+              if (page < 0 || page >= a.seqs.pool_pages) continue;
+              const int pp = (int)(pos % kPageTokens);
+#pragma unroll
+              for (int d = 0; d < 32; ++d) {
+                const int dim = 32 * c + d;
+                const float v = to_f32(static_cast<const T*>(a.v)[(((size_t)page * a.nkv + g.kvh) * HD + dim) * kPageTokens +
+                                                                  8 * kv_v_chunk(pp / 8, dim) + pp % 8]);
+                if (!(fabsf(v) <= FLT_MAX)) o[d] = __float_as_uint(NAN);
+              }
+            }
+          // through the warp's rows of the query tile (read for the last time), so that eight lanes write 128 bytes of a row
+          uint8_t* stage = qs + (warp % 4) * 32 * 128;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(stage + sw128(lane, j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          __syncwarp();
+          float* rows = dst - (size_t)lane * TL::kRow + 32 * c;
+          const int left = nrows - (warp % 4) * 32;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int rr = 4 * j + lane / 8;
+            if (rr < left)
+              *reinterpret_cast<uint4*>(rows + (size_t)rr * TL::kRow + 4 * (lane % 8)) =
+                  *reinterpret_cast<const uint4*>(stage + sw128(rr, lane % 8));
+          }
+          __syncwarp();
+        }
+        // a copy that never arrived: the rows say so
+        if (r < nrows) *reinterpret_cast<float2*>(dst + HD) = make_float2(m, ok ? l : NAN);
+        tc_before();
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMma) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// stream kernel: entries of up to 64 rows per kv head
+//
+// A team of TM warps (1, 2 or 4: a row tile of 16 each) takes a share of the line; the teams of a CTA, and the warps of
+// a team, share nothing: a warp reads its operands from global memory in the fragments' order (every K and V chunk is
+// used by one lane of a row tile; a team's further warps find it in the L1 cache), keeps its state in registers and
+// writes its own partial.  Eight warps a CTA, each with 8 to 16 KB of loads in flight, cover the memory's latency.
+//
+// Fragment mapping (mma m16n8k16, lane = 4 g + t): column n of S's n-tile jj is position 8 (n / 2) + 2 jj + n % 2 of the
+// half page, so a lane's scores are positions 8 t + 2 jj + {0, 1}; the weights of n-tiles 2 kk and 2 kk + 1 are then the A
+// fragment of P V's k-step kk, whose B fragment is the lane's one chunk of V (positions 8 t .. 8 t + 7).  The dims of a
+// score are summed in the lane's order of K chunks (any order, alike in Q and K).
+// ---------------------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
@@ -166,182 +863,65 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-// Pairs of 16-bit values with an all-ones exponent (infinities, NaN): the exponent's mask, and 1.0.
-template <typename T>
-constexpr uint32_t kExpMask = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
 template <typename T>
 constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x3C00u : 0x3F80u;
 
-template <typename T>
-__device__ __forceinline__ bool has_nonfinite(uint32_t w) {
-  return (w & kExpMask<T>) == kExpMask<T> || ((w >> 16) & kExpMask<T>) == kExpMask<T>;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {  // 0xffff at each non-finite half
-  return ((w & kExpMask<T>) == kExpMask<T> ? 0xffffu : 0u) |
-         (((w >> 16) & kExpMask<T>) == kExpMask<T> ? 0xffff0000u : 0u);
-}
-
-template <int HD>
-struct Tile {
-  static constexpr uint32_t kPage = kPageTokens * HD * 2;  // bytes of K, or V, of one page and kv head
-  static constexpr int kSlots = HD == 128 ? 4 : 8;
-  static constexpr int kRow = HD + kSegPad;
-  static constexpr size_t kSmem = (size_t)kSlots * 2 * kPage + (size_t)kWarps * 16 * kRow * sizeof(float);
-};
-
-__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(n) : "memory");
-}
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
-
-// Whether window row i sees window row j: j's bit in i's ancestor set, or the chain's j <= i.
-struct Window {
-  const uint32_t* anc;  // [positions][8] bits in shared memory, or null
-  int positions;
-  __device__ __forceinline__ bool sees(int i, long long j) const {
-    if (j >= positions) return false;
-    return anc ? (anc[8 * i + (int)(j >> 5)] >> (j & 31)) & 1u : j <= i;
-  }
-};
-
-template <typename T, int HD>
-__global__ void __launch_bounds__(32 * (kWarps + 1), 1) kv_attention_kernel(const __grid_constant__ Args a) {
-  using TL = Tile<HD>;
+template <typename T, int HD, int TM>
+__global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const __grid_constant__ Args a, int second) {
   constexpr int KW = HD / 32;  // 16-byte words of a K row per lane
-  extern __shared__ __align__(128) uint8_t at_smem[];
+  constexpr int kRow = HD + kSegPad;
   __shared__ Plan plan;
-  __shared__ __align__(8) uint64_t full[TL::kSlots], empty[TL::kSlots];
-  __shared__ int s_page[TL::kSlots];
   __shared__ uint32_t s_anc[kKvMaxWindow * 8];
-  float* parts = reinterpret_cast<float*>(at_smem + (size_t)TL::kSlots * 2 * TL::kPage);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < TL::kSlots; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kWarps);
-    }
-    mbar_fence_init();
-  }
-  griddep_wait();
+  // After the tile kernel this one starts early: what it reads was complete before the tile kernel let it start.  The
+  // combining kernel waits for this one alone, so this one waits for the tile kernel before it ends.
+  if (!second) griddep_wait();
   griddep_launch();
-  make_plan(a, &plan);
-  if (a.parent != nullptr) {  // ancestor sets of the tree's nodes
-    for (int i = threadIdx.x; i < a.positions; i += blockDim.x) {
-      uint32_t bits[8] = {};
-      for (int at = i;;) {
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-          if (w == at >> 5) bits[w] |= 1u << (at & 31);
-        const int up = a.parent[at];
-        if (up < 0 || up >= at) break;
-        at = up;
-      }
-#pragma unroll
-      for (int w = 0; w < 8; ++w) s_anc[8 * i + w] = bits[w];
-    }
+  make_plan(a, &plan, 0, gridDim.x * (kStreamWarps / TM));
+  if (a.parent != nullptr) {
+    make_ancestors(a, s_anc);
+    __syncthreads();
   }
-  if (blockIdx.x == 0)  // the combining kernel's copy
-    for (int i = threadIdx.x; i < (int)(sizeof(Plan) / 4); i += blockDim.x)
-      reinterpret_cast<int*>(a.plan)[i] = reinterpret_cast<const int*>(&plan)[i];
-  __syncthreads();
-  const int E = plan.entries;
-  const long long W = plan.cum[E];
-  const int C = (int)min((long long)gridDim.x, W);  // every share holds a unit
-  if ((int)blockIdx.x >= C) return;
-  const long long w_begin = (long long)blockIdx.x * W / C, w_end = (long long)(blockIdx.x + 1) * W / C;
-  int e = 0;  // the entry of the first unit
-  {
+  publish(a, plan, 0);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int E = a.groups.n + a.seqs.n;
+  const Shares shares = plan.cut();
+  // consecutive shares go to different SMs: short lines use all of them
+  const uint32_t share = (warp / TM) * gridDim.x + blockIdx.x;
+  const int j = warp % TM;  // row tile
+  const Window win{a.parent ? s_anc : nullptr, a.positions};
+  uint32_t w = 0, end = 0;
+  int e = 0;
+  if (share < shares.C) {
+    w = shares.begin(share);
+    end = shares.begin(share + 1);
     int lo = 0, hi = E - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (plan.cum[mid] <= w_begin)
+      if (plan.cum[mid] <= w)
         lo = mid;
       else
         hi = mid - 1;
     }
     e = lo;
   }
-
-  if (warp == kWarps) {
-    // ---------------- producer ----------------
-    int slot = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (long long w = w_begin; w < w_end && ok;) {
-      while (plan.cum[e + 1] <= w) ++e;
-      const Entry en = entry_of(a, e);
-      const int L = plan.pages[e];
-      const int tile = (int)((w - plan.cum[e]) / L), off = (int)((w - plan.cum[e]) % L);
-      const int np = (int)min((long long)(L - off), w_end - w);
-      const int kvh = tile / en.tiles;
-      const int first = (e < a.groups.n ? 0 : shared_pages(a, en.s0)) + off;
-      const int32_t* table = a.seqs.table(en.s0) + first;
-      for (int j0 = 0; j0 < np && ok; j0 += 32) {
-        const int32_t mine = j0 + lane < np ? __ldg(table + j0 + lane) : -1;
-        for (int j = 0; j < min(32, np - j0); ++j) {
-          const int32_t page = __shfl_sync(0xffffffffu, mine, j);
-          if (lane == 0) {
-            ok = mbar_wait(&empty[slot], phase ^ 1u, nullptr);
-            if (ok) {
-              const bool real = page >= 0 && page < a.seqs.pool_pages;
-              s_page[slot] = real;
-              if (real) {
-                uint8_t* dst = at_smem + (size_t)slot * 2 * TL::kPage;
-                const size_t src = ((size_t)page * a.nkv + kvh) * TL::kPage;
-                mbar_expect_tx(&full[slot], 2 * TL::kPage);
-                bulk_g2s(dst, static_cast<const uint8_t*>(a.k) + src, TL::kPage, &full[slot]);
-                bulk_g2s(dst + TL::kPage, static_cast<const uint8_t*>(a.v) + src, TL::kPage, &full[slot]);
-              } else {
-                mbar_arrive(&full[slot]);
-              }
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          if (++slot == TL::kSlots) {
-            slot = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-      w += np;
-    }
-    return;
-  }
-
-  // ---------------- consumers ----------------
-  const int g = lane / 4, t = lane % 4;
-  const Window win{a.parent ? s_anc : nullptr, a.positions};
-  long long count = 0;  // pages of this CTA's stream so far: page i is in slot i % kSlots
-  bool failed = false;
-  for (long long w = w_begin; w < w_end;) {
+  while (w < end) {
     while (plan.cum[e + 1] <= w) ++e;
     const Entry en = entry_of(a, e);
-    const bool is_group = e < a.groups.n;
-    const int L = plan.pages[e];
-    const int tile = (int)((w - plan.cum[e]) / L), off = (int)((w - plan.cum[e]) % L);
-    const int np = (int)min((long long)(L - off), w_end - w);
-    const int kvh = tile / en.tiles, x0 = (tile % en.tiles) * kRowTile;
-    const int nrows = min(en.rows - x0, kRowTile);
-    const int mt = tile_mt(nrows);
-    const int first = (is_group ? 0 : shared_pages(a, en.s0)) + off;
-    // this warp: row tile j, half (or both) of the pages of its turn
-    const int j = warp % mt, kp = warp / mt;
-    const int turns = mt == 1 ? 4 : mt == 2 ? 2 : 1, turn = mt <= 2 ? kp / 2 : 0;
-    const int h_begin = mt == 8 ? 0 : kp % 2, h_end = mt == 8 ? 2 : h_begin + 1;
-    const uint32_t arrivals = mt == 1 ? 4 : mt == 2 ? 2 : 1;
-
-    // rows r0 = 16 j + g and r0 + 8 of the tile: window row and head
+    const uint32_t L = plan.pages[e];
+    const uint32_t kvh = (w - plan.cum[e]) / L, off = w - plan.cum[e] - kvh * L;
+    const int np = (int)min(L - off, end - w);
+    w += np;
+    if (16 * j >= en.rows) continue;
+    const int first = (en.kind == 0 ? 0 : shared_pages(a, en.s0)) + (int)off;
+    const int32_t* table = a.seqs.table(en.s0) + first;
+    // rows r0 = 16 j + g and r0 + 8: window row and head
     int i0, i1;
     long long b0, b1;
     bool v0, v1;
     uint4 qw0[KW], qw1[KW];
     auto row = [&](int r, int& i, long long& base, bool& valid, uint4(&qw)[KW]) {
-      const int x = x0 + r;
-      valid = r < nrows;
-      const int srow = valid ? x / a.group : 0, head = kvh * a.group + (valid ? x % a.group : 0);
+      valid = r < en.rows;
+      const int srow = valid ? r / a.group : 0, head = (int)kvh * a.group + (valid ? r % a.group : 0);
       const int b = en.s0 + srow / a.positions;
       i = srow % a.positions;
       base = a.seqs.base(b);
@@ -361,61 +941,66 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 1) kv_attention_kernel(cons
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.0f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-
-    for (int pj = 0; pj < np; ++pj, ++count) {
-      if (turns > 1 && (pj & (turns - 1)) != turn) continue;
-      const int slot = (int)(count % TL::kSlots);
-      const bool arrived = !failed && mbar_wait(&full[slot], (uint32_t)(count / TL::kSlots) & 1u, nullptr);
-      failed = !arrived;
-      if (arrived && s_page[slot]) {
-        const T* ks = reinterpret_cast<const T*>(at_smem + (size_t)slot * 2 * TL::kPage);
-        const T* vs = ks + kPageTokens * HD;
-        const long long p_begin = (long long)(first + pj) * kPageTokens;
-        // every position visible to every valid row of the warp's tile (a row of no sequence sees nothing)
-        const bool plain = __all_sync(0xffffffffu, (!v0 || p_begin + kPageTokens <= b0) && (!v1 || p_begin + kPageTokens <= b1));
-        for (int half = h_begin; half < h_end; ++half) {
-          float S[4][4];
+    int32_t page = __ldg(table);
+    for (int pj = 0; pj < np; ++pj) {
+      const int32_t now = page;
+      if (pj + 1 < np) page = __ldg(table + pj + 1);
+      if (now < 0 || now >= a.seqs.pool_pages) continue;
+      const size_t at = ((size_t)now * a.nkv + kvh) * (size_t)(kPageTokens * HD);
+      const T* ks = static_cast<const T*>(a.k) + at;
+      const T* vs = static_cast<const T*>(a.v) + at;
+      const long long p_begin = (long long)(first + pj) * kPageTokens;
+      // every position visible to every valid row of the tile
+      const bool plain = __all_sync(0xffffffffu, (!v0 || p_begin + kPageTokens <= b0) && (!v1 || p_begin + kPageTokens <= b1));
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        uint4 kw[4][KW], va[HD / 8];
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            S[jj][0] = S[jj][1] = S[jj][2] = S[jj][3] = 0.0f;
-            const int pos = 32 * half + 8 * (g / 2) + 2 * jj + (g % 2);
-            const uint4* kr = reinterpret_cast<const uint4*>(ks + (size_t)pos * HD);
-            uint4 kw[KW];
+        for (int jj = 0; jj < 4; ++jj) {
+          const int pos = 32 * half + 8 * (g / 2) + 2 * jj + (g % 2);
+          const uint4* kr = reinterpret_cast<const uint4*>(ks + (size_t)pos * HD);
 #pragma unroll
-            for (int u = 0; u < KW; ++u) kw[u] = kr[kv_k_chunk(KW * t + u, pos)];
+          for (int u = 0; u < KW; ++u) kw[jj][u] = __ldg(kr + kv_k_chunk(KW * t + u, pos));
+        }
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              mma16<T>(S[jj], word(qw0, 2 * kk), word(qw1, 2 * kk), word(qw0, 2 * kk + 1), word(qw1, 2 * kk + 1),
-                       word(kw, 2 * kk), word(kw, 2 * kk + 1));
+        for (int n = 0; n < HD / 8; ++n) {
+          const int vrow = 8 * n + g;
+          va[n] = __ldg(reinterpret_cast<const uint4*>(vs + (size_t)vrow * kPageTokens) + kv_v_chunk(4 * half + t, vrow));
+        }
+        float S[4][4];
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          S[jj][0] = S[jj][1] = S[jj][2] = S[jj][3] = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            mma16<T>(S[jj], word(qw0, 2 * kk), word(qw1, 2 * kk), word(qw0, 2 * kk + 1), word(qw1, 2 * kk + 1),
+                     word(kw[jj], 2 * kk), word(kw[jj], 2 * kk + 1));
+        }
+        // bit x of a row's word: it sees position 8 t + x of the half page
+        uint32_t see0 = v0 ? 0xffu : 0u, see1 = v1 ? 0xffu : 0u;
+        if (!plain) {
+          if (v0) see0 = (win.word(i0, p_begin + 32 * half - b0) >> (8 * t)) & 0xffu;
+          if (v1) see1 = (win.word(i1, p_begin + 32 * half - b1) >> (8 * t)) & 0xffu;
+        }
+        float mx0 = m0, mx1 = m1;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            S[jj][x] = (see0 >> (2 * jj + x)) & 1u ? S[jj][x] * a.scale_log2 : -INFINITY;
+            S[jj][2 + x] = (see1 >> (2 * jj + x)) & 1u ? S[jj][2 + x] * a.scale_log2 : -INFINITY;
+            mx0 = fmaxf(mx0, S[jj][x]);
+            mx1 = fmaxf(mx1, S[jj][2 + x]);
           }
-          uint32_t see = 0;  // masked pages: bit 4 jj + e of the positions a row sees
-          float mx0 = m0, mx1 = m1;
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              bool s0 = v0, s1 = v1;
-              if (!plain) {
-                const long long pos = p_begin + 32 * half + 8 * t + 2 * jj + x;
-                s0 = v0 && (pos < b0 || win.sees(i0, pos - b0));
-                s1 = v1 && (pos < b1 || win.sees(i1, pos - b1));
-                see |= (s0 ? 1u : 0u) << (4 * jj + x) | (s1 ? 1u : 0u) << (4 * jj + 2 + x);
-              }
-              S[jj][x] = s0 ? S[jj][x] * a.scale_log2 : -INFINITY;
-              S[jj][2 + x] = s1 ? S[jj][2 + x] * a.scale_log2 : -INFINITY;
-              mx0 = fmaxf(mx0, S[jj][x]);
-              mx1 = fmaxf(mx1, S[jj][2 + x]);
-            }
-#pragma unroll
-          for (int o = 1; o <= 2; o <<= 1) {
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
-          }
-          // a row that has seen nothing yet keeps m = -inf: its terms are exp2(-inf) through a zero reference
-          const float r0 = mx0 == -INFINITY ? 0.0f : mx0, r1 = mx1 == -INFINITY ? 0.0f : mx1;
-          const float c0 = exp2f(m0 - r0), c1 = exp2f(m1 - r1);
-          m0 = mx0;
-          m1 = mx1;
+        for (int o = 1; o <= 2; o <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+        }
+        // a row that has seen nothing yet keeps m = -inf: its terms are 2^-inf through a zero reference
+        const float r0 = mx0 == -INFINITY ? 0.0f : mx0, r1 = mx1 == -INFINITY ? 0.0f : mx1;
+        if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
+          const float c0 = ex2(m0 - r0), c1 = ex2(m1 - r1);
           l0 *= c0;
           l1 *= c1;
 #pragma unroll
@@ -425,150 +1010,179 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 1) kv_attention_kernel(cons
             O[n][2] *= c1;
             O[n][3] *= c1;
           }
-          uint32_t pa[4][2];
+        }
+        m0 = mx0;
+        m1 = mx1;
+        uint32_t pa[4][2];
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            const float p00 = exp2f(S[jj][0] - r0), p01 = exp2f(S[jj][1] - r0);
-            const float p10 = exp2f(S[jj][2] - r1), p11 = exp2f(S[jj][3] - r1);
-            l0 += p00 + p01;  // this lane's positions; the quad's lanes add up at the end of the segment
-            l1 += p10 + p11;
-            pa[jj][0] = pack2<T>(p00, p01);
-            pa[jj][1] = pack2<T>(p10, p11);
-          }
+        for (int jj = 0; jj < 4; ++jj) {
+          const float p00 = ex2(S[jj][0] - r0), p01 = ex2(S[jj][1] - r0);
+          const float p10 = ex2(S[jj][2] - r1), p11 = ex2(S[jj][3] - r1);
+          l0 += p00 + p01;  // this lane's positions; the quad's lanes add up at the end of the segment
+          l1 += p10 + p11;
+          pa[jj][0] = pack2<T>(p00, p01);
+          pa[jj][1] = pack2<T>(p10, p11);
+        }
+        if (!plain) {
+          // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  Such values
+          // are replaced by zero, and a second product of indicators finds the outputs they reach.
+          bool odd = false;
 #pragma unroll
-          for (int n = 0; n < HD / 8; ++n) {
-            const int vrow = 8 * n + g;
-            uint4 va = reinterpret_cast<const uint4*>(vs + (size_t)vrow * kPageTokens)[kv_v_chunk(4 * half + t, vrow)];
-            if (!plain) {
-              // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  Such
-              // values are replaced by zero, and a second product of indicators finds the outputs they reach.
-              const bool odd = has_nonfinite<T>(va.x) || has_nonfinite<T>(va.y) || has_nonfinite<T>(va.z) ||
-                               has_nonfinite<T>(va.w);
-              if (__any_sync(0xffffffffu, odd)) {
-                const uint32_t bx = nonfinite_mask<T>(va.x), by = nonfinite_mask<T>(va.y), bz = nonfinite_mask<T>(va.z),
-                               bw = nonfinite_mask<T>(va.w);
-                uint32_t in[4][2];
+          for (int n = 0; n < HD / 8; ++n)
+            odd |= has_nonfinite<T>(va[n].x) || has_nonfinite<T>(va[n].y) || has_nonfinite<T>(va[n].z) ||
+                   has_nonfinite<T>(va[n].w);
+          if (__any_sync(0xffffffffu, odd)) {
+            uint32_t in[4][2];
 #pragma unroll
-                for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-                  for (int r = 0; r < 2; ++r)
-                    in[jj][r] = ((see >> (4 * jj + 2 * r)) & 1u ? kOne<T> : 0u) |
-                                ((see >> (4 * jj + 2 * r + 1)) & 1u ? kOne<T> << 16 : 0u);
-                constexpr uint32_t one2 = kOne<T> | kOne<T> << 16;
-                float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma16<T>(hit, in[0][0], in[0][1], in[1][0], in[1][1], bx & one2, by & one2);
-                mma16<T>(hit, in[2][0], in[2][1], in[3][0], in[3][1], bz & one2, bw & one2);
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  if (hit[x] > 0.0f) O[n][x] = NAN;
-                va = make_uint4(va.x & ~bx, va.y & ~by, va.z & ~bz, va.w & ~bw);
-              }
+            for (int jj = 0; jj < 4; ++jj) {
+              in[jj][0] = ((see0 >> (2 * jj)) & 1u ? kOne<T> : 0u) | ((see0 >> (2 * jj + 1)) & 1u ? kOne<T> << 16 : 0u);
+              in[jj][1] = ((see1 >> (2 * jj)) & 1u ? kOne<T> : 0u) | ((see1 >> (2 * jj + 1)) & 1u ? kOne<T> << 16 : 0u);
             }
-            mma16<T>(O[n], pa[0][0], pa[0][1], pa[1][0], pa[1][1], va.x, va.y);
-            mma16<T>(O[n], pa[2][0], pa[2][1], pa[3][0], pa[3][1], va.z, va.w);
+            constexpr uint32_t one2 = kOne<T> | kOne<T> << 16;
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) {
+              const uint32_t bx = nonfinite_mask<T>(va[n].x), by = nonfinite_mask<T>(va[n].y),
+                             bz = nonfinite_mask<T>(va[n].z), bw = nonfinite_mask<T>(va[n].w);
+              float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma16<T>(hit, in[0][0], in[0][1], in[1][0], in[1][1], bx & one2, by & one2);
+              mma16<T>(hit, in[2][0], in[2][1], in[3][0], in[3][1], bz & one2, bw & one2);
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (hit[x] > 0.0f) O[n][x] = NAN;
+              va[n] = make_uint4(va[n].x & ~bx, va[n].y & ~by, va[n].z & ~bz, va[n].w & ~bw);
+            }
           }
         }
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          mma16<T>(O[n], pa[0][0], pa[0][1], pa[1][0], pa[1][1], va[n].x, va[n].y);
+          mma16<T>(O[n], pa[2][0], pa[2][1], pa[3][0], pa[3][1], va[n].z, va[n].w);
+        }
       }
-      __syncwarp();
-      if (lane == 0 && arrived) mbar_arrive_n(&empty[slot], arrivals);
     }
-    w += np;
-
-    // the warps that share a row tile fold their states; the segment's rows go to its partial
-    float* sp = parts + (size_t)warp * 16 * TL::kRow;
+    // the segment's partial rows
 #pragma unroll
     for (int o = 1; o <= 2; o <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, o);
       l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     }
-    if (failed) l0 = l1 = NAN;  // a copy never arrived: the rows say so
+    const Args::Kind& kind = a.kind[en.kind];
+    const int seg = items_before(a, e) + (int)kvh + (int)share;
+    float* dst = kind.part + ((size_t)seg * kind.rows + 16 * j + g) * kRow;
+    if (16 * j + g < en.rows) {
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n) {
-      *reinterpret_cast<float2*>(sp + g * TL::kRow + 8 * n + 2 * t) = make_float2(O[n][0], O[n][1]);
-      *reinterpret_cast<float2*>(sp + (g + 8) * TL::kRow + 8 * n + 2 * t) = make_float2(O[n][2], O[n][3]);
+      for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) = make_float2(O[n][0], O[n][1]);
+      if (t == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(m0, l0);
     }
-    if (t == 0) {
-      sp[g * TL::kRow + HD] = m0;
-      sp[g * TL::kRow + HD + 1] = l0;
-      sp[(g + 8) * TL::kRow + HD] = m1;
-      sp[(g + 8) * TL::kRow + HD + 1] = l1;
+    if (16 * j + g + 8 < en.rows) {
+      dst += 8 * kRow;
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) = make_float2(O[n][2], O[n][3]);
+      if (t == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(m1, l1);
     }
-    consumer_sync();
-    const int seg = items_before(a, e) + tile + (int)blockIdx.x;
-    float* dst = is_group ? a.part_g + (size_t)seg * kRowTile * TL::kRow : a.part_s + (size_t)seg * a.rows_s * TL::kRow;
-    constexpr int C4 = HD / 4;
-    for (int idx = threadIdx.x; idx < nrows * C4; idx += 32 * kWarps) {
-      const int r = idx / C4, c4 = idx % C4;
-      const float* src = parts + ((size_t)(r / 16) * 16 + r % 16) * TL::kRow;
-      const size_t step = (size_t)mt * 16 * TL::kRow;
-      float M = -INFINITY;
-      for (int k = 0; k < kWarps / mt; ++k) M = fmaxf(M, src[k * step + HD]);
-      const float R = M == -INFINITY ? 0.0f : M;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float l = 0.0f;
-      for (int k = 0; k < kWarps / mt; ++k) {
-        const float f = exp2f(src[k * step + HD] - R);
-        const float4 o = *reinterpret_cast<const float4*>(src + k * step + 4 * c4);
-        acc = make_float4(acc.x + o.x * f, acc.y + o.y * f, acc.z + o.z * f, acc.w + o.w * f);
-        l += src[k * step + HD + 1] * f;
-      }
-      *reinterpret_cast<float4*>(dst + (size_t)r * TL::kRow + 4 * c4) = acc;
-      if (c4 == 0) *reinterpret_cast<float2*>(dst + (size_t)r * TL::kRow + HD) = make_float2(M, l);
-    }
-    consumer_sync();
   }
+  if (second) griddep_wait();
 }
 
-// One warp per (row, head): the row's segments of its group's item and of its own, combined by their maxima.
+// One warp per (row, head): the row's partials of its group's item and of its own, combined by their maxima.  Lane k
+// looks up partial k (32 at a time) and its maximum and sum, then the lanes share the outputs' columns.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ Args a, int ctas) {
+__global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ Args a) {
   using TL = Tile<HD>;
   constexpr int N = HD / 32;  // outputs per lane
-  griddep_wait();
-  griddep_launch();
   const int lane = threadIdx.x % 32;
-  const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  if (id >= (long long)a.seqs.n * a.positions * a.nh) return;
+  const uint32_t id = blockIdx.x * 8 + threadIdx.x / 32;
+  if (id >= (uint32_t)(a.seqs.n * a.positions) * a.nh) return;
   const int head = (int)(id % a.nh), row = (int)(id / a.nh);
   const int b = row / a.positions, kvh = head / a.group;
-  const Plan* plan = a.plan;
-  const long long W = plan->cum[plan->entries];
-  const int C = (int)min((long long)ctas, W);
+  const int grp = group_of(a, b);
+  griddep_wait();
+  griddep_launch();
   const bool idle = a.seqs.base(b) < 0;
-  const int grp = idle ? -1 : group_of(a, b);
+  // the partials: those of the group's item, then those of the sequence's
+  struct Part {
+    Shares shares;
+    uint32_t u0, wt, pages, c0, n, per;  // first unit, units a page, pages, first share, partials, partials a share
+    int first;                            // stream of the row's partial where a share has one
+    const float* row;                     // the row in the partial of (share 0, stream 0)
+    uint32_t half;                        // rows between a segment's halves
+  };
+  auto find = [&](int k) {
+    const int e = k == 0 ? grp : a.groups.n + b;
+    const Args::Kind& kind = a.kind[k];
+    Part p{Shares{0, 1, 0}, 0, 1, 1, 0, 0, 1, 0, nullptr, 0};
+    if (e < 0 || idle) return p;
+    const uint32_t cum = kind.plan->cum[e];
+    const int pages = kind.plan->pages[e];
+    p.shares = kind.plan->cut();
+    if (pages == 0) return p;
+    const Entry en = entry_of(a, e);
+    const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
+    int tile = kvh, r = x;
+    p.pages = pages;
+    p.wt = en.weight;
+    uint32_t rows = kind.rows;  // of a segment
+    if (kind.tile) {
+      tile = kvh * en.tiles + x / kRowTile;
+      p.per = min(en.rows - x / kRowTile * kRowTile, kRowTile) > 128 ? 1 : 2;
+      p.first = p.per == 1 ? x % kRowTile / 128 : 0;
+      p.half = rows;
+      rows *= 2;
+      r = x % 128;
+    }
+    p.u0 = cum + tile * p.pages * p.wt;
+    p.c0 = p.shares.of(p.u0);
+    p.n = (p.shares.of(p.u0 + (p.pages - 1) * p.wt) - p.c0 + 1) * p.per;
+    p.row = kind.part + ((size_t)(items_before(a, e) + tile) * rows + r) * TL::kRow;
+    return p;
+  };
+  const Part part[2] = {find(0), find(1)};
+  const uint32_t total = part[0].n + part[1].n;
   float M = -INFINITY, l = 0.0f, acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const int e = part == 0 ? grp : a.groups.n + b;
-    if (e < 0 || idle) continue;
-    const int L = plan->pages[e];
-    if (L == 0) continue;
-    const Entry en = entry_of(a, e);
-    const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
-    const int tile = kvh * en.tiles + x / kRowTile, r = x % kRowTile;
-    const long long w = plan->cum[e] + (long long)tile * L;
-    const int c0 = cta_of(w, W, C), c1 = cta_of(w + L - 1, W, C);
-    const int item = items_before(a, e) + tile;
-    for (int c = c0; c <= c1; ++c) {
-      const float* src = part == 0 ? a.part_g + ((size_t)(item + c) * kRowTile + r) * TL::kRow
-                                   : a.part_s + ((size_t)(item + c) * a.rows_s + r) * TL::kRow;
-      const float2 ml = *reinterpret_cast<const float2*>(src + HD);
-      float o[N];
-      if constexpr (N == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(src + 4 * lane);
-        o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
-      } else {
-        const float2 f = *reinterpret_cast<const float2*>(src + 2 * lane);
-        o[0] = f.x, o[1] = f.y;
+  for (uint32_t k0 = 0; k0 < total; k0 += 32) {
+    const float* src = nullptr;  // this lane's partial
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (k0 + lane < total) {
+      const bool own = k0 + lane >= part[0].n;
+      const Part& p = own ? part[1] : part[0];
+      const Args::Kind& kind = a.kind[own ? 1 : 0];
+      const uint32_t k = own ? k0 + lane - part[0].n : k0 + lane;
+      const uint32_t c = p.c0 + k / p.per, s = p.per == 1 ? p.first : k % 2;
+      // pages of the item that share c holds (none, where it is narrower than a page's units; stream 1 of a tile
+      // that alternates: two or more)
+      const uint32_t w0 = max(p.shares.begin(c), p.u0) - p.u0, w1 = p.shares.begin(c + 1) - p.u0;
+      const uint32_t n = min(p.pages, (w1 + p.wt - 1) / p.wt) - min(p.pages, (w0 + p.wt - 1) / p.wt);
+      if (n > (p.per == 1 ? 0u : s)) {
+        src = p.row + ((size_t)c * (kind.tile ? 2 * p.half : (uint32_t)kind.rows) + s * p.half) * TL::kRow;
+        ml = *reinterpret_cast<const float2*>(src + HD);
       }
-      const float m = fmaxf(M, ml.x), R = m == -INFINITY ? 0.0f : m;
-      const float f0 = exp2f(M - R), f1 = exp2f(ml.x - R);
-      M = m;
-      l = l * f0 + ml.y * f1;
+    }
+    float m = fmaxf(M, ml.x);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const float keep = exp2f(M - ref), f = exp2f(ml.x - ref);
+    float add = ml.y * f;
+    for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+    M = m;
+    l = l * keep + add;
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = acc[i] * f0 + o[i] * f1;
+    for (int i = 0; i < N; ++i) acc[i] *= keep;
+    const uint32_t have = __ballot_sync(0xffffffffu, src != nullptr);
+    const int count = (int)min(32u, total - k0);
+#pragma unroll 4
+    for (int k = 0; k < count; ++k) {
+      const float* q = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k));
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      if (!((have >> k) & 1u)) continue;
+      if constexpr (N == 4) {
+        const float4 o = *reinterpret_cast<const float4*>(q + 4 * lane);
+        acc[0] += o.x * fk, acc[1] += o.y * fk, acc[2] += o.z * fk, acc[3] += o.w * fk;
+      } else {
+        const float2 o = *reinterpret_cast<const float2*>(q + 2 * lane);
+        acc[0] += o.x * fk, acc[1] += o.y * fk;
+      }
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -586,44 +1200,84 @@ __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__
 
 size_t al256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-struct Sizes {
-  int rows_s, tiles_s;
-  size_t plan, part_g, part_s;  // bytes
-  size_t total() const { return plan + part_g + part_s; }
+// How a call is laid out: which kernel takes the groups and which the sequences, and the workspace.
+struct Layout {
+  bool tile[2];     // groups, sequences: the tile kernel
+  int team[2];      // warps of a team of the stream kernel
+  int tiles;        // row tiles of a sequence
+  int rows[2];      // row capacity of a segment (tile kernel: of half of one)
+  int shares[2];
+  size_t items;     // of groups and sequences
+  size_t plan, part[2];  // bytes
+  size_t total() const { return 2 * plan + part[0] + part[1]; }
 };
 
-Sizes sizes_of(int n, int positions, int nh, int nkv, int hd, const KvGroups& groups, int sm_count) {
-  Sizes s;
-  const int group = nh / nkv, rows = positions * group;
-  s.rows_s = rows >= kRowTile ? kRowTile : 16 * tile_mt(rows);
-  s.tiles_s = (rows + kRowTile - 1) / kRowTile;
-  size_t items_g = 0;
+Layout layout_of(int n, int positions, int nh, int nkv, int hd, const KvGroups& groups, int sm_count) {
+  Layout s;
+  const int rows = positions * (nh / nkv);
+  int most = 0;  // rows of the largest group
+  bool any = false;
   for (int g = 0; g < groups.n; ++g)
-    items_g += (size_t)((groups.start[g + 1] - groups.start[g]) * rows + kRowTile - 1) / kRowTile * nkv;
-  const size_t items_s = (size_t)n * s.tiles_s * nkv, row = (size_t)(hd + kSegPad) * sizeof(float);
+    if (groups.pages[g] > 0) {
+      any = true;
+      most = std::max(most, (groups.start[g + 1] - groups.start[g]) * rows);
+    }
+  const int widest[2] = {most, rows};
+  s.tile[1] = rows > kStreamRows;
+  s.tile[0] = any ? most > kStreamRows : s.tile[1];  // without shared pages there is one kernel
+  auto team_of = [](int r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; };
+  s.team[1] = team_of(rows);
+  s.team[0] = any ? team_of(most) : s.team[1];
+  if (!s.tile[0] && !s.tile[1]) s.team[0] = s.team[1] = std::max(s.team[0], s.team[1]);  // one launch, one team size
+  s.tiles = s.tile[1] ? (rows + kRowTile - 1) / kRowTile : 1;
+  size_t items[2] = {0, (size_t)n * s.tiles * nkv};
+  for (int g = 0; g < groups.n; ++g)
+    items[0] += (s.tile[0] ? (size_t)((groups.start[g + 1] - groups.start[g]) * rows + kRowTile - 1) / kRowTile : 1) * nkv;
+  s.items = items[0] + items[1];
   s.plan = al256(sizeof(Plan));
-  s.part_g = groups.n ? al256((items_g + sm_count) * kRowTile * row) : 0;
-  s.part_s = al256((items_s + sm_count) * s.rows_s * row);
+  for (int k = 0; k < 2; ++k) {
+    s.rows[k] = s.tile[k] ? std::min(k ? rows : 128, 128) : std::max(1, widest[k]);
+    s.shares[k] = s.tile[k] ? sm_count : sm_count * kStreamWarps / s.team[k];
+    s.part[k] = k == 0 && !any ? 0
+                               : al256((items[k] + s.shares[k]) * (s.tile[k] ? 2 : 1) * s.rows[k] * (size_t)(hd + kSegPad) *
+                                       sizeof(float));
+  }
   return s;
 }
 
+template <typename T, int HD>
+int launch_stream(const Args& a, int team, bool second, int sm_count, cudaStream_t st) {
+  const dim3 grid((unsigned)sm_count), block(32 * kStreamWarps);
+  if (team == 1) return launch_pdl(kv_stream_kernel<T, HD, 1>, grid, block, 0, st, a, (int)second);
+  if (team == 2) return launch_pdl(kv_stream_kernel<T, HD, 2>, grid, block, 0, st, a, (int)second);
+  return launch_pdl(kv_stream_kernel<T, HD, 4>, grid, block, 0, st, a, (int)second);
+}
+
 template <typename T, typename O, int HD>
-int launch_typed(const Args& a, int sm_count, cudaStream_t st) {
+int launch_typed(const Args& a, const Layout& s, int sm_count, cudaStream_t st) {
   using TL = Tile<HD>;
-  CLM_TRY(ensure_smem(kv_attention_kernel<T, HD>, TL::kSmem));
-  CLM_TRY(launch_pdl(kv_attention_kernel<T, HD>, dim3((unsigned)sm_count), dim3(32 * (kWarps + 1)), TL::kSmem, st, a));
-  const long long rows = (long long)a.seqs.n * a.positions * a.nh;
-  return launch_pdl(kv_combine_kernel<O, HD>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, a, sm_count);
+  const bool tiled = s.tile[0] || s.tile[1];
+  if (tiled) {
+    CLM_TRY(ensure_smem(kv_tile_kernel<T, HD>, TL::kSmem));
+    CLM_TRY(launch_pdl(kv_tile_kernel<T, HD>, dim3((unsigned)sm_count), dim3(kThreads), TL::kSmem, st, a));
+  }
+  // (on the default streams launches do not overlap, and the second one need not wait)
+  if (!s.tile[0] || !s.tile[1])
+    CLM_TRY((launch_stream<T, HD>(a, s.team[s.tile[0] ? 1 : 0], tiled, sm_count, st)));
+  const uint64_t rows = (uint64_t)a.seqs.n * a.positions * a.nh;
+  return launch_pdl(kv_combine_kernel<O, HD>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
 size_t kv_attention_work(int n, int positions, int nh, int nkv, int hd, const KvGroups& groups, int sm_count) {
-  return sizes_of(n, positions, nh, nkv, hd, groups, sm_count).total();
+  return layout_of(n, positions, nh, nkv, hd, groups, sm_count).total();
 }
 
 int launch_kv_attention(const KvAttnArgs& in, cudaStream_t st) {
-  const Sizes s = sizes_of(in.seqs.n, in.positions, in.nh, in.nkv, in.hd, in.groups, in.sm_count);
+  const Layout s = layout_of(in.seqs.n, in.positions, in.nh, in.nkv, in.hd, in.groups, in.sm_count);
+  CLM_CHECK(s.items * (size_t)(in.seqs.max_pages + 2) < (1ull << 31), CLM_OUT_OF_RANGE,
+            "attention: too many pages in one call (narrower page tables, or fewer sequences)");
   CLM_CHECK(in.work != nullptr && in.work_bytes >= s.total(), CLM_RESOURCE_EXHAUSTED, "attention workspace too small");
   Args a;
   a.seqs = in.seqs;
@@ -638,23 +1292,26 @@ int launch_kv_attention(const KvAttnArgs& in, cudaStream_t st) {
   a.nh = in.nh;
   a.nkv = in.nkv;
   a.group = in.nh / in.nkv;
-  a.scale_log2 = in.scale * 1.4426950408889634f;
+  // (a zero scale weighs all positions alike: a product with a masked score of -inf must not become NaN)
+  a.scale_log2 = std::max(in.scale * 1.4426950408889634f, FLT_MIN);
   uint8_t* w = static_cast<uint8_t*>(in.work);
-  a.plan = reinterpret_cast<Plan*>(w);
-  a.part_g = reinterpret_cast<float*>(w + s.plan);
-  a.part_s = reinterpret_cast<float*>(w + s.plan + s.part_g);
-  a.rows_s = s.rows_s;
-  a.tiles_s = s.tiles_s;
+  for (int k = 0; k < 2; ++k) {
+    a.kind[k].plan = reinterpret_cast<Plan*>(w + (s.tile[k] ? 0 : s.plan));  // one plan per kernel
+    a.kind[k].part = reinterpret_cast<float*>(w + 2 * s.plan + (k ? s.part[0] : 0));
+    a.kind[k].rows = s.rows[k];
+    a.kind[k].tiles = s.tiles;
+    a.kind[k].tile = s.tile[k];
+  }
   const bool h = in.type == CLM_DTYPE_F16, f32 = in.out_type == CLM_DTYPE_F32;
   if (in.hd == 64) {
-    if (h) return f32 ? launch_typed<__half, float, 64>(a, in.sm_count, st) : launch_typed<__half, __half, 64>(a, in.sm_count, st);
-    return f32 ? launch_typed<__nv_bfloat16, float, 64>(a, in.sm_count, st)
-               : launch_typed<__nv_bfloat16, __nv_bfloat16, 64>(a, in.sm_count, st);
+    if (h) return f32 ? launch_typed<__half, float, 64>(a, s, in.sm_count, st) : launch_typed<__half, __half, 64>(a, s, in.sm_count, st);
+    return f32 ? launch_typed<__nv_bfloat16, float, 64>(a, s, in.sm_count, st)
+               : launch_typed<__nv_bfloat16, __nv_bfloat16, 64>(a, s, in.sm_count, st);
   }
   CLM_CHECK(in.hd == 128, CLM_UNIMPLEMENTED, "head_dim 64 or 128");
-  if (h) return f32 ? launch_typed<__half, float, 128>(a, in.sm_count, st) : launch_typed<__half, __half, 128>(a, in.sm_count, st);
-  return f32 ? launch_typed<__nv_bfloat16, float, 128>(a, in.sm_count, st)
-             : launch_typed<__nv_bfloat16, __nv_bfloat16, 128>(a, in.sm_count, st);
+  if (h) return f32 ? launch_typed<__half, float, 128>(a, s, in.sm_count, st) : launch_typed<__half, __half, 128>(a, s, in.sm_count, st);
+  return f32 ? launch_typed<__nv_bfloat16, float, 128>(a, s, in.sm_count, st)
+             : launch_typed<__nv_bfloat16, __nv_bfloat16, 128>(a, s, in.sm_count, st);
 }
 
 }  // namespace clm
@@ -714,6 +1371,7 @@ int clm_b200_kv_attention(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint3
   CLM_TRY(check_kv_pool(pool));
   CLM_TRY(check_kv_seqs(seqs));
   CLM_TRY(check_shape(n, positions, n_heads, pool->n_kv_heads, pool->head_dim));
+  CLM_CHECK(scale >= 0.0f && scale <= 1e30f, CLM_INVALID_ARGUMENT, "the scale must be a number that is not negative");
   CLM_CHECK(layer < pool->layers, CLM_OUT_OF_RANGE, "layer outside the pool");
   CLM_CHECK(n <= seqs->rows, CLM_OUT_OF_RANGE, "more sequences than page tables");
   KvAttnArgs a;

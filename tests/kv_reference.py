@@ -114,7 +114,7 @@ def attention(k_pool, v_pool, tables, pos, q, parents=None, scale=None):
             # the exponent's error: f32 sums of hd products (truncated adds count double), the scale's two roundings,
             # the exponential's own; every weight carries it, numerator and denominator
             size = (qq.abs() @ torch.nan_to_num(kk).abs().T * scale * seen).amax(1, keepdim=True)
-            delta = 2.0**-24 * (2 * hd + 16) * size + 2.0**-21
+            delta = 2.0**-24 * (2 * hd + 16) * size + 2.0**-18
             spread = torch.where(l > 0, w @ clean.abs() / l, 0.0)  # sum p |v| / l
             tiny = 2.0**-25 * clean.abs().sum(0) if q.dtype == torch.float16 else 0.0  # f16 weights below 2^-14
             bound[b, :, h] = spread * (half + 2 * delta + 2 * length * 2.0**-24) + tiny + half * o.abs() * 1.01 + 2.0**-25

@@ -185,13 +185,13 @@ def test_append_refuses(kw, code):
 
 
 def attention(ctx=CTX, p=None, layer=0, s=None, n=3, positions=2, heads=4, q=A, ld_q=512, groups=(), parents=0, out=A,
-              work=A, work_bytes=1 << 40, null_groups=False):
+              work=A, work_bytes=1 << 40, null_groups=False, scale=0.1):
     p, s = pool() if p is None else p, seqs() if s is None else s
     counts = (C.c_uint32 * 80)(*[g[0] for g in groups])
     pages = (C.c_uint32 * 80)(*[g[1] for g in groups])
     return _native.lib.clm_b200_kv_attention(ctx, C.byref(p), layer, C.byref(s), n, positions, heads, vp(q), ld_q,
                                              len(groups) or int(null_groups), None if null_groups else counts,
-                                             None if null_groups else pages, vp(parents), 0.1, vp(out), vp(work),
+                                             None if null_groups else pages, vp(parents), scale, vp(out), vp(work),
                                              work_bytes, None)
 
 
@@ -200,6 +200,7 @@ ATTENTION = [(dict(ctx=None), INVALID), (dict(layer=2), RANGE), (dict(n=5), RANG
              (dict(q=0), INVALID), (dict(out=0), INVALID), (dict(work=0), INVALID), (dict(ld_q=504), INVALID),
              (dict(ld_q=513), INVALID), (dict(q=A + 2), INVALID), (dict(out=A + 8), INVALID), (dict(work=A + 8), INVALID),
              (dict(groups=[(2, 1), (2, 1)]), INVALID), (dict(groups=[(0, 1)] * 65), RANGE),
+             (dict(scale=-0.1), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
              (dict(null_groups=True), INVALID), (dict(groups=[(2**32 - 1, 1), (2, 1)]), INVALID)]
 
 

@@ -230,6 +230,13 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                : "memory");
 }
+// One lane of the warp.  (The compiler knows that a single lane runs what this guards: the products' operands then need no
+// loop over lanes.  Guarded by a comparison of the lane's number an instruction took 95 clocks to issue.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_smem_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
   } else if (warp >= kMma) {
     // ---------------- products of stream s ----------------
     const int s = warp - kMma;
-    if (lane == 0) {
+    {
       const uint32_t qa = smem_addr(smem) + s * TL::kQ, ra = smem_addr(ring), t0 = tmem + 256 * s;
       uint32_t idx0 = 0, segs = 0, done = 0, asked = 0;  // pages before the segment; the stream's segments, pages, scores
       bool ok = true;
@@ -637,14 +644,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           if (!wait(&full_k[s][asked % SL], (asked / SL) & 1u)) return false;
           tc_after();
           const uint32_t k = ra + (uint32_t)slot * 2 * TL::kHalf;
+          if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < HD / 64; ++c)
+            for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_ss(t0 + 64 * (asked & 1u), tile_desc(qa + c * (128 * 128) + 32 * kk),
-                     tile_desc(k + c * (kPageTokens * 128) + 32 * kk), instr_desc<T>(kPageTokens), c + kk > 0);
-          tc_commit(&s_full[s][asked & 1u]);
-          release(&free_k[slot]);
+              for (int kk = 0; kk < 4; ++kk)
+                mma_ss(t0 + 64 * (asked & 1u), tile_desc(qa + c * (128 * 128) + 32 * kk),
+                       tile_desc(k + c * (kPageTokens * 128) + 32 * kk), instr_desc<T>(kPageTokens), c + kk > 0);
+            tc_commit(&s_full[s][asked & 1u]);
+            release(&free_k[slot]);
+          }
+          __syncwarp();
           ++asked;
           return true;
         };
@@ -655,16 +665,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           if (!(ok = wait(&full_v[s][done % SL], (done / SL) & 1u) && wait(&p_ready[s][done & 1u], (done >> 1) & 1u))) break;
           tc_after();
           const uint32_t v = ra + (uint32_t)slot * 2 * TL::kHalf + TL::kHalf;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)  // O (+)= P V
-            mma_ts(t0 + 128, t0 + 64 * (done & 1u) + 8 * kk, tile_desc(v + 32 * kk), instr_desc<T>(HD), !first || kk > 0);
-          tc_commit(&o_done[s][done & 1u]);
-          release(&free_v[slot]);
+            for (int kk = 0; kk < 4; ++kk)  // O (+)= P V
+              mma_ts(t0 + 128, t0 + 64 * (done & 1u) + 8 * kk, tile_desc(v + 32 * kk), instr_desc<T>(HD), !first || kk > 0);
+            tc_commit(&o_done[s][done & 1u]);
+            release(&free_v[slot]);
+          }
+          __syncwarp();
           if (b + 2 * step < g.pages) ok = scores(b + 2 * step);  // over the weights that these products read
         }
       }
       if (!ok) {  // products may be in flight: the accumulators are freed after them
-        tc_commit(&drained[s]);
+        if (elect_one()) tc_commit(&drained[s]);
+        __syncwarp();
         mbar_wait(&drained[s], 0, nullptr);
       }
     }

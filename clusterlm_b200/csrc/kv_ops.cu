@@ -430,7 +430,7 @@ bool aligned16(const void* p, long long ld, size_t es) {
 template <typename S, typename T>
 int launch_append(const AppendArgs& a, cudaStream_t st) {
   const size_t smem = (size_t)kPageTokens * (a.rot / 2) * sizeof(float2) + (size_t)kPageTokens * (a.hd + 2) * sizeof(T);
-  CLM_TRY(ensure_smem(kv_append_kernel<S, T>, smem));
+  CLM_TRY(ensure_smem(kv_append_kernel<S, T>, smem + kPageTokens * sizeof(int)));  // (the limit counts static memory too)
   return launch_pdl(kv_append_kernel<S, T>, dim3((unsigned)(a.seqs.n * a.chunks), (unsigned)a.nkv),
                     dim3(kAppendThreads), smem, st, a);
 }

@@ -15,11 +15,14 @@
 //   2. without top-k / top-p: the masses of the CTAs' sixteen warp segments;
 //      with them: the row's whole mass and a histogram of the entries over 64 bins per octave of e, whose counts bound
 //      the cumulative mass within 1.1%: the cut falls into known bins.  Entries above these are allowed (their exact
-//      mass is summed), entries below are not, and the few in them are ranked one against the other.  Where more than
-//      kCand entries share those bins (many equal logits, as from 16-bit types, or a flat row), the key range is
-//      bisected until few enough or one key value is left; of one value the lowest indices stay.
+//      mass is summed), entries below are not, and the few in them are ranked: their key range in 64 parts with exact
+//      masses, then the members of the cut's part one against the other.  Where more than kCand entries share those
+//      bins (many equal logits, as from 16-bit types, or a flat row), the key range is bisected until few enough or
+//      one key value is left; of one value the lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
 #include <cooperative_groups.h>
+
+#include <cfloat>
 
 #include "kv_ops.cuh"
 #include "pdl.cuh"
@@ -36,15 +39,16 @@ constexpr int kWrp = kThr / 32;    // warp segments of a CTA's slice
 constexpr int kBinsOct = 64;       // histogram bins per octave
 constexpr int kBins = 44 * kBinsOct;
 constexpr int kOwn = kBins / kCl;  // bins whose row totals a CTA forms
-constexpr int kCand = 1024;        // entries ranked one against the other
+constexpr int kCand = 1024;        // candidates of a row that are ranked
+constexpr int kMine = 384;         // of one CTA
+constexpr int kSub = 64;           // parts of the candidates' key range
 constexpr int kFrac = 44;          // fraction bits of a mass
-constexpr uint32_t kMaxVocab = 8 * 44032;  // a slice and the tables fit in 227 KB
+constexpr uint32_t kMaxVocab = 8 * 48128;  // a slice and the tables fit in 227 KB
 
 typedef unsigned long long u64;
 
 struct Cand {
-  float d;
-  uint32_t idx;
+  uint32_t u, idx;  // |d| (ascends as the order does) and index
   u64 w;
 };
 
@@ -60,10 +64,9 @@ struct SampleArgs {
   int vec;  // rows and slices start 16-byte aligned
 };
 
-// round(2^44 * 2^y) for y <= 0 (0 below y = -45, and for -inf and NaN): 2^y = 2^n 2^f with |f| <= 1/2 and a degree-8
-// polynomial for 2^f (least maximum relative error by weighted least squares: 7.8e-13).
+// round(2^44 * 2^y) for -45.6 < y <= 0: 2^y = 2^n 2^f with |f| <= 1/2 and a degree-8 polynomial for 2^f (least maximum
+// relative error by weighted least squares: 7.8e-13).
 __device__ __forceinline__ u64 mass_of(double y) {
-  if (!(y > -45.0)) return 0;
   constexpr double kShift = 0x1.8p52;
   const double k = y + kShift;
   const int n = (int)(unsigned)__double_as_longlong(k);
@@ -106,10 +109,26 @@ struct Shared {
   u64 red[kWrp];
   uint32_t redc[kWrp];
   double redd[kWrp];
-  uint32_t cand_n;
+  u64 sub_mass[kSub];
+  uint32_t sub_cnt[kSub];
+  uint32_t cand_n, cut_n, umin, umax;
   int lo, hi;
   uint32_t cnt_above;
 };
+
+// Sums over the CTA of one value per warp (slots of shared memory; every thread gets the sum).
+__device__ __forceinline__ u64 cta_sum(u64 warp_value, u64* slots, int warp, int lane) {
+  __syncthreads();
+  if (lane == 0) slots[warp] = warp_value;
+  __syncthreads();
+  return warp_sum(lane < kWrp ? slots[lane] : 0ull);
+}
+__device__ __forceinline__ uint32_t cta_sum(uint32_t warp_value, uint32_t* slots, int warp, int lane) {
+  __syncthreads();
+  if (lane == 0) slots[warp] = warp_value;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, lane < kWrp ? slots[lane] : 0u);
+}
 
 template <typename S>
 __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
@@ -117,12 +136,13 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   extern __shared__ __align__(16) uint8_t sl_smem[];
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
-  float* key = reinterpret_cast<float*>(sl_smem);  // [slice]
+  float* key = reinterpret_cast<float*>(sl_smem);  // [slice], padded with -inf
   uint32_t* hist = reinterpret_cast<uint32_t*>(key + a.slice);
   uint32_t* tot = hist + kBins;  // the row's histogram
-  Cand* mine = reinterpret_cast<Cand*>(tot + kBins);
-  Cand* all = reinterpret_cast<Cand*>(hist);  // the row's candidates, once the histograms are read
-  static_assert(sizeof(Cand) * kCand <= 2 * kBins * sizeof(uint32_t), "the candidates fit over the histograms");
+  // once the histograms are read, their memory holds the row's candidates and this CTA's
+  Cand* all = reinterpret_cast<Cand*>(hist);
+  Cand* mine = all + kCand;
+  static_assert(sizeof(Cand) * (kCand + kMine) <= 2 * kBins * sizeof(uint32_t), "the candidates fit over the histograms");
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = cluster.block_rank(), row = blockIdx.x / kCl;
   const uint32_t v0 = min(a.V, rank * a.slice), cnt = min(a.V, v0 + a.slice) - v0;
@@ -137,10 +157,10 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   // ---- 1. load and maximum (NaN counts as -inf; -0 as 0)
   const S* src = static_cast<const S*>(a.logits) + (long long)row * a.ld + v0;
   float mx = -INFINITY;
-  auto put = [&](uint32_t i, float x) {
+  auto clean = [&](float x) {
     x = x == x ? x + 0.0f : -INFINITY;
-    key[i] = x;
     mx = fmaxf(mx, x);
+    return x;
   };
   if (a.vec) {
     constexpr int N = 16 / sizeof(S);
@@ -151,33 +171,39 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       S e[N];
       memcpy(e, &w, 16);
 #pragma unroll
-      for (int j = 0; j < N; ++j) put(i * N + j, to_f32(e[j]));
+      for (int j = 0; j < N; j += 4)
+        *reinterpret_cast<float4*>(key + i * N + j) =
+            make_float4(clean(to_f32(e[j])), clean(to_f32(e[j + 1])), clean(to_f32(e[j + 2])), clean(to_f32(e[j + 3])));
     }
-    for (uint32_t i = nv * N + tid; i < cnt; i += kThr) put(i, to_f32(src[i]));
+    for (uint32_t i = nv * N + tid; i < cnt; i += kThr) key[i] = clean(to_f32(src[i]));
   } else {
 #pragma unroll 4
-    for (uint32_t i = tid; i < cnt; i += kThr) put(i, to_f32(src[i]));
+    for (uint32_t i = tid; i < cnt; i += kThr) key[i] = clean(to_f32(src[i]));
   }
+  for (uint32_t i = cnt + tid; i < a.slice; i += kThr) key[i] = -INFINITY;
   for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
   if (tid == 0) s.cand_n = 0;
+  const float T = a.temp ? a.temp[row] : 1.0f;
+  const bool greedy = !(T > 0.0f);
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if (lane == 0) s.redd[warp] = mx;
   __syncthreads();
-  for (int w = 0; w < kWrp; ++w) mx = fmaxf(mx, (float)s.redd[w]);
-  const float T = a.temp ? a.temp[row] : 1.0f;
-  const bool greedy = !(T > 0.0f);
+  mx = (float)s.redd[lane % kWrp];
+  for (int o = kWrp / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   uint32_t first = 0xffffffffu;  // lowest index of the slice's maximum (greedy rows)
-  if (greedy)
+  if (greedy) {
     for (uint32_t i = tid; i < cnt; i += kThr)
       if (key[i] == mx) first = min(first, v0 + i);
-  for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-  if (lane == 0) s.redc[warp] = first;
-  __syncthreads();
-  for (int w = 0; w < kWrp; ++w) first = min(first, s.redc[w]);
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.redc[warp] = first;
+    __syncthreads();
+    first = __reduce_min_sync(0xffffffffu, s.redc[lane % kWrp]);
+  }
   cluster.barrier_wait();  // every CTA of the row runs
   push(s.top, (u64)ord_of(mx) << 32 | (u64)(0xffffffffu - first));
   cluster.sync();
   u64 best = 0;
+#pragma unroll
   for (int r = 0; r < kCl; ++r) best = max(best, s.top[r]);
   const float M = of_ord((uint32_t)(best >> 32));
   if (greedy || M == -INFINITY) {  // the same for the whole cluster
@@ -189,54 +215,81 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
 
   // ---- 2. what is allowed
-  const double c = 1.4426950408889634 / (double)T;
+  const double c = 1.4426950408889634 / (double)T;  // y = c d: e = 2^y
   const float cf = (float)c;
   const int32_t k_in = a.top_k ? a.top_k[row] : 0;
   const float p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f;
   const bool need_k = k_in > 0 && (uint32_t)k_in < a.V, need_p = p_in < 1.0f;
   const uint32_t k = need_k ? (uint32_t)k_in : 0xffffffffu;
-  const double ymin = m_in > 0.0f ? log2((double)fminf(m_in, 1.0f)) : -46.0;
+  // entries below dcut have no mass (y < -45: it rounds to zero); entries below dlow are not allowed: dcut, or the
+  // first float whose y is log2(min_p) or more
+  const float dcut = fmaxf(-FLT_MAX, (float)(-45.5 / c));
+  float dlow = dcut;
+  if (m_in > 0.0f) {
+    const double ymin = log2((double)fminf(m_in, 1.0f));
+    float d = fminf(0.0f, fmaxf(-FLT_MAX, (float)(ymin / c)));
+    while (d < 0.0f && (double)d * c < ymin) d = nextafterf(d, 0.0f);
+    while (d > -FLT_MAX && (double)nextafterf(d, -INFINITY) * c >= ymin) d = nextafterf(d, -INFINITY);
+    dlow = fmaxf(dcut, d);
+  }
   auto d_of = [&](float x) { return x == M ? 0.0f : __fsub_rn(x, M); };
-  auto y_of = [&](float d) { return d == 0.0f ? 0.0 : (double)d * c; };
+  auto mass = [&](float d) {  // of any entry
+    const u64 w = mass_of((double)fmaxf(d, dcut) * c);
+    return d >= dcut ? w : 0ull;
+  };
   auto bin_of = [&](float d) {  // ascends as the order does (cf may be infinite: 0 has bin 0)
     return d == 0.0f ? 0 : min(kBins - 1, (int)fminf(-d * cf * (float)kBinsOct, (float)kBins));
   };
   auto u_of = [&](float d) { return __float_as_uint(fabsf(d)); };  // ascends as the order does
-  const uint32_t seg = (a.slice + kWrp - 1) / kWrp;
-  const uint32_t s0 = min(cnt, warp * seg), s1 = min(cnt, s0 + seg);  // this warp's segment
-  int hi = kBins;                 // allowed entries: bin <= hi, u <= umax, key not struck out
+  const uint32_t seg = (a.slice / 4 + kWrp - 1) / kWrp * 4;
+  const uint32_t s0 = min(a.slice, warp * seg), s1 = min(a.slice, s0 + seg);  // this warp's segment
+  // f(index, d) for the segment's entries, four consecutive ones a lane at a time (independent chains)
+  auto each = [&](auto&& f) {
+    for (uint32_t i = s0 + 4 * lane; i < s1; i += 128) {
+      const float4 x = *reinterpret_cast<const float4*>(key + i);
+      f(i, d_of(x.x));
+      f(i + 1, d_of(x.y));
+      f(i + 2, d_of(x.z));
+      f(i + 3, d_of(x.w));
+    }
+  };
+  int hi = kBins;  // allowed entries: d >= dlow, bin <= hi, u <= umax, key not struck out
   uint32_t umax = 0x7f7fffffu;
   u64 seg_mass = 0;
   if (!need_k && !need_p) {
-    for (uint32_t i = s0 + lane; i < s1; i += 32) {
-      const double y = y_of(d_of(key[i]));
-      if (y >= ymin) seg_mass += mass_of(y);
-    }
+    each([&](uint32_t, float d) { seg_mass += d >= dlow ? mass(d) : 0ull; });
     seg_mass = warp_sum(seg_mass);
   } else {
     u64 sum = 0;
-    for (uint32_t i = s0 + lane; i < s1; i += 32) {
-      const float d = d_of(key[i]);
-      const double y = y_of(d);
-      if (!(y > -45.0)) continue;
-      if (need_p) sum += mass_of(y);
-      if (y >= ymin) atomicAdd(&hist[bin_of(d)], 1u);
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) s.red[warp] = sum;
-    __syncthreads();
-    sum = 0;
-    for (int w = 0; w < kWrp; ++w) sum += s.red[w];
-    push(s.total, sum);
+    if (need_p)
+      each([&](uint32_t, float d) {
+        sum += mass(d);
+        if (d >= dlow) atomicAdd(&hist[bin_of(d)], 1u);
+      });
+    else
+      each([&](uint32_t, float d) {
+        if (d >= dlow) atomicAdd(&hist[bin_of(d)], 1u);
+      });
+    push(s.total, cta_sum(warp_sum(sum), s.red, warp, lane));
     cluster.sync();
     for (int b = tid; b < kOwn; b += kThr) {
       const int bin = (int)rank * kOwn + b;
-      uint32_t n = 0;
-      for (int r = 0; r < kCl; ++r) n += cluster.map_shared_rank(hist, r)[bin];
+      uint32_t part[kCl], n = 0;
+#pragma unroll
+      for (int r = 0; r < kCl; ++r) part[r] = cluster.map_shared_rank(hist, r)[bin];
+#pragma unroll
+      for (int r = 0; r < kCl; ++r) n += part[r];
+#pragma unroll
       for (int r = 0; r < kCl; ++r) cluster.map_shared_rank(tot, r)[bin] = n;
+    }
+    if (tid == 0) {
+      s.lo = kBins;
+      s.hi = kBins;
+      s.cnt_above = 0;
     }
     cluster.sync();
     u64 total = 0;
+#pragma unroll
     for (int r = 0; r < kCl; ++r) total += s.total[r];
     // allowed by top-p: entries with less than `thr` mass before them (p in units of 2^-40, rounded up)
     u64 thr = ~0ull;
@@ -256,7 +309,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     for (int j = 0; j < kPer; ++j) {
       const int bin = tid * kPer + j;
       n[j] = bin < kBins ? tot[bin] : 0u;
-      m[j] = n[j] ? (double)n[j] * (double)exp2f((float)kFrac - (float)bin / kBinsOct) : 0.0;
+      m[j] = (double)((float)n[j] * exp2f((float)kFrac - (float)bin / kBinsOct));
       nsum += n[j];
       msum += m[j];
     }
@@ -274,156 +327,134 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       s.redc[warp] = nx;
       s.redd[warp] = mm;
     }
-    if (tid == 0) {
-      s.lo = kBins;
-      s.hi = kBins;
-    }
     __syncthreads();
-    for (int w = 0; w < warp; ++w) {
-      nx += s.redc[w];
-      mm += s.redd[w];
+    {
+      nx += __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u) - nsum;
+      double before = lane < warp ? s.redd[lane % kWrp] : 0.0;
+      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      mm += before - msum;
     }
-    nx -= nsum;
-    mm -= msum;
     // a bin's entries weigh between 2^(-1/64) and 1 times its upper edge (1e-4 covers the f32 roundings)
     constexpr double kUp = 1.0001, kDown = 0.989228 * 0.9999;
+    int lo_mine = kBins, hi_mine = kBins;
+    uint32_t before_lo = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int bin = tid * kPer + j;
-      if (bin >= kBins) break;
+      const uint32_t n0 = nx;
       nx += n[j];
       mm += m[j];
       const bool by_k = nx >= k;
-      if (by_k || (need_p && mm * kUp >= (double)thr)) atomicMin(&s.lo, bin);
-      if (by_k || (need_p && mm * kDown >= (double)thr)) atomicMin(&s.hi, bin);
+      if (bin < kBins && lo_mine == kBins && (by_k || (need_p && mm * kUp >= (double)thr))) {
+        lo_mine = bin;
+        before_lo = n0;
+      }
+      if (bin < kBins && hi_mine == kBins && (by_k || (need_p && mm * kDown >= (double)thr))) hi_mine = bin;
     }
+    if (lo_mine < kBins) atomicMin(&s.lo, lo_mine);
+    if (hi_mine < kBins) atomicMin(&s.hi, hi_mine);
     __syncthreads();
     const int lo = s.lo;
     hi = s.hi;
-    if (lo < kBins) {  // else every entry with mass is allowed
-      if (tid == lo / kPer) {
-        uint32_t before = nx - nsum;
-        for (int j = 0; j < lo % kPer; ++j) before += n[j];
-        s.cnt_above = before;
-      }
-    } else if (tid == 0) {
-      s.cnt_above = 0;
-    }
-    for (uint32_t i = s0 + lane; i < s1; i += 32) {
-      const float d = d_of(key[i]);
-      const double y = y_of(d);
-      if (!(y > -45.0) || y < ymin) continue;
+    if (lo_mine == lo && lo < kBins) s.cnt_above = before_lo;  // (one thread; without a cut every entry is above it)
+    each([&](uint32_t i, float d) {
       const int bin = bin_of(d);
-      if (bin > hi) continue;
-      const u64 w = mass_of(y);
+      if (d < dlow || bin > hi) return;
+      const u64 w = mass(d);
       if (bin < lo) {
         seg_mass += w;
       } else {
         const uint32_t at = atomicAdd(&s.cand_n, 1u);
-        if (at < kCand) mine[at] = Cand{d, v0 + i, w};
+        if (at < kMine) mine[at] = Cand{u_of(d), v0 + i, w};
       }
-    }
+    });
     seg_mass = warp_sum(seg_mass);
-    if (lane == 0) s.seg[warp] = seg_mass;
-    __syncthreads();
     {
-      u64 x = 0;
-      for (int w = 0; w < kWrp; ++w) x += s.seg[w];
+      const u64 x = cta_sum(seg_mass, s.seg, warp, lane);
       push(s.above, x);
       push(s.ncand, s.cand_n);
     }
     cluster.sync();
     u64 above = 0;
-    uint32_t cand = 0, before = 0;
+    uint32_t cand = 0, before = 0, most = 0;
+    uint32_t in[kCl];  // candidates of each CTA
+#pragma unroll
     for (int r = 0; r < kCl; ++r) {
       above += s.above[r];
-      if (r < (int)rank) before += s.ncand[r];
-      cand += s.ncand[r];
+      in[r] = s.ncand[r];
     }
+    auto recount_candidates = [&] {
+      cand = before = most = 0;
+#pragma unroll
+      for (int r = 0; r < kCl; ++r) {
+        if (r < (int)rank) before += in[r];
+        cand += in[r];
+        most = max(most, in[r]);
+      }
+    };
+    recount_candidates();
     uint32_t cnt_above = s.cnt_above;
     bool recount = false;  // the segments' masses are summed anew
     bool struck = false;
-    if (cand > kCand) {
+    if (cand > kCand || most > kMine) {
       // bisect the keys of the bins [lo, hi]: entries with u < ul are allowed, entries with u > uh are not
       uint32_t ul = 0, uh = 0x7f7fffffu;
       int turn = 0;
       recount = true;
-      while (ul < uh && cand > kCand) {
+      auto inside = [&](float d) {
+        const uint32_t u = u_of(d);
+        const int bin = bin_of(d);
+        return u >= ul && u <= uh && bin >= lo && bin <= hi && d >= dlow;
+      };
+      while (ul < uh && (cand > kCand || most > kMine)) {
         const uint32_t mid = ul + (uh - ul) / 2;
         uint32_t cl = 0;
         u64 ml = 0;
-        for (uint32_t i = s0 + lane; i < s1; i += 32) {
-          const float d = d_of(key[i]);
-          const uint32_t u = u_of(d);
-          if (u < ul || u > mid) continue;
-          const int bin = bin_of(d);
-          const double y = y_of(d);
-          if (bin < lo || bin > hi || !(y > -45.0) || y < ymin) continue;
+        each([&](uint32_t, float d) {
+          if (u_of(d) > mid || !inside(d)) return;
           ++cl;
-          ml += mass_of(y);
-        }
-        cl = __reduce_add_sync(0xffffffffu, cl);
-        ml = warp_sum(ml);
-        __syncthreads();
-        if (lane == 0) {
-          s.redc[warp] = cl;
-          s.red[warp] = ml;
-        }
-        __syncthreads();
-        cl = 0;
-        ml = 0;
-        for (int w = 0; w < kWrp; ++w) {
-          cl += s.redc[w];
-          ml += s.red[w];
-        }
-        push(s.it_cnt[turn], cl);
-        push(s.it_mass[turn], ml);
+          ml += mass(d);
+        });
+        push(s.it_cnt[turn], cta_sum(__reduce_add_sync(0xffffffffu, cl), s.redc, warp, lane));
+        push(s.it_mass[turn], cta_sum(warp_sum(ml), s.red, warp, lane));
         cluster.sync();
+        uint32_t got[kCl];
         cl = 0;
         ml = 0;
+#pragma unroll
         for (int r = 0; r < kCl; ++r) {
-          cl += s.it_cnt[turn][r];
+          got[r] = s.it_cnt[turn][r];
+          cl += got[r];
           ml += s.it_mass[turn][r];
         }
         turn ^= 1;
-        if (cnt_above + cl >= k || above + ml >= thr) {
+        const bool down = cnt_above + cl >= k || above + ml >= thr;
+        if (down) {
           uh = mid;
-          cand = cl;
         } else {
           ul = mid + 1;
           cnt_above += cl;
           above += ml;
-          cand -= cl;
         }
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) in[r] = down ? got[r] : in[r] - got[r];
+        recount_candidates();
       }
       umax = uh;
-      if (cand <= kCand) {
+      if (cand <= kCand && most <= kMine) {
         // collect the candidates again, from the narrowed range
         __syncthreads();
         if (tid == 0) s.cand_n = 0;
         __syncthreads();
-        for (uint32_t i = s0 + lane; i < s1; i += 32) {
-          const float d = d_of(key[i]);
-          const uint32_t u = u_of(d);
-          if (u < ul || u > uh) continue;
-          const int bin = bin_of(d);
-          const double y = y_of(d);
-          if (bin < lo || bin > hi || !(y > -45.0) || y < ymin) continue;
-          mine[atomicAdd(&s.cand_n, 1u)] = Cand{d, v0 + i, mass_of(y)};
-        }
-        __syncthreads();
-        push(s.ncand, s.cand_n);
+        each([&](uint32_t i, float d) {
+          if (!inside(d)) return;
+          mine[atomicAdd(&s.cand_n, 1u)] = Cand{u_of(d), v0 + i, mass(d)};
+        });
         cluster.sync();
-        before = cand = 0;
-        for (int r = 0; r < kCl; ++r) {
-          if (r < (int)rank) before += s.ncand[r];
-          cand += s.ncand[r];
-        }
       } else {
         // one key value: its `stay` lowest indices are allowed
         struck = true;
-        const float d = -__uint_as_float(ul);
-        const u64 w = mass_of(y_of(d));
+        const u64 w = mass(-__uint_as_float(ul));
         u64 stay = ~0ull;
         if (need_k) stay = k - cnt_above;
         if (need_p && w > 0) stay = min(stay, (thr - above + w - 1) / w);
@@ -432,14 +463,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           const uint32_t i = i0 + lane;
           ties += __popc(__ballot_sync(0xffffffffu, i < s1 && u_of(d_of(key[i])) == ul));
         }
-        __syncthreads();
-        if (lane == 0) s.redc[warp] = ties;
-        __syncthreads();
-        uint32_t all_ties = 0, rank_in = 0;
-        for (int w2 = 0; w2 < kWrp; ++w2) {
-          if (w2 < warp) rank_in += s.redc[w2];
-          all_ties += s.redc[w2];
-        }
+        const uint32_t all_ties = cta_sum(ties, s.redc, warp, lane);
+        uint32_t rank_in = __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u);
         push(s.ties, all_ties);
         cluster.sync();
         for (int r = 0; r < (int)rank; ++r) rank_in += s.ties[r];
@@ -450,60 +475,129 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           if (tie && rank_in + __popc(bal & ((1u << lane) - 1u)) >= stay) key[i] = -INFINITY;
           rank_in += __popc(bal);
         }
-        __syncthreads();
       }
     }
     if (!struck && cand > 0) {
-      // every candidate's rank and the mass before it, against all candidates of the row
+      // The candidates' key range in kSub parts, with exact counts and masses: the cut falls into one part, and only its
+      // members are ranked one against the other.
+      for (int i = tid; i < kSub; i += kThr) {
+        s.sub_mass[i] = 0;
+        s.sub_cnt[i] = 0;
+      }
+      if (tid == 0) {
+        s.umin = 0xffffffffu;
+        s.umax = 0;
+        s.cut_n = 0;
+      }
+      __syncthreads();
+      // (mine lies behind `all`, so the copies do not touch what other CTAs read)
+      uint32_t least = 0xffffffffu, largest = 0;
+#pragma unroll 1
       for (int r = 0, at = 0; r < kCl; ++r) {
         const Cand* theirs = cluster.map_shared_rank(mine, r);
-        for (uint32_t i = tid; i < s.ncand[r]; i += kThr) all[at + i] = theirs[i];
-        at += s.ncand[r];
+        for (uint32_t i = tid; i < in[r]; i += kThr) {
+          const Cand x = theirs[i];
+          all[at + i] = x;
+          least = min(least, x.u);
+          largest = max(largest, x.u);
+        }
+        at += in[r];
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
+      largest = __reduce_max_sync(0xffffffffu, largest);
+      if (lane == 0) {
+        atomicMin(&s.umin, least);
+        atomicMax(&s.umax, largest);
       }
       __syncthreads();
-      for (uint32_t i = tid; i < s.ncand[rank]; i += kThr) {
+      const uint32_t u0 = s.umin;
+      const float per = (float)kSub / ((float)(s.umax - u0) + 1.0f);
+      auto part_of = [&](uint32_t u) { return min(kSub - 1, (int)((float)(u - u0) * per)); };  // ascends with u
+      for (uint32_t i = tid; i < cand; i += kThr) {
+        const Cand x = all[i];
+        const int p = part_of(x.u);
+        atomicAdd(&s.sub_cnt[p], 1u);
+        atomicAdd(&s.sub_mass[p], x.w);
+      }
+      __syncthreads();
+      // every warp: two parts a lane, cumulative; the first part that reaches top-k or top-p holds the cut
+      static_assert(kSub == 64, "two parts a lane");
+      const uint32_t c0 = s.sub_cnt[2 * lane], c1 = s.sub_cnt[2 * lane + 1];
+      const u64 w0 = s.sub_mass[2 * lane], w1 = s.sub_mass[2 * lane + 1];
+      uint32_t cx = c0 + c1;
+      u64 wx = w0 + w1;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t oc = __shfl_up_sync(0xffffffffu, cx, o);
+        const u64 ow = __shfl_up_sync(0xffffffffu, wx, o);
+        if (lane >= o) {
+          cx += oc;
+          wx += ow;
+        }
+      }
+      cx += cnt_above;
+      wx += above;
+      const bool at1 = cx >= k || wx >= thr, at0 = cx - c1 >= k || wx - w1 >= thr;
+      const uint32_t reach = __ballot_sync(0xffffffffu, at1);
+      int cut = kSub;  // no part reaches it: all candidates are allowed
+      uint32_t cb = 0;
+      u64 mb = 0;
+      if (reach) {
+        const int l = __ffs(reach) - 1;
+        const bool low = __shfl_sync(0xffffffffu, at0, l);
+        cut = 2 * l + (low ? 0 : 1);
+        cb = __shfl_sync(0xffffffffu, low ? cx - c1 - c0 : cx - c1, l);
+        mb = __shfl_sync(0xffffffffu, low ? wx - w1 - w0 : wx - w1, l);
+      }
+      // the cut part's members, in the place of this CTA's candidates (which every CTA has read: the barrier)
+      cluster.sync();
+      for (uint32_t i = tid; i < cand; i += kThr)
+        if (part_of(all[i].u) == cut) {
+          const uint32_t at = atomicAdd(&s.cut_n, 1u);
+          if (at < kMine) mine[at] = all[i];
+        }
+      __syncthreads();
+      const uint32_t members = s.cut_n;
+      const bool few = members <= kMine;
+      const Cand* rivals = few ? mine : all;
+      for (uint32_t i = tid; i < in[rank]; i += kThr) {
         const Cand me = all[before + i];
-        uint32_t cb = cnt_above;
-        u64 mb = above;
-        for (uint32_t j = 0; j < cand; ++j) {
-          const Cand o = all[j];
-          if (o.d > me.d || (o.d == me.d && o.idx < me.idx)) {
-            ++cb;
-            mb += o.w;
+        const int p = part_of(me.u);
+        bool allowed = p < cut;
+        if (p == cut) {
+          uint32_t nb = cb;
+          u64 wb = mb;
+#pragma unroll 4
+          for (uint32_t j = 0; j < (few ? members : cand); ++j) {
+            const Cand o = rivals[j];
+            const bool ahead = (o.u < me.u || (o.u == me.u && o.idx < me.idx)) && (few || part_of(o.u) == cut);
+            nb += ahead;
+            wb += ahead ? o.w : 0ull;
           }
+          allowed = nb < k && wb < thr;
         }
-        if (cb < k && mb < thr) {
-          if (!recount) atomicAdd(&s.seg[(me.idx - v0) / seg], me.w);
-        } else {
+        if (!allowed)
           key[me.idx - v0] = -INFINITY;
-        }
+        else if (!recount)
+          atomicAdd(&s.seg[(me.idx - v0) / seg], me.w);
       }
-      __syncthreads();
     }
+    __syncthreads();
     if (recount) {
       seg_mass = 0;
-      for (uint32_t i = s0 + lane; i < s1; i += 32) {
-        const float d = d_of(key[i]);
-        const double y = y_of(d);
-        if (bin_of(d) <= hi && u_of(d) <= umax && y >= ymin) seg_mass += mass_of(y);
-      }
+      each([&](uint32_t, float d) {
+        if (d >= dlow && bin_of(d) <= hi && u_of(d) <= umax) seg_mass += mass(d);
+      });
       seg_mass = warp_sum(seg_mass);
     } else {
       seg_mass = s.seg[warp];
     }
-    __syncthreads();
   }
 
   // ---- 3. the token
-  if (lane == 0) s.seg[warp] = seg_mass;
-  __syncthreads();
-  {
-    u64 x = 0;
-    for (int w = 0; w < kWrp; ++w) x += s.seg[w];
-    push(s.kept, x);
-  }
+  push(s.kept, cta_sum(seg_mass, s.seg, warp, lane));
   cluster.sync();
   u64 W = 0;
+#pragma unroll
   for (int r = 0; r < kCl; ++r) W += s.kept[r];
   // floor(u W), exactly: u = m 2^-e with a 53-bit m
   const double u = a.u[row];
@@ -523,13 +617,12 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   if (owner != rank) return;
   int ws = 0;
   for (; ws + 1 < kWrp && base + s.seg[ws] <= r; ++ws) base += s.seg[ws];
-  // entries of the segment, kPerT consecutive ones a thread
-  const uint32_t g0 = min(cnt, ws * seg), g1 = min(cnt, g0 + seg), per = (seg + kThr - 1) / kThr;
+  // entries of the segment, consecutive ones a thread
+  const uint32_t g0 = min(a.slice, ws * seg), g1 = min(a.slice, g0 + seg), per = (seg + kThr - 1) / kThr;
   const uint32_t e0 = min(g1, g0 + tid * per), e1 = min(g1, e0 + per);
   auto mass_at = [&](uint32_t i) -> u64 {
     const float d = d_of(key[i]);
-    const double y = y_of(d);
-    return bin_of(d) <= hi && u_of(d) <= umax && y >= ymin ? mass_of(y) : 0ull;
+    return d >= dlow && bin_of(d) <= hi && u_of(d) <= umax ? mass(d) : 0ull;
   };
   u64 own = 0;
   for (uint32_t i = e0; i < e1; ++i) own += mass_at(i);
@@ -538,17 +631,15 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     const u64 x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += x;
   }
-  __syncthreads();
   if (lane == 31) s.red[warp] = inc;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) base += s.red[w];
-  base += inc - own;
+  base += warp_sum(lane < warp ? s.red[lane % kWrp] : 0ull) + inc - own;
   if (own > 0 && base <= r && r < base + own) {
     for (uint32_t i = e0; i < e1; ++i) {
       const u64 w = mass_at(i);
       if (w > 0 && r < base + w) {
         a.token[row] = (int32_t)(v0 + i);
-        if (a.prob) a.prob[row] = (float)(exp2(y_of(d_of(key[i]))) / ((double)W * 0x1p-44));
+        if (a.prob) a.prob[row] = (float)(exp2((double)d_of(key[i]) * c) / ((double)W * 0x1p-44));
         break;
       }
       base += w;
@@ -560,10 +651,10 @@ template <typename S>
 int launch_sample_logits(SampleArgs a, uint32_t rows, cudaStream_t st) {
   constexpr int N = 16 / sizeof(S);
   a.slice = (uint32_t)((ceil_div(a.V, kCl) + N - 1) / N * N);
-  a.slice = (a.slice + 3) / 4 * 4;  // the tables after the keys stay 16-byte aligned
+  a.slice = (a.slice + 3) / 4 * 4;  // four entries a lane, and the tables after the keys stay 16-byte aligned
   a.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.ld % N == 0;
-  const size_t smem = (size_t)a.slice * 4 + 2 * kBins * sizeof(uint32_t) + kCand * sizeof(Cand);
-  CLM_TRY(ensure_smem(sample_logits_kernel<S>, smem));
+  const size_t smem = (size_t)a.slice * 4 + 2 * kBins * sizeof(uint32_t);
+  CLM_TRY(ensure_smem(sample_logits_kernel<S>, smem + sizeof(Shared)));  // (the limit counts static memory too)
   return launch_pdl(sample_logits_kernel<S>, dim3(rows * kCl), dim3(kThr), smem, st, a);
 }
 

@@ -134,7 +134,7 @@ CLM_API int clm_b200_distribution_rows(clm_b200_ctx* ctx, const float* d_logits,
  * error bound proves the serial rounding cannot change it; otherwise the row is re-walked serially. */
 CLM_API int clm_b200_sample_rows(clm_b200_ctx* ctx, const float* d_probs, uint32_t rows, uint32_t vocab,
                          const double* d_uniforms, int32_t* d_out, void* stream);
-/* A token per row straight from logits (f32, f16 or bf16; row r starts ld elements after row r - 1; vocab <= 352256),
+/* A token per row straight from logits (f32, f16 or bf16; row r starts ld elements after row r - 1; vocab <= 385024),
  * every row with its own settings; a NULL array is the default for all rows.  No reference counterpart in this form
  * (distribution() and sample_from(), sampling.cpp:51-101, with one setting; min-p is not in the reference).
  *   d_temperature  e_i = exp((l_i - max) / T), default 1; T <= 0 (or NaN): the lowest index of the maximum

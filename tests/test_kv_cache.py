@@ -253,7 +253,7 @@ def sample(ctx=CTX, logits=A, dtype=0, rows=3, vocab=100, ld=100, u=A, out=A):
 
 
 @pytest.mark.parametrize("kw,code", [(dict(ctx=None), INVALID), (dict(vocab=0), INVALID),
-                                     (dict(vocab=352257, ld=352257), RANGE), (dict(ld=99), INVALID),
+                                     (dict(vocab=385025, ld=385025), RANGE), (dict(ld=99), INVALID),
                                      (dict(dtype=3), INVALID), (dict(dtype=-1), INVALID), (dict(logits=0), INVALID),
                                      (dict(u=0), INVALID), (dict(out=0), INVALID), (dict(rows=2**30), RANGE)])
 def test_sample_refuses(kw, code):

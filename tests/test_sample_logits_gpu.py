@@ -207,5 +207,5 @@ def test_refusals(ctx, sample):
     from clusterlm_b200._native import ClmError
 
     with pytest.raises(ClmError):
-        sample(ctx, torch.zeros(1, 352257, device="cuda"), u[:1])
+        sample(ctx, torch.zeros(1, 385025, device="cuda"), u[:1])
     assert sample(ctx, logits[:0], u[:0]).numel() == 0

@@ -17,8 +17,8 @@
 //      the cumulative mass within 1.1%: the cut falls into known bins.  Entries above these are allowed (their exact
 //      mass is summed), entries below are not, and the few in them are ranked: their key range in 64 parts with exact
 //      masses, then the members of the cut's part one against the other.  Where more than kCand entries share those
-//      bins (many equal logits, as from 16-bit types, or a flat row), the key range is bisected until few enough or
-//      one key value is left; of one value the lowest indices stay.
+//      bins (a flat row, or equal logits, as from 16-bit types), their key range is divided again; where one key value
+//      is left, its lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
 #include <cooperative_groups.h>
 
@@ -101,19 +101,18 @@ struct Shared {
   u64 total[kCl];     // whole mass (pass 2)
   u64 above[kCl];     // mass above the candidates
   u64 kept[kCl];      // allowed mass
-  uint32_t ncand[kCl];
-  u64 it_mass[2][kCl];  // bisection, alternating
-  uint32_t it_cnt[2][kCl];
+  uint32_t ncand[kCl], umin[kCl], umax[kCl];  // candidates: how many, their key range
   uint32_t ties[kCl];
   u64 seg[kWrp];      // allowed mass of the warp segments
   u64 red[kWrp];
   uint32_t redc[kWrp];
-  double redd[kWrp];
+  double redd[kWrp], rede[kWrp];
   u64 sub_mass[kSub];
   uint32_t sub_cnt[kSub];
-  uint32_t cand_n, cut_n, umin, umax;
+  uint32_t cand_n, cut_n;
+  float few[kWrp][160];  // entries whose masses a warp has yet to sum
   int lo, hi;
-  uint32_t cnt_above;
+  uint32_t cnt_before;
 };
 
 // Sums over the CTA of one value per warp (slots of shared memory; every thread gets the sum).
@@ -237,9 +236,6 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     const u64 w = mass_of((double)fmaxf(d, dcut) * c);
     return d >= dcut ? w : 0ull;
   };
-  auto bin_of = [&](float d) {  // ascends as the order does (cf may be infinite: 0 has bin 0)
-    return d == 0.0f ? 0 : min(kBins - 1, (int)fminf(-d * cf * (float)kBinsOct, (float)kBins));
-  };
   auto u_of = [&](float d) { return __float_as_uint(fabsf(d)); };  // ascends as the order does
   const uint32_t seg = (a.slice / 4 + kWrp - 1) / kWrp * 4;
   const uint32_t s0 = min(a.slice, warp * seg), s1 = min(a.slice, s0 + seg);  // this warp's segment
@@ -253,205 +249,221 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       f(i + 3, d_of(x.w));
     }
   };
-  int hi = kBins;  // allowed entries: d >= dlow, bin <= hi, u <= umax, key not struck out
+  // allowed entries: d >= dlow, u <= umax, key not struck out
   uint32_t umax = 0x7f7fffffu;
   u64 seg_mass = 0;
   if (!need_k && !need_p) {
     each([&](uint32_t, float d) { seg_mass += d >= dlow ? mass(d) : 0ull; });
     seg_mass = warp_sum(seg_mass);
   } else {
-    u64 sum = 0;
-    if (need_p)
-      each([&](uint32_t, float d) {
-        sum += mass(d);
-        if (d >= dlow) atomicAdd(&hist[bin_of(d)], 1u);
-      });
-    else
-      each([&](uint32_t, float d) {
-        if (d >= dlow) atomicAdd(&hist[bin_of(d)], 1u);
-      });
-    push(s.total, cta_sum(warp_sum(sum), s.red, warp, lane));
-    cluster.sync();
-    for (int b = tid; b < kOwn; b += kThr) {
-      const int bin = (int)rank * kOwn + b;
-      uint32_t part[kCl], n = 0;
-#pragma unroll
-      for (int r = 0; r < kCl; ++r) part[r] = cluster.map_shared_rank(hist, r)[bin];
-#pragma unroll
-      for (int r = 0; r < kCl; ++r) n += part[r];
-#pragma unroll
-      for (int r = 0; r < kCl; ++r) cluster.map_shared_rank(tot, r)[bin] = n;
-    }
-    if (tid == 0) {
-      s.lo = kBins;
-      s.hi = kBins;
-      s.cnt_above = 0;
-    }
-    cluster.sync();
-    u64 total = 0;
-#pragma unroll
-    for (int r = 0; r < kCl; ++r) total += s.total[r];
-    // allowed by top-p: entries with less than `thr` mass before them (p in units of 2^-40, rounded up)
-    u64 thr = ~0ull;
-    if (need_p) {
-      const u64 pi = (u64)ceil(fmax((double)p_in, 0.0) * 0x1p40);
-      const u64 ph = __umul64hi(pi, total), pl = pi * total;
-      thr = (ph << 24 | pl >> 40) + ((pl & 0xffffffffffull) != 0);
-      if (thr == 0) thr = 1;
-    }
-    // cumulative counts and (approximate) masses over the bins
-    constexpr int kPer = (kBins + kThr - 1) / kThr;
-    uint32_t n[kPer];
-    double m[kPer];
-    uint32_t nsum = 0;
-    double msum = 0.0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int bin = tid * kPer + j;
-      n[j] = bin < kBins ? tot[bin] : 0u;
-      m[j] = (double)((float)n[j] * exp2f((float)kFrac - (float)bin / kBinsOct));
-      nsum += n[j];
-      msum += m[j];
-    }
-    uint32_t nx = nsum;
-    double mm = msum;
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t on = __shfl_up_sync(0xffffffffu, nx, o);
-      const double om = __shfl_up_sync(0xffffffffu, mm, o);
-      if (lane >= o) {
-        nx += on;
-        mm += om;
-      }
-    }
-    if (lane == 31) {
-      s.redc[warp] = nx;
-      s.redd[warp] = mm;
-    }
-    __syncthreads();
-    {
-      nx += __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u) - nsum;
-      double before = lane < warp ? s.redd[lane % kWrp] : 0.0;
-      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      mm += before - msum;
-    }
-    // a bin's entries weigh between 2^(-1/64) and 1 times its upper edge (1e-4 covers the f32 roundings)
-    constexpr double kUp = 1.0001, kDown = 0.989228 * 0.9999;
-    int lo_mine = kBins, hi_mine = kBins;
-    uint32_t before_lo = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int bin = tid * kPer + j;
-      const uint32_t n0 = nx;
-      nx += n[j];
-      mm += m[j];
-      const bool by_k = nx >= k;
-      if (bin < kBins && lo_mine == kBins && (by_k || (need_p && mm * kUp >= (double)thr))) {
-        lo_mine = bin;
-        before_lo = n0;
-      }
-      if (bin < kBins && hi_mine == kBins && (by_k || (need_p && mm * kDown >= (double)thr))) hi_mine = bin;
-    }
-    if (lo_mine < kBins) atomicMin(&s.lo, lo_mine);
-    if (hi_mine < kBins) atomicMin(&s.hi, hi_mine);
-    __syncthreads();
-    const int lo = s.lo;
-    hi = s.hi;
-    if (lo_mine == lo && lo < kBins) s.cnt_above = before_lo;  // (one thread; without a cut every entry is above it)
-    each([&](uint32_t i, float d) {
-      const int bin = bin_of(d);
-      if (d < dlow || bin > hi) return;
-      const u64 w = mass(d);
-      if (bin < lo) {
-        seg_mass += w;
+    // The cut is located level by level.  A level looks at the entries with keys in [ul, uh]: those before are allowed
+    // (cnt_above of them, with the mass `above`), those behind are not.  Level 0 has all entries in bins of 1/64 octave of
+    // e; the others divide what is left evenly.
+    uint32_t ul = 0, uh = umax, span = umax, cand = 0, before = 0, cnt_above = 0, most = 0;
+    uint32_t in[kCl];  // candidates of each CTA
+    u64 above = 0, thr = ~0ull;
+    bool struck = false;
+    auto look = [&](auto level0) {  // (two copies of the code: level 0 reads every entry)
+      constexpr bool kFirst = decltype(level0)::value;
+      const float inv = (float)kBins / ((float)(uh - ul) + 1.0f);
+      auto bin_of = [&](float d) {  // ascends as the order does (cf may be infinite: 0 has bin 0)
+        if (!kFirst) return min(kBins - 1, (int)((float)(u_of(d) - ul) * inv));
+        return d == 0.0f ? 0 : min(kBins - 1, (int)fminf(-d * cf * (float)kBinsOct, (float)kBins));
+      };
+      auto inside = [&](float d) { return d >= dlow && (kFirst || (u_of(d) >= ul && u_of(d) <= uh)); };
+      u64 sum = 0;
+      if (kFirst && need_p) {
+        each([&](uint32_t, float d) {
+          sum += mass(d);
+          if (d >= dlow) atomicAdd(&hist[bin_of(d)], 1u);
+        });
       } else {
-        const uint32_t at = atomicAdd(&s.cand_n, 1u);
-        if (at < kMine) mine[at] = Cand{u_of(d), v0 + i, w};
+        each([&](uint32_t, float d) {
+          if (inside(d)) atomicAdd(&hist[bin_of(d)], 1u);
+        });
       }
-    });
-    seg_mass = warp_sum(seg_mass);
-    {
-      const u64 x = cta_sum(seg_mass, s.seg, warp, lane);
+      push(s.total, cta_sum(warp_sum(sum), s.red, warp, lane));
+      cluster.sync();
+      for (int b = tid; b < kOwn; b += kThr) {
+        const int bin = (int)rank * kOwn + b;
+        uint32_t part[kCl], n = 0;
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) part[r] = cluster.map_shared_rank(hist, r)[bin];
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) n += part[r];
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) cluster.map_shared_rank(tot, r)[bin] = n;
+      }
+      if (tid == 0) {
+        s.lo = kBins;
+        s.hi = kBins;
+        s.cand_n = 0;
+      }
+      cluster.sync();
+      if (kFirst && need_p) {
+        // allowed by top-p: entries with less than `thr` mass before them (p in units of 2^-40, rounded up)
+        u64 total = 0;
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) total += s.total[r];
+        const u64 pi = (u64)ceil(fmax((double)p_in, 0.0) * 0x1p40);
+        const u64 ph = __umul64hi(pi, total), pl = pi * total;
+        thr = (ph << 24 | pl >> 40) + ((pl & 0xffffffffffull) != 0);
+        if (thr == 0) thr = 1;
+      }
+      // cumulative counts, and masses were every entry at its bin's upper (lower) edge; 1e-4 covers the edges' roundings
+      constexpr int kPer = (kBins + kThr - 1) / kThr;
+      uint32_t n[kPer];
+      double up[kPer], down[kPer];
+      uint32_t nsum = 0;
+      double usum = 0.0, dsum = 0.0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int bin = tid * kPer + j;
+        n[j] = bin < kBins ? tot[bin] : 0u;
+        float a0, a1;  // y at the edges
+        if (kFirst) {
+          a0 = (float)bin * (-1.0f / kBinsOct);
+          a1 = a0 - 1.0f / kBinsOct;
+        } else {
+          const float step = ((float)(uh - ul) + 1.0f) * (1.0f / kBins);
+          a0 = -__uint_as_float(ul + (uint32_t)((float)bin * step)) * cf;
+          a1 = -__uint_as_float(min(uh, ul + (uint32_t)((float)(bin + 1) * step) + 1u)) * cf;
+        }
+        up[j] = n[j] ? (double)((float)n[j] * exp2f((float)kFrac + a0)) * 1.0001 : 0.0;
+        down[j] = n[j] ? (double)((float)n[j] * exp2f((float)kFrac + a1)) * 0.9999 : 0.0;
+        nsum += n[j];
+        usum += up[j];
+        dsum += down[j];
+      }
+      uint32_t nx = nsum;
+      double ux = usum, dx = dsum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t on = __shfl_up_sync(0xffffffffu, nx, o);
+        const double ou = __shfl_up_sync(0xffffffffu, ux, o), od = __shfl_up_sync(0xffffffffu, dx, o);
+        if (lane >= o) {
+          nx += on;
+          ux += ou;
+          dx += od;
+        }
+      }
+      if (lane == 31) {
+        s.redc[warp] = nx;
+        s.redd[warp] = ux;
+        s.rede[warp] = dx;
+      }
+      __syncthreads();
+      {
+        nx += __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u) - nsum;
+        double bu = lane < warp ? s.redd[lane % kWrp] : 0.0, bd = lane < warp ? s.rede[lane % kWrp] : 0.0;
+        for (int o = 8; o > 0; o >>= 1) {
+          bu += __shfl_xor_sync(0xffffffffu, bu, o);
+          bd += __shfl_xor_sync(0xffffffffu, bd, o);
+        }
+        ux += __shfl_sync(0xffffffffu, bu, 0) - usum;
+        dx += __shfl_sync(0xffffffffu, bd, 0) - dsum;
+      }
+      const double need = (double)(thr - above);
+      int lo_mine = kBins, hi_mine = kBins;
+      uint32_t before_lo = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int bin = tid * kPer + j;
+        const uint32_t n0 = nx;
+        nx += n[j];
+        ux += up[j];
+        dx += down[j];
+        const bool by_k = n[j] && nx >= k - cnt_above;
+        if (lo_mine == kBins && (by_k || (n[j] && need_p && ux >= need))) {
+          lo_mine = bin;
+          before_lo = n0;
+        }
+        if (hi_mine == kBins && (by_k || (n[j] && need_p && dx >= need))) hi_mine = bin;
+      }
+      if (lo_mine < kBins) atomicMin(&s.lo, lo_mine);
+      if (hi_mine < kBins) atomicMin(&s.hi, hi_mine);
+      __syncthreads();
+      const int lo = s.lo, hi = s.hi;
+      if (lo_mine == lo && lo < kBins) s.cnt_before = before_lo;  // (one thread)
+      // the masses of entries before the cut's bins (gathered, so that every lane has one to evaluate), and the candidates
+      uint32_t waiting = 0, least = 0xffffffffu, largest = 0;
+      float* few = s.few[warp];
+      auto add_up = [&](uint32_t count) {
+        waiting -= count;
+        __syncwarp();
+        if (lane < count) seg_mass += mass(few[waiting + lane]);
+        __syncwarp();
+      };
+      for (uint32_t i0 = s0; i0 < s1; i0 += 128) {
+        const uint32_t i = i0 + 4 * lane;
+        const float4 x = i < s1 ? *reinterpret_cast<const float4*>(key + i)
+                                : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        const float d[4] = {d_of(x.x), d_of(x.y), d_of(x.z), d_of(x.w)};
+        int bin[4];
+        uint32_t early[4];
+        bool some = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bin[j] = inside(d[j]) ? bin_of(d[j]) : kBins + 1;
+          early[j] = __ballot_sync(0xffffffffu, bin[j] < lo);
+          some |= bin[j] >= lo && bin[j] <= hi;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (bin[j] < lo) few[waiting + __popc(early[j] & ((1u << lane) - 1u))] = d[j];
+          waiting += __popc(early[j]);
+        }
+        while (waiting >= 32) add_up(32);
+        if (some) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (bin[j] >= lo && bin[j] <= hi) {
+              const uint32_t u = u_of(d[j]), at = atomicAdd(&s.cand_n, 1u);
+              least = min(least, u);
+              largest = max(largest, u);
+              // (in the place of the histograms, which every CTA has read)
+              if (at < kMine) mine[at] = Cand{u, v0 + i + j, mass(d[j])};
+            }
+        }
+      }
+      if (waiting) add_up(waiting);
+      const u64 level_mass = warp_sum(seg_mass);  // with the levels before
+      const u64 x = cta_sum(level_mass, s.seg, warp, lane);
       push(s.above, x);
       push(s.ncand, s.cand_n);
-    }
-    cluster.sync();
-    u64 above = 0;
-    uint32_t cand = 0, before = 0, most = 0;
-    uint32_t in[kCl];  // candidates of each CTA
-#pragma unroll
-    for (int r = 0; r < kCl; ++r) {
-      above += s.above[r];
-      in[r] = s.ncand[r];
-    }
-    auto recount_candidates = [&] {
+      least = __reduce_min_sync(0xffffffffu, least);
+      largest = __reduce_max_sync(0xffffffffu, largest);
+      if (lane == 0) {
+        s.redc[warp] = least;
+        s.rede[warp] = (double)largest;
+      }
+      __syncthreads();
+      push(s.umin, __reduce_min_sync(0xffffffffu, s.redc[lane % kWrp]));
+      push(s.umax, __reduce_max_sync(0xffffffffu, (uint32_t)s.rede[lane % kWrp]));
+      if (lo < kBins) cnt_above += s.cnt_before;
+      cluster.sync();
+      above = 0;
       cand = before = most = 0;
+      uint32_t nl = 0xffffffffu, nh = 0;
 #pragma unroll
       for (int r = 0; r < kCl; ++r) {
+        above += s.above[r];
+        in[r] = s.ncand[r];
         if (r < (int)rank) before += in[r];
         cand += in[r];
         most = max(most, in[r]);
+        nl = min(nl, s.umin[r]);
+        nh = max(nh, s.umax[r]);
       }
+      const bool all_allowed = lo == kBins;
+      if (!all_allowed) {
+        ul = nl;
+        uh = umax = nh;
+      }
+      return all_allowed || (cand <= kCand && most <= kMine);
     };
-    recount_candidates();
-    uint32_t cnt_above = s.cnt_above;
-    bool recount = false;  // the segments' masses are summed anew
-    bool struck = false;
-    if (cand > kCand || most > kMine) {
-      // bisect the keys of the bins [lo, hi]: entries with u < ul are allowed, entries with u > uh are not
-      uint32_t ul = 0, uh = 0x7f7fffffu;
-      int turn = 0;
-      recount = true;
-      auto inside = [&](float d) {
-        const uint32_t u = u_of(d);
-        const int bin = bin_of(d);
-        return u >= ul && u <= uh && bin >= lo && bin <= hi && d >= dlow;
-      };
-      while (ul < uh && (cand > kCand || most > kMine)) {
-        const uint32_t mid = ul + (uh - ul) / 2;
-        uint32_t cl = 0;
-        u64 ml = 0;
-        each([&](uint32_t, float d) {
-          if (u_of(d) > mid || !inside(d)) return;
-          ++cl;
-          ml += mass(d);
-        });
-        push(s.it_cnt[turn], cta_sum(__reduce_add_sync(0xffffffffu, cl), s.redc, warp, lane));
-        push(s.it_mass[turn], cta_sum(warp_sum(ml), s.red, warp, lane));
-        cluster.sync();
-        uint32_t got[kCl];
-        cl = 0;
-        ml = 0;
-#pragma unroll
-        for (int r = 0; r < kCl; ++r) {
-          got[r] = s.it_cnt[turn][r];
-          cl += got[r];
-          ml += s.it_mass[turn][r];
-        }
-        turn ^= 1;
-        const bool down = cnt_above + cl >= k || above + ml >= thr;
-        if (down) {
-          uh = mid;
-        } else {
-          ul = mid + 1;
-          cnt_above += cl;
-          above += ml;
-        }
-#pragma unroll
-        for (int r = 0; r < kCl; ++r) in[r] = down ? got[r] : in[r] - got[r];
-        recount_candidates();
-      }
-      umax = uh;
-      if (cand <= kCand && most <= kMine) {
-        // collect the candidates again, from the narrowed range
-        __syncthreads();
-        if (tid == 0) s.cand_n = 0;
-        __syncthreads();
-        each([&](uint32_t i, float d) {
-          if (!inside(d)) return;
-          mine[atomicAdd(&s.cand_n, 1u)] = Cand{u_of(d), v0 + i, mass(d)};
-        });
-        cluster.sync();
-      } else {
+    bool done = look(std::true_type{});
+    for (int level = 1; !done; ++level) {
+      if (ul == uh) {
         // one key value: its `stay` lowest indices are allowed
         struck = true;
         const u64 w = mass(-__uint_as_float(ul));
@@ -464,10 +476,12 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           ties += __popc(__ballot_sync(0xffffffffu, i < s1 && u_of(d_of(key[i])) == ul));
         }
         const uint32_t all_ties = cta_sum(ties, s.redc, warp, lane);
-        uint32_t rank_in = __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u);
+        const uint32_t first_rank = __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u);
         push(s.ties, all_ties);
         cluster.sync();
+        u64 rank_in = first_rank;
         for (int r = 0; r < (int)rank; ++r) rank_in += s.ties[r];
+        if (lane == 0 && rank_in < stay) seg_mass += min((u64)ties, stay - rank_in) * w;
         for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
           const uint32_t i = i0 + lane;
           const bool tie = i < s1 && u_of(d_of(key[i])) == ul;
@@ -475,8 +489,46 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           if (tie && rank_in + __popc(bal & ((1u << lane) - 1u)) >= stay) key[i] = -INFINITY;
           rank_in += __popc(bal);
         }
+        break;
       }
+      if (level > 1 && uh - ul > span / 2) {
+        // the masses' bounds did not separate them (one entry outweighs the others): the exact ones halve the range
+        const uint32_t mid = ul + (uh - ul) / 2;
+        uint32_t cl = 0;
+        u64 ml = 0;
+        each([&](uint32_t, float d) {
+          if (d < dlow || u_of(d) < ul || u_of(d) > mid) return;
+          ++cl;
+          ml += mass(d);
+        });
+        push(s.ncand, cta_sum(__reduce_add_sync(0xffffffffu, cl), s.redc, warp, lane));
+        push(s.total, cta_sum(warp_sum(ml), s.red, warp, lane));
+        cluster.sync();
+        uint32_t count = 0;
+        u64 sum = 0;
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) {
+          count += s.ncand[r];
+          sum += s.total[r];
+        }
+        if (cnt_above + count >= k || above + sum >= thr) {
+          uh = umax = mid;
+        } else {
+          ul = mid + 1;
+          cnt_above += count;
+          above += sum;
+          seg_mass += ml;
+        }
+      }
+      span = uh - ul;
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
+      __syncthreads();
+      done = look(std::false_type{});
     }
+    seg_mass = warp_sum(seg_mass);
+    __syncthreads();
+    if (lane == 0) s.seg[warp] = seg_mass;
     if (!struck && cand > 0) {
       // The candidates' key range in kSub parts, with exact counts and masses: the cut falls into one part, and only its
       // members are ranked one against the other.
@@ -484,40 +536,23 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         s.sub_mass[i] = 0;
         s.sub_cnt[i] = 0;
       }
-      if (tid == 0) {
-        s.umin = 0xffffffffu;
-        s.umax = 0;
-        s.cut_n = 0;
-      }
+      if (tid == 0) s.cut_n = 0;
       __syncthreads();
+      const uint32_t u0 = ul;
+      const float per = (float)kSub / ((float)(uh - ul) + 1.0f);
+      auto part_of = [&](uint32_t u) { return min(kSub - 1, (int)((float)(u - u0) * per)); };  // ascends with u
       // (mine lies behind `all`, so the copies do not touch what other CTAs read)
-      uint32_t least = 0xffffffffu, largest = 0;
 #pragma unroll 1
       for (int r = 0, at = 0; r < kCl; ++r) {
         const Cand* theirs = cluster.map_shared_rank(mine, r);
         for (uint32_t i = tid; i < in[r]; i += kThr) {
           const Cand x = theirs[i];
           all[at + i] = x;
-          least = min(least, x.u);
-          largest = max(largest, x.u);
+          const int p = part_of(x.u);
+          atomicAdd(&s.sub_cnt[p], 1u);
+          atomicAdd(&s.sub_mass[p], x.w);
         }
         at += in[r];
-      }
-      least = __reduce_min_sync(0xffffffffu, least);
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      if (lane == 0) {
-        atomicMin(&s.umin, least);
-        atomicMax(&s.umax, largest);
-      }
-      __syncthreads();
-      const uint32_t u0 = s.umin;
-      const float per = (float)kSub / ((float)(s.umax - u0) + 1.0f);
-      auto part_of = [&](uint32_t u) { return min(kSub - 1, (int)((float)(u - u0) * per)); };  // ascends with u
-      for (uint32_t i = tid; i < cand; i += kThr) {
-        const Cand x = all[i];
-        const int p = part_of(x.u);
-        atomicAdd(&s.sub_cnt[p], 1u);
-        atomicAdd(&s.sub_mass[p], x.w);
       }
       __syncthreads();
       // every warp: two parts a lane, cumulative; the first part that reaches top-k or top-p holds the cut
@@ -577,20 +612,12 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         }
         if (!allowed)
           key[me.idx - v0] = -INFINITY;
-        else if (!recount)
+        else
           atomicAdd(&s.seg[(me.idx - v0) / seg], me.w);
       }
     }
     __syncthreads();
-    if (recount) {
-      seg_mass = 0;
-      each([&](uint32_t, float d) {
-        if (d >= dlow && bin_of(d) <= hi && u_of(d) <= umax) seg_mass += mass(d);
-      });
-      seg_mass = warp_sum(seg_mass);
-    } else {
-      seg_mass = s.seg[warp];
-    }
+    seg_mass = s.seg[warp];
   }
 
   // ---- 3. the token
@@ -622,7 +649,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   const uint32_t e0 = min(g1, g0 + tid * per), e1 = min(g1, e0 + per);
   auto mass_at = [&](uint32_t i) -> u64 {
     const float d = d_of(key[i]);
-    return d >= dlow && bin_of(d) <= hi && u_of(d) <= umax ? mass(d) : 0ull;
+    return d >= dlow && u_of(d) <= umax ? mass(d) : 0ull;
   };
   u64 own = 0;
   for (uint32_t i = e0; i < e1; ++i) own += mass_at(i);

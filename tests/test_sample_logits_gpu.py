@@ -88,6 +88,18 @@ def test_flat_rows_bisect_the_keys(ctx, sample):
         check(ctx, sample, logits, uniforms(4, 8), **kw)
 
 
+def test_one_entry_outweighs_thousands(ctx, sample):
+    """The cut lies among entries whose whole mass is a rounding of the first one's: bounds on masses cannot find it."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    logits = torch.rand(5, 40000, device="cuda", generator=g) - 20.0
+    logits[:, 17] = 0.0
+    rest = float(torch.exp(logits[0].double()).sum() - 1.0)
+    for part in (0.1, 0.5, 0.9, 0.999):
+        p = np.float32((1.0 + part * rest) / (1.0 + rest))
+        assert p < 1
+        check(ctx, sample, logits, torch.tensor([0.0, 0.5, 1 - 1e-6, 1 - 1e-7, 1 - 2.0**-53], dtype=torch.float64).cuda(), top_p=p)
+
+
 def test_masks_infinities_and_nan(ctx, sample):
     logits = gaussian(9, 3001, 6)
     logits[0] = -math.inf                       # nothing left

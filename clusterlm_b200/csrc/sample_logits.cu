@@ -64,23 +64,20 @@ struct SampleArgs {
   int vec;  // rows and slices start 16-byte aligned
 };
 
-// round(2^44 * 2^y) for -45.6 < y <= 0: 2^y = 2^n 2^f with |f| <= 1/2 and a degree-8 polynomial for 2^f (least maximum
-// relative error by weighted least squares: 7.8e-13).
-__device__ __forceinline__ u64 mass_of(double y) {
-  constexpr double kShift = 0x1.8p52;
-  const double k = y + kShift;
+// round(2^44 * 2^y) for -45.6 < y <= 0: 2^y = 2^n 2^(j / 64) 2^f with |f| <= 1/128, a table of the 2^(j / 64) and a
+// degree-3 polynomial for 2^f (least maximum relative error by weighted least squares: 4.5e-12).  Eight double
+// operations; a polynomial alone takes thirteen and measured 12% slower in the passes that evaluate every entry.
+__device__ __forceinline__ u64 mass_of(double y, const double* table) {
+  constexpr double kShift = 0x1.8p52, kShift64 = 0x1.8p46;
+  const double k = y + kShift64;
   const int n = (int)(unsigned)__double_as_longlong(k);
-  const double f = y - (k - kShift);
-  double p = 0x1.61afce9c47e39p-20;
-  p = fma(p, f, 0x1.00dad250307efp-16);
-  p = fma(p, f, 0x1.430acca365ca2p-13);
-  p = fma(p, f, 0x1.5d87483855d48p-10);
-  p = fma(p, f, 0x1.3b2ab5c52912fp-7);
-  p = fma(p, f, 0x1.c6b08dd46d38ep-5);
-  p = fma(p, f, 0x1.ebfbdff9319e2p-3);
-  p = fma(p, f, 0x1.62e42fef8615ep-1);
-  p = fma(p, f, 0x1.ffffffffff7a3p-1);
-  const double scale = __hiloint2double((1023 + kFrac + n) << 20, 0);
+  const double f = y - (k - kShift64);
+  double p = 0x1.c6b0616cd9777p-5;
+  p = fma(p, f, 0x1.ebfc2ec2e07ffp-3);
+  p = fma(p, f, 0x1.62e42fefb2b20p-1);
+  p = fma(p, f, 0x1.fffffffff626bp-1);
+  const double t = table[n & 63];
+  const double scale = __hiloint2double(__double2hiint(t) + (((n >> 6) + kFrac) << 20), __double2loint(t));
   return (u64)(__double_as_longlong(fma(p, scale, kShift)) - __double_as_longlong(kShift));
 }
 
@@ -106,10 +103,11 @@ struct Shared {
   u64 seg[kWrp];      // allowed mass of the warp segments
   u64 red[kWrp];
   uint32_t redc[kWrp];
-  double redd[kWrp], rede[kWrp];
+  float redf[2][kWrp];
   u64 sub_mass[kSub];
   uint32_t sub_cnt[kSub];
   uint32_t cand_n, cut_n;
+  double table[64];     // 2^(j / 64)
   float few[kWrp][160];  // entries whose masses a warp has yet to sum
   int lo, hi;
   uint32_t cnt_before;
@@ -181,13 +179,13 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
   for (uint32_t i = cnt + tid; i < a.slice; i += kThr) key[i] = -INFINITY;
   for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
-  if (tid == 0) s.cand_n = 0;
+  if (tid < 64) s.table[tid] = exp2(tid / 64.0);
   const float T = a.temp ? a.temp[row] : 1.0f;
   const bool greedy = !(T > 0.0f);
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) s.redd[warp] = mx;
+  if (lane == 0) s.redf[0][warp] = mx;
   __syncthreads();
-  mx = (float)s.redd[lane % kWrp];
+  mx = s.redf[0][lane % kWrp];
   for (int o = kWrp / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   uint32_t first = 0xffffffffu;  // lowest index of the slice's maximum (greedy rows)
   if (greedy) {
@@ -233,7 +231,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
   auto d_of = [&](float x) { return x == M ? 0.0f : __fsub_rn(x, M); };
   auto mass = [&](float d) {  // of any entry
-    const u64 w = mass_of((double)fmaxf(d, dcut) * c);
+    const u64 w = mass_of((double)fmaxf(d, dcut) * c, s.table);
     return d >= dcut ? w : 0ull;
   };
   auto u_of = [&](float d) { return __float_as_uint(fabsf(d)); };  // ascends as the order does
@@ -310,36 +308,36 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         thr = (ph << 24 | pl >> 40) + ((pl & 0xffffffffffull) != 0);
         if (thr == 0) thr = 1;
       }
-      // cumulative counts, and masses were every entry at its bin's upper (lower) edge; 1e-4 covers the edges' roundings
+      // cumulative counts, and masses were every entry at its bin's upper (lower) edge; 1e-4 covers the roundings of
+      // the edges and of these f32 sums, which only bound where the cut can be
       constexpr int kPer = (kBins + kThr - 1) / kThr;
+      auto edge = [&](int bin) {  // e at a bin's upper edge, in units of 2^-44
+        if (kFirst) return exp2f((float)kFrac - (float)bin * (1.0f / kBinsOct));
+        const float step = ((float)(uh - ul) + 1.0f) * (1.0f / kBins);
+        return exp2f((float)kFrac - __uint_as_float(min(uh, ul + (uint32_t)((float)bin * step) + (bin > 0))) * cf);
+      };
       uint32_t n[kPer];
-      double up[kPer], down[kPer];
+      float up[kPer], down[kPer];
       uint32_t nsum = 0;
-      double usum = 0.0, dsum = 0.0;
+      float usum = 0.0f, dsum = 0.0f;
+      float top = edge(tid * kPer);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int bin = tid * kPer + j;
+        const float next = edge(bin + 1);
         n[j] = bin < kBins ? tot[bin] : 0u;
-        float a0, a1;  // y at the edges
-        if (kFirst) {
-          a0 = (float)bin * (-1.0f / kBinsOct);
-          a1 = a0 - 1.0f / kBinsOct;
-        } else {
-          const float step = ((float)(uh - ul) + 1.0f) * (1.0f / kBins);
-          a0 = -__uint_as_float(ul + (uint32_t)((float)bin * step)) * cf;
-          a1 = -__uint_as_float(min(uh, ul + (uint32_t)((float)(bin + 1) * step) + 1u)) * cf;
-        }
-        up[j] = n[j] ? (double)((float)n[j] * exp2f((float)kFrac + a0)) * 1.0001 : 0.0;
-        down[j] = n[j] ? (double)((float)n[j] * exp2f((float)kFrac + a1)) * 0.9999 : 0.0;
+        up[j] = n[j] ? (float)n[j] * top * 1.0001f : 0.0f;
+        down[j] = n[j] ? (float)n[j] * next * 0.9999f : 0.0f;
+        top = next;
         nsum += n[j];
         usum += up[j];
         dsum += down[j];
       }
       uint32_t nx = nsum;
-      double ux = usum, dx = dsum;
+      float ux = usum, dx = dsum;
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t on = __shfl_up_sync(0xffffffffu, nx, o);
-        const double ou = __shfl_up_sync(0xffffffffu, ux, o), od = __shfl_up_sync(0xffffffffu, dx, o);
+        const float ou = __shfl_up_sync(0xffffffffu, ux, o), od = __shfl_up_sync(0xffffffffu, dx, o);
         if (lane >= o) {
           nx += on;
           ux += ou;
@@ -348,21 +346,21 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       }
       if (lane == 31) {
         s.redc[warp] = nx;
-        s.redd[warp] = ux;
-        s.rede[warp] = dx;
+        s.redf[0][warp] = ux;
+        s.redf[1][warp] = dx;
       }
       __syncthreads();
       {
         nx += __reduce_add_sync(0xffffffffu, lane < warp ? s.redc[lane % kWrp] : 0u) - nsum;
-        double bu = lane < warp ? s.redd[lane % kWrp] : 0.0, bd = lane < warp ? s.rede[lane % kWrp] : 0.0;
-        for (int o = 8; o > 0; o >>= 1) {
+        float bu = lane < warp ? s.redf[0][lane % kWrp] : 0.0f, bd = lane < warp ? s.redf[1][lane % kWrp] : 0.0f;
+        for (int o = kWrp / 2; o > 0; o >>= 1) {
           bu += __shfl_xor_sync(0xffffffffu, bu, o);
           bd += __shfl_xor_sync(0xffffffffu, bd, o);
         }
         ux += __shfl_sync(0xffffffffu, bu, 0) - usum;
         dx += __shfl_sync(0xffffffffu, bd, 0) - dsum;
       }
-      const double need = (double)(thr - above);
+      const float need = (float)(thr - above);
       int lo_mine = kBins, hi_mine = kBins;
       uint32_t before_lo = 0;
 #pragma unroll
@@ -434,11 +432,11 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       largest = __reduce_max_sync(0xffffffffu, largest);
       if (lane == 0) {
         s.redc[warp] = least;
-        s.rede[warp] = (double)largest;
+        s.redf[0][warp] = __uint_as_float(largest);
       }
       __syncthreads();
       push(s.umin, __reduce_min_sync(0xffffffffu, s.redc[lane % kWrp]));
-      push(s.umax, __reduce_max_sync(0xffffffffu, (uint32_t)s.rede[lane % kWrp]));
+      push(s.umax, __reduce_max_sync(0xffffffffu, __float_as_uint(s.redf[0][lane % kWrp])));
       if (lo < kBins) cnt_above += s.cnt_before;
       cluster.sync();
       above = 0;
@@ -541,18 +539,24 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       const uint32_t u0 = ul;
       const float per = (float)kSub / ((float)(uh - ul) + 1.0f);
       auto part_of = [&](uint32_t u) { return min(kSub - 1, (int)((float)(u - u0) * per)); };  // ascends with u
-      // (mine lies behind `all`, so the copies do not touch what other CTAs read)
-#pragma unroll 1
-      for (int r = 0, at = 0; r < kCl; ++r) {
-        const Cand* theirs = cluster.map_shared_rank(mine, r);
-        for (uint32_t i = tid; i < in[r]; i += kThr) {
+      // Every CTA's candidates, a warp or two per CTA.  (mine lies behind `all`, so the copies do not touch what other
+      // CTAs read.)
+      const bool direct = cand <= 64;  // few enough to be ranked at once
+      {
+        uint32_t at = 0;
+        const int from = warp % kCl;
+#pragma unroll
+        for (int r = 0; r < kCl; ++r) at += r < from ? in[r] : 0u;
+        const Cand* theirs = cluster.map_shared_rank(mine, from);
+        for (uint32_t i = warp / kCl * 32 + lane; i < s.ncand[from]; i += 32 * (kWrp / kCl)) {
           const Cand x = theirs[i];
           all[at + i] = x;
-          const int p = part_of(x.u);
-          atomicAdd(&s.sub_cnt[p], 1u);
-          atomicAdd(&s.sub_mass[p], x.w);
+          if (!direct) {
+            const int p = part_of(x.u);
+            atomicAdd(&s.sub_cnt[p], 1u);
+            atomicAdd(&s.sub_mass[p], x.w);
+          }
         }
-        at += in[r];
       }
       __syncthreads();
       // every warp: two parts a lane, cumulative; the first part that reaches top-k or top-p holds the cut
@@ -574,31 +578,33 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       const bool at1 = cx >= k || wx >= thr, at0 = cx - c1 >= k || wx - w1 >= thr;
       const uint32_t reach = __ballot_sync(0xffffffffu, at1);
       int cut = kSub;  // no part reaches it: all candidates are allowed
-      uint32_t cb = 0;
-      u64 mb = 0;
-      if (reach) {
+      uint32_t cb = cnt_above;
+      u64 mb = above;
+      if (reach && !direct) {
         const int l = __ffs(reach) - 1;
         const bool low = __shfl_sync(0xffffffffu, at0, l);
         cut = 2 * l + (low ? 0 : 1);
         cb = __shfl_sync(0xffffffffu, low ? cx - c1 - c0 : cx - c1, l);
         mb = __shfl_sync(0xffffffffu, low ? wx - w1 - w0 : wx - w1, l);
       }
-      // the cut part's members, in the place of this CTA's candidates (which every CTA has read: the barrier)
-      cluster.sync();
-      for (uint32_t i = tid; i < cand; i += kThr)
-        if (part_of(all[i].u) == cut) {
-          const uint32_t at = atomicAdd(&s.cut_n, 1u);
-          if (at < kMine) mine[at] = all[i];
-        }
-      __syncthreads();
-      const uint32_t members = s.cut_n;
+      if (!direct) {
+        // the cut part's members, in the place of this CTA's candidates (which every CTA has read: the barrier)
+        cluster.sync();
+        for (uint32_t i = tid; i < cand; i += kThr)
+          if (part_of(all[i].u) == cut) {
+            const uint32_t at = atomicAdd(&s.cut_n, 1u);
+            if (at < kMine) mine[at] = all[i];
+          }
+        __syncthreads();
+      }
+      const uint32_t members = direct ? cand : s.cut_n;
       const bool few = members <= kMine;
-      const Cand* rivals = few ? mine : all;
-      for (uint32_t i = tid; i < in[rank]; i += kThr) {
+      const Cand* rivals = few && !direct ? mine : all;
+      for (uint32_t i = tid; i < s.ncand[rank]; i += kThr) {
         const Cand me = all[before + i];
         const int p = part_of(me.u);
-        bool allowed = p < cut;
-        if (p == cut) {
+        bool allowed = p < cut && !direct;
+        if (p == cut || direct) {
           uint32_t nb = cb;
           u64 wb = mb;
 #pragma unroll 4

@@ -1098,10 +1098,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
   if (second) griddep_wait();
 }
 
-// One warp per (row, head): the row's partials of its group's item and of its own, combined by their maxima.  Lane k
-// looks up partial k (32 at a time) and its maximum and sum, then the lanes share the outputs' columns.
+// One warp per (row, head): the row's partials of its group's item (found by lanes 0..15) and of its own (lanes 16..31),
+// combined by their maxima.  A lane looks up a partial and its maximum and sum; then the lanes share the outputs' columns.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constant__ Args a) {
   using TL = Tile<HD>;
   constexpr int N = HD / 32;  // outputs per lane
   const int lane = threadIdx.x % 32;
@@ -1109,94 +1109,92 @@ __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__
   if (id >= (uint32_t)(a.seqs.n * a.positions) * a.nh) return;
   const int head = (int)(id % a.nh), row = (int)(id / a.nh);
   const int b = row / a.positions, kvh = head / a.group;
-  const int grp = group_of(a, b);
+  const int k = lane / 16;  // kind
+  const int e = k == 0 ? group_of(a, b) : a.groups.n + b;
+  const Args::Kind& kind = a.kind[k];
+  // the item of the row, and its row in a segment
+  Entry en;
+  int tile = 0, r = 0;
+  bool pair = false;
+  if (e >= 0) {
+    en = entry_of(a, e);
+    const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
+    tile = kind.tile ? kvh * en.tiles + x / kRowTile : kvh;
+    r = kind.tile ? x % 128 : x;
+    // in a tile of more than 128 rows a row has one partial a segment, that of its stream; else one of each stream
+    pair = kind.tile && min(en.rows - x / kRowTile * kRowTile, kRowTile) > 128;
+    if (pair) r += x % kRowTile / 128 * kind.rows;
+  }
+  const uint32_t per = kind.tile && !pair ? 2 : 1, seg_rows = kind.tile ? 2 * kind.rows : kind.rows;
+  const uint32_t item = e >= 0 ? items_before(a, e) + tile : 0;
   griddep_wait();
   griddep_launch();
-  const bool idle = a.seqs.base(b) < 0;
-  // the partials: those of the group's item, then those of the sequence's
-  struct Part {
-    Shares shares;
-    uint32_t u0, wt, pages, c0, n, per;  // first unit, units a page, pages, first share, partials, partials a share
-    int first;                            // stream of the row's partial where a share has one
-    const float* row;                     // the row in the partial of (share 0, stream 0)
-    uint32_t half;                        // rows between a segment's halves
-  };
-  auto find = [&](int k) {
-    const int e = k == 0 ? grp : a.groups.n + b;
-    const Args::Kind& kind = a.kind[k];
-    Part p{Shares{0, 1, 0}, 0, 1, 1, 0, 0, 1, 0, nullptr, 0};
-    if (e < 0 || idle) return p;
+  uint32_t n = 0, c0 = 0, u0 = 0, pages = 0, wt = 1;
+  Shares shares{0, 1, 0};
+  if (e >= 0 && a.seqs.base(b) >= 0) {
+    pages = kind.plan->pages[e];
     const uint32_t cum = kind.plan->cum[e];
-    const int pages = kind.plan->pages[e];
-    p.shares = kind.plan->cut();
-    if (pages == 0) return p;
-    const Entry en = entry_of(a, e);
-    const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
-    int tile = kvh, r = x;
-    p.pages = pages;
-    p.wt = en.weight;
-    uint32_t rows = kind.rows;  // of a segment
-    if (kind.tile) {
-      tile = kvh * en.tiles + x / kRowTile;
-      p.per = min(en.rows - x / kRowTile * kRowTile, kRowTile) > 128 ? 1 : 2;
-      p.first = p.per == 1 ? x % kRowTile / 128 : 0;
-      p.half = rows;
-      rows *= 2;
-      r = x % 128;
+    shares = kind.plan->cut();
+    if (pages > 0) {
+      wt = en.weight;
+      u0 = cum + tile * pages * wt;
+      c0 = shares.of(u0);
+      n = (shares.of(u0 + (pages - 1) * wt) - c0 + 1) * per;
     }
-    p.u0 = cum + tile * p.pages * p.wt;
-    p.c0 = p.shares.of(p.u0);
-    p.n = (p.shares.of(p.u0 + (p.pages - 1) * p.wt) - p.c0 + 1) * p.per;
-    p.row = kind.part + ((size_t)(items_before(a, e) + tile) * rows + r) * TL::kRow;
-    return p;
-  };
-  const Part part[2] = {find(0), find(1)};
-  const uint32_t total = part[0].n + part[1].n;
+  }
+  const uint32_t rounds = __reduce_max_sync(0xffffffffu, (n + 15) / 16);
   float M = -INFINITY, l = 0.0f, acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-  for (uint32_t k0 = 0; k0 < total; k0 += 32) {
-    const float* src = nullptr;  // this lane's partial
+  for (uint32_t round = 0; round < rounds; ++round) {
+    const uint32_t i = 16 * round + lane % 16;
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (k0 + lane < total) {
-      const bool own = k0 + lane >= part[0].n;
-      const Part& p = own ? part[1] : part[0];
-      const Args::Kind& kind = a.kind[own ? 1 : 0];
-      const uint32_t k = own ? k0 + lane - part[0].n : k0 + lane;
-      const uint32_t c = p.c0 + k / p.per, s = p.per == 1 ? p.first : k % 2;
-      // pages of the item that share c holds (none, where it is narrower than a page's units; stream 1 of a tile
-      // that alternates: two or more)
-      const uint32_t w0 = max(p.shares.begin(c), p.u0) - p.u0, w1 = p.shares.begin(c + 1) - p.u0;
-      const uint32_t n = min(p.pages, (w1 + p.wt - 1) / p.wt) - min(p.pages, (w0 + p.wt - 1) / p.wt);
-      if (n > (p.per == 1 ? 0u : s)) {
-        src = p.row + ((size_t)c * (kind.tile ? 2 * p.half : (uint32_t)kind.rows) + s * p.half) * TL::kRow;
-        ml = *reinterpret_cast<const float2*>(src + HD);
-      }
+    uint32_t src = 0;  // the partial's row
+    bool have = false;
+    if (i < n) {
+      const uint32_t c = c0 + i / per, s = i % per;
+      // pages of the item that share c holds (none, where it is narrower than a page's units; the second stream has
+      // some where there are two or more)
+      const uint32_t w0 = max(shares.begin(c), u0) - u0, w1 = shares.begin(c + 1) - u0;
+      have = min(pages, (w1 + wt - 1) / wt) - min(pages, (w0 + wt - 1) / wt) > s;
+      src = (item + c) * seg_rows + s * kind.rows + r;
+      if (have) ml = *reinterpret_cast<const float2*>(kind.part + (size_t)src * TL::kRow + HD);
     }
     float m = fmaxf(M, ml.x);
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float ref = m == -INFINITY ? 0.0f : m;
-    const float keep = exp2f(M - ref), f = exp2f(ml.x - ref);
+    const float keep = ex2(M - ref), f = ex2(ml.x - ref);
     float add = ml.y * f;
     for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
     M = m;
     l = l * keep + add;
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] *= keep;
-    const uint32_t have = __ballot_sync(0xffffffffu, src != nullptr);
-    const int count = (int)min(32u, total - k0);
-#pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-      const float* q = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k));
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-      if (!((have >> k) & 1u)) continue;
-      if constexpr (N == 4) {
-        const float4 o = *reinterpret_cast<const float4*>(q + 4 * lane);
-        acc[0] += o.x * fk, acc[1] += o.y * fk, acc[2] += o.z * fk, acc[3] += o.w * fk;
-      } else {
-        const float2 o = *reinterpret_cast<const float2*>(q + 2 * lane);
-        acc[0] += o.x * fk, acc[1] += o.y * fk;
+    for (int j = 0; j < N; ++j) acc[j] *= keep;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, have); todo;) {
+      float o[4][N], w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // four partials' loads in flight
+        const int from = todo ? __ffs(todo) - 1 : 0;
+        w[q] = todo ? __shfl_sync(0xffffffffu, f, from) : 0.0f;
+        const float* p = (from < 16 ? a.kind[0].part : a.kind[1].part) + (size_t)__shfl_sync(0xffffffffu, src, from) * TL::kRow;
+        if (todo) {
+          if constexpr (N == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + 4 * lane);
+            o[q][0] = v.x, o[q][1] = v.y, o[q][2] = v.z, o[q][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(p + 2 * lane);
+            o[q][0] = v.x, o[q][1] = v.y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) o[q][j] = 0.0f;
+        }
+        todo &= todo - 1;
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += o[q][j] * w[q];
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;

@@ -85,6 +85,7 @@ _SIGS = {
     "clm_b200_engine_info": (_i, [_vp, C.POINTER(_u64), C.POINTER(_u64), C.POINTER(_u32)]),
     "clm_b200_session_open": (_i, [_vp, _u64]),
     "clm_b200_session_close": (_i, [_vp, _u64]),
+    "clm_b200_session_fork": (_i, [_vp, _u64, _u64]),
     "clm_b200_run_window": (_i, [_vp, _u64, _u64, _u32, _vp, _vp, _vp, _vp]),
     "clm_b200_run_window_device": (_i, [_vp, _u64, _u64, _u32, _vp, _vp, _vp, _vp, _vp]),
     "clm_b200_commit": (_i, [_vp, _u64, _u32]),

@@ -27,6 +27,7 @@
 #include "pdl.cuh"
 #include "sampling.cuh"
 #include "gemm_tc.cuh"
+#include "kv_ops.cuh"
 #include "wide.cuh"
 
 namespace clm {
@@ -48,7 +49,8 @@ struct Gemv {
 
 struct Session {
   uint64_t id = 0;
-  std::vector<int32_t> pages;
+  std::vector<int32_t> pages;     // of its context; the leading ones may be shared (clm_b200_session_fork)
+  int slot = -1;                  // its row of the engine's page tables and states
   int32_t* d_pages = nullptr;
   SessionState* d_state = nullptr;
   long long pos = 0;          // committed position as known to the host
@@ -215,7 +217,10 @@ struct LlamaEngine : clm_b200_engine {
   bool prepared = false, weights_ready = false;
   int max_pages = 0;  // pages per session
   int pages_total = 0;
-  std::vector<int32_t> free_pages;
+  std::unique_ptr<PageLedger> ledger;  // which pages are free, how many sessions hold each
+  int32_t* d_tables = nullptr;         // [max_sessions][max_pages] page tables, by slot
+  SessionState* d_states = nullptr;    // [max_sessions]
+  std::vector<int> free_slots;
   // weights
   struct Layer {
     Gemv qkv, o, gu, down;
@@ -273,6 +278,8 @@ struct LlamaEngine : clm_b200_engine {
   float* wpart = nullptr;    // split-K partials of the tensor-core GEMMs
   size_t wpart_floats = 0;
   float* wattn = nullptr;    // attention outputs [W][qd]
+  void* share_work = nullptr;   // attention of sessions that share pages: its workspace
+  size_t share_bytes = 0;
   float* wattn_part = nullptr;  // wide attention: KV-split partials and their tile counters
   size_t wattn_part_floats = 0;
   int* wattn_cnt = nullptr;
@@ -733,10 +740,76 @@ struct LlamaEngine : clm_b200_engine {
   };
   int enqueue_window_wide(Session& s, int q, const int32_t* d_tok, const int32_t* parent, cudaStream_t st) {
     const WideSeg seg{&s, 0, q};
-    return enqueue_window_wide(&seg, 1, q, d_tok, parent, st);
+    return enqueue_window_wide(&seg, 1, q, d_tok, parent, KvGroups{}, st);
+  }
+  // The runs of consecutive segments whose sessions share leading pages (forks of one prompt).  Only full pages of
+  // committed positions are ever shared.
+  static KvGroups shared_groups(const WideSeg* segs, int nseg) {
+    KvGroups g;
+    int at = 0;
+    bool any = false;
+    while (at < nseg) {
+      size_t common = segs[at].s->pages.size();
+      int end = at + 1;
+      for (; end < nseg; ++end) {
+        const std::vector<int32_t>&a = segs[at].s->pages, &b = segs[end].s->pages;
+        size_t n = 0;
+        while (n < common && n < b.size() && a[n] == b[n]) ++n;
+        if (n == 0) break;
+        common = n;
+      }
+      g.start[g.n] = (uint16_t)at;
+      g.pages[g.n] = end - at > 1 ? (uint32_t)common : 0u;
+      any |= end - at > 1;
+      g.start[++g.n] = (uint16_t)end;
+      at = end;
+    }
+    return any ? g : KvGroups{};
+  }
+  // Attention of the segments over the cache, the pages that a group shares read once.
+  KvAttnArgs shared_attention(const WideSeg* segs, int nseg, const KvGroups& groups, const int32_t* parent) const {
+    KvAttnArgs a;
+    a.seqs.tables = d_tables;
+    a.seqs.table_stride = max_pages;
+    a.seqs.pos = reinterpret_cast<const char*>(&d_states[0].pos);
+    a.seqs.pos_stride = sizeof(SessionState);
+    a.seqs.n = nseg;
+    a.seqs.max_pages = max_pages;
+    a.seqs.pool_pages = pages_total;
+    a.seqs.mapped = 1;
+    for (int k = 0; k < nseg; ++k) a.seqs.slot[k] = (uint16_t)segs[k].s->slot;
+    a.groups = groups;
+    a.q = q16;
+    a.ld_q = d.qd();
+    a.out = wattn;
+    a.parent = parent;
+    a.positions = segs[0].q;
+    a.nh = d.nh;
+    a.nkv = d.nkv;
+    a.hd = d.hd;
+    a.type = CLM_DTYPE_F16;
+    a.out_type = CLM_DTYPE_F32;
+    a.scale = (float)(1.0 / sqrt((double)d.hd));
+    a.work = share_work;
+    a.work_bytes = share_bytes;
+    a.sm_count = ctx->sm_count;
+    return a;
+  }
+  // Its workspace (grown outside of captures; captured batched windows hold the old one's address and are dropped).
+  int reserve_shared(const WideSeg* segs, int nseg, const KvGroups& groups) {
+    const size_t need = kv_attention_work(nseg, segs[0].q, d.nh, d.nkv, d.hd, groups, ctx->sm_count);
+    if (need <= share_bytes) return CLM_OK;
+    CLM_CUDA(cudaStreamSynchronize(ctx->stream));
+    drop_batch_graphs();
+    if (share_work) CLM_CUDA(cudaFree(share_work));
+    share_work = nullptr;
+    share_bytes = 0;
+    CLM_CUDA(cudaMalloc(&share_work, need));
+    share_bytes = need;
+    return CLM_OK;
   }
   int enqueue_window_wide(const WideSeg* segs, int nseg, int q, const int32_t* d_tok, const int32_t* parent,
-                          cudaStream_t st) {
+                          const KvGroups& groups, cudaStream_t st) {
     const int P = (q + 15) / 16 * 16;
     const size_t qkv_rows = (size_t)d.qd() + 2 * d.kvd();
     CLM_CHECK(nseg >= 1 && nseg <= kWideAttnMaxSegs, CLM_OUT_OF_RANGE, "wide window: at most 16 sessions");
@@ -767,10 +840,17 @@ struct LlamaEngine : clm_b200_engine {
         ys.p += (size_t)g.row0 * qkv_rows;
         CLM_TRY(launch_wide_rope_kv(ys, g.q, d, rope, pos, g.s->d_pages, parent, qs, kpool[li], vpool[li], st));
       }
-      // one attention launch over every segment (all segments have segs[0].q rows)
-      CLM_TRY(launch_attention_wide(q16, kpool[li], vpool[li], attn_segs, nseg, parent, segs[0].q, d, max_pages,
-                                    wattn_part, wattn_part_floats, wattn_cnt, wattn_tiles, ctx->sm_count, wattn, bad,
-                                    st));
+      // one attention over every segment (all segments have segs[0].q rows)
+      if (groups.n > 0) {
+        KvAttnArgs a = shared_attention(segs, nseg, groups, parent);
+        a.k = kpool[li];
+        a.v = vpool[li];
+        CLM_TRY(launch_kv_attention(a, st));
+      } else {
+        CLM_TRY(launch_attention_wide(q16, kpool[li], vpool[li], attn_segs, nseg, parent, segs[0].q, d, max_pages,
+                                      wattn_part, wattn_part_floats, wattn_cnt, wattn_tiles, ctx->sm_count, wattn, bad,
+                                      st));
+      }
       CLM_TRY(launch_tc_xprep(wattn, q, d.qd(), P, wxh, st));
       CLM_TRY(gemm_wide(L.o, q, wy, st, &y));
       CLM_TRY(launch_wide_norm_prep(y, h, q, d.H, L.ffn_norm, d.eps, P, wxh, st));
@@ -1066,14 +1146,14 @@ struct LlamaEngine : clm_b200_engine {
     s.graphs.clear();
     for (auto& kv : s.flow_phases) cudaFree(kv.second);
     s.flow_phases.clear();
-    if (s.d_pages) cudaFree(s.d_pages);
-    if (s.d_state) cudaFree(s.d_state);
     if (s.d_win) cudaFree(s.d_win);
     if (s.d_dprobs) cudaFree(s.d_dprobs);
     s.d_win = nullptr;
     s.d_dprobs = nullptr;
-    for (int32_t p : s.pages) free_pages.push_back(p);
+    for (int32_t p : s.pages) ledger->release(p);
     s.pages.clear();
+    if (s.slot >= 0) free_slots.push_back(s.slot);
+    s.slot = -1;
     s.d_pages = nullptr;
     s.d_state = nullptr;
   }
@@ -1103,6 +1183,7 @@ struct LlamaEngine : clm_b200_engine {
     free_m(mtp_gu);
     free_m(mtp_down);
     for (void* p : allocations) cudaFree(p);
+    if (share_work) cudaFree(share_work);
     if (pin_in) cudaFreeHost(pin_in);
     if (pin_out) cudaFreeHost(pin_out);
   }
@@ -1556,16 +1637,22 @@ int llama_prepare(LlamaEngine* e) {
   CLM_TRY(e->alloc_t(&e->ctl, 1));
   CLM_CUDA(cudaMemset(e->ctl, 0, sizeof(RoundCtl)));
   CLM_CUDA(cudaMemset(e->zero_counter, 0, sizeof(unsigned long long)));
-  for (size_t li = 0; li < e->layers.size(); ++li) {
+  if (!e->layers.empty()) {  // the layers' pools one behind the other, so that page copies address all of them
+    const size_t layer = page_bytes / sizeof(__half) * e->pages_total;
     __half *k = nullptr, *v = nullptr;
-    CLM_TRY(e->alloc_t(&k, page_bytes / sizeof(__half) * e->pages_total));
-    CLM_TRY(e->alloc_t(&v, page_bytes / sizeof(__half) * e->pages_total));
-    CLM_CUDA(cudaMemset(k, 0, page_bytes * e->pages_total));
-    CLM_CUDA(cudaMemset(v, 0, page_bytes * e->pages_total));
-    e->kpool.push_back(k);
-    e->vpool.push_back(v);
+    CLM_TRY(e->alloc_t(&k, layer * e->layers.size()));
+    CLM_TRY(e->alloc_t(&v, layer * e->layers.size()));
+    CLM_CUDA(cudaMemset(k, 0, layer * e->layers.size() * sizeof(__half)));
+    CLM_CUDA(cudaMemset(v, 0, layer * e->layers.size() * sizeof(__half)));
+    for (size_t li = 0; li < e->layers.size(); ++li) {
+      e->kpool.push_back(k + li * layer);
+      e->vpool.push_back(v + li * layer);
+    }
   }
-  for (int p = e->pages_total - 1; p >= 0; --p) e->free_pages.push_back(p);
+  e->ledger = std::make_unique<PageLedger>((uint32_t)e->pages_total);
+  CLM_TRY(e->alloc_t(&e->d_tables, (size_t)e->spec.max_sessions * e->max_pages));
+  CLM_TRY(e->alloc_t(&e->d_states, e->spec.max_sessions));
+  for (int k = (int)e->spec.max_sessions - 1; k >= 0; --k) e->free_slots.push_back(k);
   CLM_CUDA(cudaStreamSynchronize(e->ctx->stream));
   e->prepared = true;
   return CLM_OK;
@@ -1580,32 +1667,68 @@ int llama_info(const LlamaEngine* e, uint64_t* weight_bytes, uint64_t* state_byt
   return CLM_OK;
 }
 
+static int add_session(LlamaEngine* e, uint64_t id, const Session* parent);
+
 int llama_session_open(LlamaEngine* e, uint64_t id) {
   CLM_TRY(engine_enter(e));
   CLM_CHECK(e->prepared, CLM_FAILED_PRECONDITION, "engine not prepared");
   CLM_CHECK(find_session(e, id) == nullptr, CLM_ALREADY_EXISTS, "session already open");
-  CLM_CHECK((int)e->free_pages.size() >= e->max_pages, CLM_RESOURCE_EXHAUSTED, "max_sessions reached");
+  return add_session(e, id, nullptr);
+}
+
+// A new session: all of its context's pages its own, or (a fork) the parent's full pages shared.
+static int add_session(LlamaEngine* e, uint64_t id, const Session* parent) {
+  const uint32_t shared = parent ? (uint32_t)(parent->pos / kPageTokens) : 0u;
+  CLM_CHECK(!e->free_slots.empty() && e->ledger->free_count() >= (uint32_t)e->max_pages - shared, CLM_RESOURCE_EXHAUSTED,
+            "max_sessions reached");
   auto s = std::make_unique<Session>();
   s->id = id;
-  for (int i = 0; i < e->max_pages; ++i) {
-    s->pages.push_back(e->free_pages.back());
-    e->free_pages.pop_back();
+  s->pages.resize(e->max_pages);
+  for (uint32_t i = 0; i < shared; ++i) {
+    s->pages[i] = parent->pages[i];
+    e->ledger->retain(s->pages[i]);
   }
-  cudaError_t err = cudaMalloc(&s->d_pages, s->pages.size() * sizeof(int32_t));
-  if (err == cudaSuccess) err = cudaMalloc(&s->d_state, sizeof(SessionState));
+  e->ledger->alloc((uint32_t)e->max_pages - shared, s->pages.data() + shared);
+  s->slot = e->free_slots.back();
+  e->free_slots.pop_back();
+  s->d_pages = e->d_tables + (size_t)s->slot * e->max_pages;
+  s->d_state = e->d_states + s->slot;
+  cudaStream_t st = e->ctx->stream;
+  cudaError_t err = cudaMemcpyAsync(s->d_pages, s->pages.data(), s->pages.size() * sizeof(int32_t), cudaMemcpyHostToDevice, st);
   if (err == cudaSuccess)
-    err = cudaMemcpy(s->d_pages, s->pages.data(), s->pages.size() * sizeof(int32_t), cudaMemcpyHostToDevice);
-  if (err == cudaSuccess) err = cudaMemset(s->d_state, 0, sizeof(SessionState));
+    err = parent ? cudaMemcpyAsync(s->d_state, parent->d_state, sizeof(SessionState), cudaMemcpyDeviceToDevice, st)
+                 : cudaMemsetAsync(s->d_state, 0, sizeof(SessionState), st);
   if (err == cudaSuccess && e->spec.role == CLM_ROLE_TAIL && e->has_mtp) {
     // a pipeline tail keeps each session's window and draft distributions across rounds
-    err = cudaMalloc(&s->d_win, (size_t)(e->wmax() + 1) * sizeof(int32_t));
-    if (err == cudaSuccess) err = cudaMemset(s->d_win, 0, (size_t)(e->wmax() + 1) * sizeof(int32_t));
-    if (err == cudaSuccess) err = cudaMalloc(&s->d_dprobs, (size_t)e->wmax() * e->d.V * sizeof(float));
+    const size_t win = (size_t)(e->wmax() + 1) * sizeof(int32_t), probs = (size_t)e->wmax() * e->d.V * sizeof(float);
+    err = cudaMalloc(&s->d_win, win);
+    if (err == cudaSuccess) err = cudaMalloc(&s->d_dprobs, probs);
+    if (err == cudaSuccess)
+      err = parent ? cudaMemcpyAsync(s->d_win, parent->d_win, win, cudaMemcpyDeviceToDevice, st)
+                   : cudaMemsetAsync(s->d_win, 0, win, st);
+    if (err == cudaSuccess && parent)
+      err = cudaMemcpyAsync(s->d_dprobs, parent->d_dprobs, probs, cudaMemcpyDeviceToDevice, st);
   }
-  if (err != cudaSuccess) {
+  int rc = err == cudaSuccess ? CLM_OK : cuda_fail(err, "session_open");
+  if (rc == CLM_OK && parent && !e->layers.empty() && parent->pos % kPageTokens != 0) {
+    // the parent's last page, in every layer
+    KvCopyJob job;
+    job.n = 1;
+    job.src[0] = parent->pages[shared];
+    job.dst[0] = s->pages[shared];
+    const uint64_t page = (uint64_t)e->d.nkv * kPageTokens * e->d.hd * sizeof(__half);
+    rc = launch_kv_copy(e->kpool[0], e->vpool[0], (uint32_t)e->layers.size(), page * e->pages_total, page, job, nullptr, 0,
+                        e->ctx->sm_count, st);
+  }
+  if (rc == CLM_OK) {
+    err = cudaStreamSynchronize(st);
+    if (err != cudaSuccess) rc = cuda_fail(err, "session_open");
+  }
+  if (rc != CLM_OK) {
     e->release_session(*s);
-    return cuda_fail(err, "session_open");
+    return rc;
   }
+  if (parent) s->pos = s->pos_bound = parent->pos;
   e->sessions[id] = std::move(s);
   return CLM_OK;
 }
@@ -1630,6 +1753,17 @@ static int sync_pos(LlamaEngine* e, Session* s) {
   s->pos = s->pos_bound = p;
   s->pos_stale = false;
   return CLM_OK;
+}
+
+int llama_session_fork(LlamaEngine* e, uint64_t parent_id, uint64_t id) {
+  CLM_TRY(engine_enter(e));
+  CLM_CHECK(e->prepared, CLM_FAILED_PRECONDITION, "engine not prepared");
+  Session* parent = find_session(e, parent_id);
+  CLM_CHECK(parent != nullptr, CLM_NOT_FOUND, "session not open");
+  CLM_CHECK(find_session(e, id) == nullptr, CLM_ALREADY_EXISTS, "session already open");
+  CLM_CHECK(parent->outstanding == 0, CLM_FAILED_PRECONDITION, "a window is outstanding for the parent session");
+  CLM_TRY(sync_pos(e, parent));
+  return add_session(e, id, parent);
 }
 
 static int run_window_common(LlamaEngine* e, uint64_t id, uint64_t base, uint32_t q, cudaStream_t st,
@@ -1785,12 +1919,14 @@ int llama_run_batch(LlamaEngine* e, uint32_t n, const uint64_t* ids, const uint6
   if (h_parents != nullptr)
     CLM_CUDA(cudaMemcpyAsync(e->parents, h_parents, q * sizeof(int32_t), cudaMemcpyHostToDevice, st));
   // one CUDA graph per session set (eager on first use, captured on the second, replayed after)
+  const KvGroups groups = LlamaEngine::shared_groups(segs.data(), (int)n);
+  if (groups.n > 0) CLM_TRY(e->reserve_shared(segs.data(), (int)n, groups));
   std::vector<uint64_t> key(ids, ids + n);
   auto& holder = e->batch_graphs[key];
   if (!holder) holder = std::make_unique<Session>();
   const int32_t* par = h_parents ? e->parents : nullptr;
   CLM_TRY(e->run_graph(*holder, 7, (int)Q, h_parents ? 1 : 0, st, [&](cudaStream_t cs) {
-    return e->enqueue_window_wide(segs.data(), (int)n, (int)Q, e->win, par, cs);
+    return e->enqueue_window_wide(segs.data(), (int)n, (int)Q, e->win, par, groups, cs);
   }));
   if (h_logits)
     CLM_CUDA(cudaMemcpyAsync(h_logits, e->logits, (size_t)Q * e->d.V * sizeof(float), cudaMemcpyDeviceToHost, st));

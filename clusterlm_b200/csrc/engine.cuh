@@ -27,6 +27,7 @@ int llama_prepare(LlamaEngine* e);
 int llama_info(const LlamaEngine* e, uint64_t* weight_bytes, uint64_t* state_bytes, uint32_t* fpp);
 int llama_session_open(LlamaEngine* e, uint64_t id);
 int llama_session_close(LlamaEngine* e, uint64_t id);
+int llama_session_fork(LlamaEngine* e, uint64_t parent_id, uint64_t id);
 int llama_run_window_device(LlamaEngine* e, uint64_t id, uint64_t base, uint32_t q, const int32_t* d_tokens,
                             const float* d_in, float* d_out, float* d_logits, void* stream);
 int llama_run_window(LlamaEngine* e, uint64_t id, uint64_t base, uint32_t q, const int32_t* h_tokens, const float* h_in,

@@ -218,6 +218,11 @@ int clm_b200_pipe_status(clm_b200_engine* e, void* stream) {
   return llama_pipe_status(llama(e), stream);
 }
 
+int clm_b200_session_fork(clm_b200_engine* e, uint64_t parent, uint64_t child) {
+  CLM_TRY(llama_only(e));
+  return llama_session_fork(llama(e), parent, child);
+}
+
 int clm_b200_pipe_attach_session(clm_b200_engine* e, uint64_t id, clm_b200_link* in, clm_b200_link* out) {
   CLM_TRY(llama_only(e));
   return llama_pipe_attach_session(llama(e), id, in, out);

@@ -141,6 +141,10 @@ class Engine:
     def close_session(self, session: int):
         call("clm_b200_session_close", self.h, session)
 
+    def fork_session(self, parent: int, child: int):
+        """Opens `child` as a continuation of `parent` at its committed position (clm_b200_session_fork)."""
+        call("clm_b200_session_fork", self.h, parent, child)
+
     def last_launches(self) -> int:
         v = C.c_uint64()
         call("clm_b200_engine_last_launches", self.h, C.byref(v))

@@ -15,16 +15,16 @@ sequence state is private to a domain (runtime/domain/src/reference_domain.cpp:2
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 import numpy as np
 import torch
 
-from ._native import call
+from ._native import call, check, lib
 from .runtime import DTYPES, Context, _operand, _stream_on
 
 _vp = C.c_void_p
 PAGE_TOKENS = 64
+_POOL_TYPES = {torch.float16: 1, torch.bfloat16: 2}  # CLM_DTYPE_*
 
 
 class _Pool(C.Structure):
@@ -41,37 +41,40 @@ class _Rope(C.Structure):
 
 
 def _pool(ctx: Context, k: torch.Tensor, v: torch.Tensor, layers: bool) -> _Pool:
-    kp, vp = _operand(ctx, "k_pool", k), _operand(ctx, "v_pool", v, k.dtype)
-    dims = 5 if layers else 4
-    if k.dtype not in (torch.float16, torch.bfloat16):
+    kp = _operand(ctx, "k_pool", k)
+    dtype, shape = _POOL_TYPES.get(k.dtype), k.shape
+    if dtype is None:
         raise ValueError("k_pool: expected float16 or bfloat16")
-    if k.dim() != dims or k.shape[-2] != PAGE_TOKENS:
+    if len(shape) != 4 + layers or shape[-2] != PAGE_TOKENS:
         raise ValueError(f"k_pool: expected {'(layers, ' if layers else '('}pages, n_kv_heads, 64, head_dim)")
-    if tuple(v.shape) != (*k.shape[:-2], k.shape[-1], PAGE_TOKENS):
-        raise ValueError(f"v_pool: expected {'(layers, ' if layers else '('}pages, n_kv_heads, head_dim, 64)")
-    return _Pool(kp, vp, k.shape[0] if layers else 1, k.shape[-4], k.shape[-3], k.shape[-1], DTYPES[k.dtype])
+    *lead, pages, heads, _, hd = shape
+    vp = _operand(ctx, "v_pool", v, k.dtype, (*lead, pages, heads, hd, PAGE_TOKENS))
+    return _Pool(kp, vp, lead[0] if layers else 1, pages, heads, hd, dtype)
 
 
 def _seqs(ctx: Context, tables: torch.Tensor, pos: torch.Tensor) -> _Seqs:
-    if not isinstance(tables, torch.Tensor) or tables.dim() != 2:
-        raise ValueError("tables: expected (rows, max_pages)")
     tp = _operand(ctx, "tables", tables, torch.int32)
-    return _Seqs(tp, _operand(ctx, "pos", pos, torch.int64, (tables.shape[0],)), *tables.shape)
+    if tables.dim() != 2:
+        raise ValueError("tables: expected (rows, max_pages)")
+    rows, width = tables.shape
+    return _Seqs(tp, _operand(ctx, "pos", pos, torch.int64, (rows,)), rows, width)
 
 
 def _rows(ctx: Context, name: str, t: torch.Tensor, heads, head_dim: int):
     """(address, n, positions, heads, row stride) of rows (n, positions, heads, head_dim): the heads of a row are
     contiguous, and consecutive rows lie a fixed number of elements apart (a slice of a fused projection)."""
     p = _operand(ctx, name, t, contiguous=False)
-    if t.dim() != 4 or t.shape[3] != head_dim or (heads is not None and t.shape[2] != heads):
-        raise ValueError(f"{name}: expected (n, positions, {heads or 'heads'}, {head_dim}), got {tuple(t.shape)}")
-    n, positions, h, d = t.shape
-    if t.numel() == 0:
+    shape = t.shape
+    if len(shape) != 4 or shape[3] != head_dim or (heads is not None and shape[2] != heads):
+        raise ValueError(f"{name}: expected (n, positions, {heads or 'heads'}, {head_dim}), got {tuple(shape)}")
+    n, positions, h, d = shape
+    s0, s1, s2, s3 = t.stride()
+    if n == 0 or positions == 0 or h == 0:
         return p, n, positions, h, h * d
-    if (d > 1 and t.stride(3) != 1) or (h > 1 and t.stride(2) != d):
+    if s3 != 1 or (h > 1 and s2 != d):
         raise ValueError(f"{name}: a row's heads must be contiguous")
-    ld = t.stride(1) if positions > 1 else (t.stride(0) if n > 1 else h * d)
-    if ld < h * d or (n > 1 and positions > 1 and t.stride(0) != positions * ld):
+    ld = s1 if positions > 1 else (s0 if n > 1 else h * d)
+    if ld < h * d or (n > 1 and positions > 1 and s0 != positions * ld):
         raise ValueError(f"{name}: rows must lie a fixed distance apart")
     return p, n, positions, h, ld
 
@@ -130,8 +133,9 @@ def kv_append(ctx: Context, k_pool, v_pool, tables, pos, q, k, v, rope: Rope | N
             out = torch.empty((n, positions, heads, hd), dtype=k_pool.dtype, device=k_pool.device)
         op = _operand(ctx, "out", out, k_pool.dtype, (n, positions, heads, hd))
     r = rope._c(ctx) if rope is not None else None
-    call("clm_b200_kv_append", ctx.h, C.byref(pool), 0, C.byref(seqs), n, positions, heads, DTYPES[k.dtype], qp, ldq, kp,
-         ldk, vp, ldv, None if r is None else C.byref(r), _parents(ctx, parents, positions), op, _stream_on(ctx.device))
+    check(lib.clm_b200_kv_append(ctx.h, C.byref(pool), 0, C.byref(seqs), n, positions, heads, DTYPES[k.dtype], qp, ldq, kp,
+                                 ldk, vp, ldv, None if r is None else C.byref(r), _parents(ctx, parents, positions), op,
+                                 _stream_on(ctx.device)))
     return out if q is not None else None
 
 
@@ -144,29 +148,33 @@ def kv_attention(ctx: Context, k_pool, v_pool, tables, pos, q, groups=None, scal
     pool, seqs = _pool(ctx, k_pool, v_pool, False), _seqs(ctx, tables, pos)
     hd = pool.head_dim
     qp, n, positions, heads, ldq = _rows(ctx, "q", q, None, hd)
-    if q.dtype != k_pool.dtype:
+    if q.dtype is not k_pool.dtype:
         raise ValueError(f"q: expected {k_pool.dtype}, got {q.dtype}")
-    g = list(groups) if groups is not None else []
-    counts, pages = (C.c_uint32 * max(1, len(g)))(), (C.c_uint32 * max(1, len(g)))()
-    for i, (c, p) in enumerate(g):
-        if c < 0 or p < 0:
-            raise ValueError("groups: expected (sequences, pages) of zero or more")
-        counts[i], pages[i] = c, p
+    g, counts, pages = 0, None, None
+    if groups:
+        g = len(groups)
+        for c, p in groups:
+            if not (0 <= c < 2**32 and 0 <= p < 2**32):
+                raise ValueError("groups: expected (sequences, pages) of zero or more")
+        counts, pages = (C.c_uint32 * g)(*[c for c, _ in groups]), (C.c_uint32 * g)(*[p for _, p in groups])
     if out is None:
         out = torch.empty((n, positions, heads, hd), dtype=q.dtype, device=q.device)
     op = _operand(ctx, "out", out, q.dtype, (n, positions, heads, hd))
     need = C.c_uint64()
-    call("clm_b200_kv_attention_workspace", ctx.h, n, positions, heads, pool.n_kv_heads, hd, len(g), counts, pages,
-         C.byref(need))
-    work = torch.empty(need.value, dtype=torch.uint8, device=q.device)  # this call's own: captured graphs keep theirs
-    call("clm_b200_kv_attention", ctx.h, C.byref(pool), 0, C.byref(seqs), n, positions, heads, qp, ldq, len(g), counts,
-         pages, _parents(ctx, parents, positions), 1.0 / math.sqrt(hd) if scale is None else scale, op,
-         _vp(work.data_ptr()), need.value, _stream_on(ctx.device))
+    check(lib.clm_b200_kv_attention_workspace(ctx.h, n, positions, heads, pool.n_kv_heads, hd, g, counts, pages,
+                                              C.byref(need)))
+    need = need.value
+    work = torch.empty(need, dtype=torch.uint8, device=q.device)  # this call's own: captured graphs keep theirs
+    check(lib.clm_b200_kv_attention(ctx.h, C.byref(pool), 0, C.byref(seqs), n, positions, heads, qp, ldq, g, counts, pages,
+                                    _parents(ctx, parents, positions), hd**-0.5 if scale is None else scale, op,
+                                    work.data_ptr(), need, _stream_on(ctx.device)))
     return out
 
 
 def _ints(name: str, a, dtype) -> np.ndarray:
     a = np.asarray(a)
+    if a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:
+        return a
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise ValueError(f"{name}: expected a list of integers")
     lim = np.iinfo(dtype)
@@ -182,8 +190,8 @@ def kv_fork(ctx: Context, k_pools, v_pools, tables, pos, parents, children, new_
     p, c, g = _ints("parents", parents, np.uint32), _ints("children", children, np.uint32), _ints("new_pages", new_pages, np.int32)
     if not p.size == c.size == g.size:
         raise ValueError("parents, children and new_pages: expected one entry per fork")
-    call("clm_b200_kv_fork", ctx.h, C.byref(pool), C.byref(seqs), p.size, p.ctypes.data_as(_vp), c.ctypes.data_as(_vp),
-         g.ctypes.data_as(_vp), _stream_on(ctx.device))
+    check(lib.clm_b200_kv_fork(ctx.h, C.byref(pool), C.byref(seqs), p.size, p.ctypes.data, c.ctypes.data, g.ctypes.data,
+                               _stream_on(ctx.device)))
 
 
 def kv_copy_pages(ctx: Context, k_pools, v_pools, src, dst, tables=None) -> None:
@@ -194,8 +202,8 @@ def kv_copy_pages(ctx: Context, k_pools, v_pools, src, dst, tables=None) -> None
     if s.size != d.size:
         raise ValueError("src and dst: expected one entry per page")
     tp = None if tables is None else _operand(ctx, "tables", tables, torch.int32)
-    call("clm_b200_kv_copy_pages", ctx.h, C.byref(pool), s.size, s.ctypes.data_as(_vp), d.ctypes.data_as(_vp), tp,
-         0 if tables is None else tables.numel(), _stream_on(ctx.device))
+    check(lib.clm_b200_kv_copy_pages(ctx.h, C.byref(pool), s.size, s.ctypes.data, d.ctypes.data, tp,
+                                     0 if tables is None else tables.numel(), _stream_on(ctx.device)))
 
 
 class Pages:

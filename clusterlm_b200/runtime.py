@@ -13,7 +13,7 @@ import ctypes as C
 
 import torch
 
-from ._native import QUANTS, call, lib
+from ._native import QUANTS, call, check, lib
 
 _vp = C.c_void_p
 
@@ -42,23 +42,26 @@ def _stream() -> _vp:
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _stream_on(device: int) -> _vp:
+def _stream_on(device: int) -> int:
     """torch's current stream of `device` (which need not be the current device)."""
-    h = torch.cuda.current_stream(device).cuda_stream
-    return _vp(h if h else _LEGACY_STREAM)
+    return torch._C._cuda_getCurrentRawStream(device) or _LEGACY_STREAM
 
 
-def _operand(ctx: "Context", name: str, t: torch.Tensor, dtype=None, shape=None, contiguous: bool = True) -> _vp:
+def _operand(ctx: "Context", name: str, t: torch.Tensor, dtype=None, shape=None, contiguous: bool = True) -> int:
     """The address of an operator's tensor, checked: on the context's device, of this type and shape."""
+    try:
+        if (t.get_device() == ctx.device and (dtype is None or t.dtype is dtype) and (shape is None or t.shape == shape)
+                and (not contiguous or t.is_contiguous())):
+            return t.data_ptr()
+    except (AttributeError, RuntimeError):
+        pass
     if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != ctx.device:
         raise ValueError(f"{name}: expected a tensor on cuda:{ctx.device}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor")
-    return _vp(t.data_ptr())
+    raise ValueError(f"{name}: expected a contiguous tensor")
 
 
 def device_count() -> int:
@@ -185,14 +188,17 @@ def sample_logits(ctx: Context, logits: torch.Tensor, uniforms: torch.Tensor, te
     ones), with one float64 uniform per row.  temperature (<= 0: argmax), top_k (0: all), top_p (1: all) and min_p (0:
     all) are numbers, or tensors (rows,) of float32 (top_k: int32).  Returns int32 tokens (rows,), -1 for a row without
     a finite logit; with_probs: also the tokens' probabilities among the allowed entries, float32 (rows,)."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in DTYPES:
+    dtype = DTYPES.get(getattr(logits, "dtype", None))
+    if dtype is None or logits.dim() != 2:
         raise ValueError("logits: expected a (rows, vocab) tensor of float32, float16 or bfloat16")
     rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    ld, step = logits.stride()
+    if vocab > 1 and step != 1:
         raise ValueError("logits: the last dimension must be contiguous")
-    if rows > 1 and logits.stride(0) < vocab:
+    if rows <= 1:
+        ld = vocab
+    elif ld < vocab:
         raise ValueError("logits: rows overlap")
-    ld = logits.stride(0) if rows > 1 else vocab
     lp = _operand(ctx, "logits", logits, contiguous=False)
     up = _operand(ctx, "uniforms", uniforms, torch.float64, (rows,))
     keep = []
@@ -202,15 +208,17 @@ def sample_logits(ctx: Context, logits: torch.Tensor, uniforms: torch.Tensor, te
             if value == default:
                 return None
             value = torch.full((rows,), value, dtype=dtype, device=logits.device)
-        keep.append(value)
+            keep.append(value)
         return _operand(ctx, name, value, dtype, (rows,))
 
-    settings = (setting("temperature", temperature, 1.0, torch.float32), setting("top_k", top_k, 0, torch.int32),
-                setting("top_p", top_p, 1.0, torch.float32), setting("min_p", min_p, 0.0, torch.float32))
+    temperature = setting("temperature", temperature, 1.0, torch.float32)
+    top_k = setting("top_k", top_k, 0, torch.int32)
+    top_p = setting("top_p", top_p, 1.0, torch.float32)
+    min_p = setting("min_p", min_p, 0.0, torch.float32)
     out = torch.empty(rows, dtype=torch.int32, device=logits.device)
     probs = torch.empty(rows, dtype=torch.float32, device=logits.device) if with_probs else None
-    call("clm_b200_sample_logits", ctx.h, lp, DTYPES[logits.dtype], rows, vocab, ld, *settings, up,
-         _vp(out.data_ptr()), _vp(probs.data_ptr()) if with_probs else None, _stream_on(ctx.device))
+    check(lib.clm_b200_sample_logits(ctx.h, lp, dtype, rows, vocab, ld, temperature, top_k, top_p, min_p, up,
+                                     out.data_ptr(), probs.data_ptr() if with_probs else None, _stream_on(ctx.device)))
     return (out, probs) if with_probs else out
 
 

@@ -64,13 +64,14 @@ struct SampleArgs {
   int vec;  // rows and slices start 16-byte aligned
 };
 
-// round(2^44 * 2^y) for -45.6 < y <= 0: 2^y = 2^n 2^(j / 64) 2^f with |f| <= 1/128, a table of the 2^(j / 64) and a
+// round(2^44 * 2^y) for -48 < y <= 0: 2^y = 2^n 2^(j / 64) 2^f with |f| <= 1/128, a table of the 2^(j / 64) and a
 // degree-3 polynomial for 2^f (least maximum relative error by weighted least squares: 4.5e-12).  Eight double
 // operations; a polynomial alone takes thirteen and measured 12% slower in the passes that evaluate every entry.
-__device__ __forceinline__ u64 mass_of(double y, const double* table) {
+// n64: 64 y rounded to an integer.
+__device__ __forceinline__ u64 mass_of(double y, const double* table, int& n64) {
   constexpr double kShift = 0x1.8p52, kShift64 = 0x1.8p46;
   const double k = y + kShift64;
-  const int n = (int)(unsigned)__double_as_longlong(k);
+  const int n = n64 = (int)(unsigned)__double_as_longlong(k);
   const double f = y - (k - kShift64);
   double p = 0x1.c6b0616cd9777p-5;
   p = fma(p, f, 0x1.ebfc2ec2e07ffp-3);
@@ -108,7 +109,7 @@ struct Shared {
   uint32_t sub_cnt[kSub];
   uint32_t cand_n, cut_n;
   double table[64];     // 2^(j / 64)
-  float few[kWrp][160];  // entries whose masses a warp has yet to sum
+  float few[kWrp][192];  // entries whose masses a warp has yet to sum
   int lo, hi;
   uint32_t cnt_before;
 };
@@ -147,9 +148,15 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   auto push = [&](auto* slot, auto value) {
     if (tid < kCl) *cluster.map_shared_rank(slot + rank, tid) = value;
   };
+  for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
+  if (tid < 64) s.table[tid] = exp2(tid / 64.0);
   cluster.barrier_arrive();  // waited for before the first write into another CTA's shared memory
   griddep_wait();
   griddep_launch();
+
+  const float T = a.temp ? a.temp[row] : 1.0f;
+  const int32_t k_in = a.top_k ? a.top_k[row] : 0;
+  const float p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f;
 
   // ---- 1. load and maximum (NaN counts as -inf; -0 as 0)
   const S* src = static_cast<const S*>(a.logits) + (long long)row * a.ld + v0;
@@ -178,9 +185,6 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     for (uint32_t i = tid; i < cnt; i += kThr) key[i] = clean(to_f32(src[i]));
   }
   for (uint32_t i = cnt + tid; i < a.slice; i += kThr) key[i] = -INFINITY;
-  for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
-  if (tid < 64) s.table[tid] = exp2(tid / 64.0);
-  const float T = a.temp ? a.temp[row] : 1.0f;
   const bool greedy = !(T > 0.0f);
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if (lane == 0) s.redf[0][warp] = mx;
@@ -198,7 +202,23 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
   cluster.barrier_wait();  // every CTA of the row runs
   push(s.top, (u64)ord_of(mx) << 32 | (u64)(0xffffffffu - first));
-  cluster.sync();
+  cluster.barrier_arrive();
+  // (the row's settings, while the maxima arrive)
+  const double c = 1.4426950408889634 / (double)T;  // y = c d: e = 2^y
+  const float cf = (float)c;
+  const bool need_k = k_in > 0 && (uint32_t)k_in < a.V, need_p = p_in < 1.0f;
+  const uint32_t k = need_k ? (uint32_t)k_in : 0xffffffffu;
+  // entries below dcut have no mass (y < -45: it rounds to zero); entries below dlow are not allowed: dcut, or the first float whose y is log2(min_p) or more
+  const float dcut = fmaxf(-FLT_MAX, (float)(-45.5 / c));
+  float dlow = dcut;
+  if (m_in > 0.0f && !greedy) {
+    const double ymin = log2((double)fminf(m_in, 1.0f));
+    float d = fminf(0.0f, fmaxf(-FLT_MAX, (float)(ymin / c)));
+    while (d < 0.0f && (double)d * c < ymin) d = nextafterf(d, 0.0f);
+    while (d > -FLT_MAX && (double)nextafterf(d, -INFINITY) * c >= ymin) d = nextafterf(d, -INFINITY);
+    dlow = fmaxf(dcut, d);
+  }
+  cluster.barrier_wait();
   u64 best = 0;
 #pragma unroll
   for (int r = 0; r < kCl; ++r) best = max(best, s.top[r]);
@@ -212,27 +232,18 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
 
   // ---- 2. what is allowed
-  const double c = 1.4426950408889634 / (double)T;  // y = c d: e = 2^y
-  const float cf = (float)c;
-  const int32_t k_in = a.top_k ? a.top_k[row] : 0;
-  const float p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f;
-  const bool need_k = k_in > 0 && (uint32_t)k_in < a.V, need_p = p_in < 1.0f;
-  const uint32_t k = need_k ? (uint32_t)k_in : 0xffffffffu;
-  // entries below dcut have no mass (y < -45: it rounds to zero); entries below dlow are not allowed: dcut, or the
-  // first float whose y is log2(min_p) or more
-  const float dcut = fmaxf(-FLT_MAX, (float)(-45.5 / c));
-  float dlow = dcut;
-  if (m_in > 0.0f) {
-    const double ymin = log2((double)fminf(m_in, 1.0f));
-    float d = fminf(0.0f, fmaxf(-FLT_MAX, (float)(ymin / c)));
-    while (d < 0.0f && (double)d * c < ymin) d = nextafterf(d, 0.0f);
-    while (d > -FLT_MAX && (double)nextafterf(d, -INFINITY) * c >= ymin) d = nextafterf(d, -INFINITY);
-    dlow = fmaxf(dcut, d);
+  float top = M;
+  if (M == INFINITY) {  // the infinite entries share the whole mass
+    __syncthreads();
+    for (uint32_t i = tid; i < a.slice; i += kThr) key[i] = key[i] == M ? 0.0f : -INFINITY;
+    top = 0.0f;
+    __syncthreads();
   }
-  auto d_of = [&](float x) { return x == M ? 0.0f : __fsub_rn(x, M); };
-  auto mass = [&](float d) {  // of any entry
-    const u64 w = mass_of((double)fmaxf(d, dcut) * c, s.table);
-    return d >= dcut ? w : 0ull;
+  auto d_of = [&](float x) { return __fsub_rn(x, top); };
+  auto mass_n = [&](float d, int& n) { return mass_of((double)fmaxf(d, dcut) * c, s.table, n); };  // of d >= dcut
+  auto mass = [&](float d) {
+    int n;
+    return mass_n(d, n);
   };
   auto u_of = [&](float d) { return __float_as_uint(fabsf(d)); };  // ascends as the order does
   const uint32_t seg = (a.slice / 4 + kWrp - 1) / kWrp * 4;
@@ -264,16 +275,20 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     auto look = [&](auto level0) {  // (two copies of the code: level 0 reads every entry)
       constexpr bool kFirst = decltype(level0)::value;
       const float inv = (float)kBins / ((float)(uh - ul) + 1.0f);
-      auto bin_of = [&](float d) {  // ascends as the order does (cf may be infinite: 0 has bin 0)
+      auto bin_of = [&](float d) {  // ascends as the order does
         if (!kFirst) return min(kBins - 1, (int)((float)(u_of(d) - ul) * inv));
-        return d == 0.0f ? 0 : min(kBins - 1, (int)fminf(-d * cf * (float)kBinsOct, (float)kBins));
+        int n;
+        mass_n(d, n);
+        return min(kBins - 1, -n);
       };
       auto inside = [&](float d) { return d >= dlow && (kFirst || (u_of(d) >= ul && u_of(d) <= uh)); };
       u64 sum = 0;
       if (kFirst && need_p) {
         each([&](uint32_t, float d) {
-          sum += mass(d);
-          if (d >= dlow) atomicAdd(&hist[bin_of(d)], 1u);
+          int n;
+          const u64 w = mass_n(d, n);
+          if (d >= dcut) sum += w;
+          if (d >= dlow) atomicAdd(&hist[min(kBins - 1, -n)], 1u);
         });
       } else {
         each([&](uint32_t, float d) {
@@ -312,7 +327,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       // the edges and of these f32 sums, which only bound where the cut can be
       constexpr int kPer = (kBins + kThr - 1) / kThr;
       auto edge = [&](int bin) {  // e at a bin's upper edge, in units of 2^-44
-        if (kFirst) return exp2f((float)kFrac - (float)bin * (1.0f / kBinsOct));
+        if (kFirst) return exp2f((float)kFrac - ((float)bin - 0.5f) * (1.0f / kBinsOct));
         const float step = ((float)(uh - ul) + 1.0f) * (1.0f / kBins);
         return exp2f((float)kFrac - __uint_as_float(min(uh, ul + (uint32_t)((float)bin * step) + (bin > 0))) * cf);
       };
@@ -320,15 +335,15 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       float up[kPer], down[kPer];
       uint32_t nsum = 0;
       float usum = 0.0f, dsum = 0.0f;
-      float top = edge(tid * kPer);
+      float begin = edge(tid * kPer);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int bin = tid * kPer + j;
         const float next = edge(bin + 1);
         n[j] = bin < kBins ? tot[bin] : 0u;
-        up[j] = n[j] ? (float)n[j] * top * 1.0001f : 0.0f;
+        up[j] = n[j] ? (float)n[j] * begin * 1.0001f : 0.0f;
         down[j] = n[j] ? (float)n[j] * next * 0.9999f : 0.0f;
-        top = next;
+        begin = next;
         nsum += n[j];
         usum += up[j];
         dsum += down[j];
@@ -382,13 +397,32 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       __syncthreads();
       const int lo = s.lo, hi = s.hi;
       if (lo_mine == lo && lo < kBins) s.cnt_before = before_lo;  // (one thread)
+      // Bins ascend with u: the first u of a bin or a later one, by a search of 32 parts a step (the same in every warp),
+      // so that the entries need no bins again.
+      auto first_of = [&](int bin) -> uint32_t {
+        uint32_t at = ul, left = uh - ul + 1;  // the first is in [at, at + left]
+        while (left > 0) {
+          const uint32_t step = (left + 31) / 32, probe = at + min(left, (lane + 1) * step) - 1;
+          const uint32_t under = __popc(__ballot_sync(0xffffffffu, bin_of(-__uint_as_float(probe)) < bin));
+          const uint32_t skip = min(left, under * step);
+          at += skip;
+          left = under == 32 ? 0 : min(left - skip, step - 1);
+        }
+        return at;
+      };
+      const uint32_t ulo = first_of(lo), uhi = lo == kBins ? ulo : first_of(hi + 1);
+      const float dtop = -__uint_as_float(ul);
+      // before the cut's bins: dtop >= d > dlo (and d >= dlow); in them: dlo >= d >= dhi
+      const float dlo = -__uint_as_float(ulo), dhi = uhi > ul ? fmaxf(dlow, -__uint_as_float(uhi - 1)) : INFINITY;
       // the masses of entries before the cut's bins (gathered, so that every lane has one to evaluate), and the candidates
       uint32_t waiting = 0, least = 0xffffffffu, largest = 0;
       float* few = s.few[warp];
       auto add_up = [&](uint32_t count) {
         waiting -= count;
         __syncwarp();
-        if (lane < count) seg_mass += mass(few[waiting + lane]);
+        const bool one = lane < count, two = lane + 32 < count;
+        const u64 w0 = mass(one ? few[waiting + lane] : 0.0f), w1 = mass(two ? few[waiting + lane + 32] : 0.0f);
+        seg_mass += (one ? w0 : 0ull) + (two ? w1 : 0ull);
         __syncwarp();
       };
       for (uint32_t i0 = s0; i0 < s1; i0 += 128) {
@@ -396,36 +430,50 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         const float4 x = i < s1 ? *reinterpret_cast<const float4*>(key + i)
                                 : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         const float d[4] = {d_of(x.x), d_of(x.y), d_of(x.z), d_of(x.w)};
-        int bin[4];
-        uint32_t early[4];
-        bool some = false;
+        bool in_cut[4], some = false, any = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          bin[j] = inside(d[j]) ? bin_of(d[j]) : kBins + 1;
-          early[j] = __ballot_sync(0xffffffffu, bin[j] < lo);
-          some |= bin[j] >= lo && bin[j] <= hi;
+          const bool in = d[j] >= dhi && d[j] <= dtop;
+          any |= in;
+          in_cut[j] = in && d[j] <= dlo;
+          some |= in_cut[j];
         }
+        if (!__any_sync(0xffffffffu, any)) continue;
+        uint32_t early[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) early[j] = __ballot_sync(0xffffffffu, d[j] > dlo && d[j] >= dhi && d[j] <= dtop);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (bin[j] < lo) few[waiting + __popc(early[j] & ((1u << lane) - 1u))] = d[j];
+          if (early[j] >> lane & 1u) few[waiting + __popc(early[j] & ((1u << lane) - 1u))] = d[j];
           waiting += __popc(early[j]);
         }
-        while (waiting >= 32) add_up(32);
-        if (some) {
+        while (waiting >= 64) add_up(64);
+        if (__any_sync(0xffffffffu, some)) {
+          uint32_t mates[4], at = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (bin[j] >= lo && bin[j] <= hi) {
-              const uint32_t u = u_of(d[j]), at = atomicAdd(&s.cand_n, 1u);
+          for (int j = 0; j < 4; ++j) {
+            mates[j] = __ballot_sync(0xffffffffu, in_cut[j]);
+            at += __popc(mates[j]);
+          }
+          if (lane == 0) at = atomicAdd(&s.cand_n, at);
+          at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (in_cut[j]) {
+              const uint32_t u = u_of(d[j]), to = at + __popc(mates[j] & ((1u << lane) - 1u));
               least = min(least, u);
               largest = max(largest, u);
-              // (in the place of the histograms, which every CTA has read)
-              if (at < kMine) mine[at] = Cand{u, v0 + i + j, mass(d[j])};
+              // (in the place of the histograms, which every CTA has read; its mass follows)
+              if (to < kMine) mine[to] = Cand{u, v0 + i + j, 0ull};
             }
+            at += __popc(mates[j]);
+          }
         }
       }
       if (waiting) add_up(waiting);
       const u64 level_mass = warp_sum(seg_mass);  // with the levels before
       const u64 x = cta_sum(level_mass, s.seg, warp, lane);
+      for (uint32_t i = tid; i < min(s.cand_n, (uint32_t)kMine); i += kThr) mine[i].w = mass(-__uint_as_float(mine[i].u));
       push(s.above, x);
       push(s.ncand, s.cand_n);
       least = __reduce_min_sync(0xffffffffu, least);

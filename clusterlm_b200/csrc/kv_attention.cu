@@ -11,9 +11,9 @@
 // all sequences; so a call is one or two launches and the combining one.
 //
 // Work of a kernel is one line of units: per entry, per item (kv head, and row tile in the tile kernel), its pages (tile
-// kernel: counted double for more than 128 rows).  The line is cut into equal shares, one per CTA (stream
-// kernel: per team of warps), so ragged lengths balance without any host knowledge of them.  A share's part of an item
-// is a segment, numbered by (item + share): both only grow along the line.
+// kernel: counted double for more than 128 rows; stream kernel: half pages), and some for the item's own start and end.  The line is cut into
+// equal shares, one per CTA (stream kernel: per warp), so ragged lengths balance without any host knowledge of
+// them.  A share's part of an item is a segment, numbered by (item + share): both only grow along the line.
 #include <algorithm>
 #include <cfloat>
 
@@ -26,14 +26,16 @@ namespace clm {
 namespace {
 
 constexpr int kMaxEntries = kKvMaxGroups + kKvMaxSeqs;
-constexpr int kStreamRows = 64;  // entries of up to this many rows per kv head: the stream kernel
+constexpr int kStreamRows = 16;  // entries of up to this many rows per kv head: the stream kernel
 constexpr int kStreamWarps = 8;  // warps of a stream CTA
 constexpr int kRowTile = 256;    // rows of an item of the tile kernel: two tiles of 128
-constexpr int kSegPad = 4;     // floats after a partial row's hd outputs: m, l, padding to 16 bytes
+constexpr int kSegPad = 8;     // floats after a partial row's hd outputs: m, l, padding to 32 bytes
+constexpr int kStreamSwitch = 2;  // stream kernel: a segment's start and end take as long as this many half pages
+constexpr int kSwitch = 12;    // tile kernel: a segment's start and end take as long as this many units
 
 struct Plan {
   uint32_t cum[kMaxEntries + 1];  // work units before entry e (below 2^31, checked by the host)
-  int pages[kMaxEntries];         // pages of an item of entry e
+  int pages[kMaxEntries];         // pages of an item of entry e (stream kernel: half pages with a position that is seen)
   uint32_t shares, q, r;          // how the line is cut (below)
   __device__ __forceinline__ struct Shares cut() const;
 };
@@ -64,6 +66,7 @@ struct Entry {
   int rows;    // rows per kv head
   int tiles;   // row tiles per kv head
   int weight;  // work units of a page
+  int over;    // and of an item besides its pages
 };
 __device__ __forceinline__ Entry entry_of(const Args& a, int e) {
   Entry r;
@@ -79,7 +82,16 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int e) {
   const bool tile = a.kind[r.kind].tile;
   r.tiles = tile ? (r.rows + kRowTile - 1) / kRowTile : 1;
   r.weight = tile && r.rows > 128 ? 2 : 1;
+  r.over = tile ? kSwitch : kStreamSwitch;
   return r;
+}
+
+// Pages of an item before its unit `u`.
+__device__ __forceinline__ uint32_t pages_before(const Entry& e, uint32_t u) {
+  return u <= (uint32_t)e.over ? 0u : (u - e.over + e.weight - 1) / e.weight;
+}
+__device__ __forceinline__ uint32_t units_of(const Entry& e, uint32_t pages) {
+  return pages ? pages * e.weight + e.over : 0u;
 }
 
 // The group of sequence b, or -1.
@@ -124,22 +136,24 @@ struct Shares {
 __device__ __forceinline__ Shares Plan::cut() const { return Shares{shares, q, r}; }
 
 // Fills the plan of the tile (or stream) kernel from the device-side positions: pages per item, then the running work of
-// its entries (the other kernel's have none).
-__device__ void make_plan(const Args& a, Plan* plan, int tile, uint32_t shares) {
+// its entries (the other kernel's have none).  first: the entries' first pages.
+__device__ void make_plan(const Args& a, Plan* plan, int* first, int tile, uint32_t shares) {
   const int E = a.groups.n + a.seqs.n;
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    int pages = 0;
     const Entry en = entry_of(a, e);
+    const int per = tile ? 1 : 2, unit = kPageTokens / per;
+    int pages = 0, at = 0;
     if (e < a.groups.n) {
-      pages = min((int)a.groups.pages[e], a.seqs.max_pages);
+      pages = per * min((int)a.groups.pages[e], a.seqs.max_pages);
     } else {
       const long long base = a.seqs.base(en.s0);
+      at = shared_pages(a, en.s0);
       if (base >= 0)
-        pages = max(0, (int)min((base + a.positions + kPageTokens - 1) / kPageTokens, (long long)a.seqs.max_pages) -
-                           shared_pages(a, en.s0));
+        pages = max(0, (int)min((base + a.positions + unit - 1) / unit, (long long)per * a.seqs.max_pages) - per * at);
     }
     plan->pages[e] = pages;
-    plan->cum[e + 1] = a.kind[en.kind].tile == tile ? (uint32_t)pages * (uint32_t)(en.weight * en.tiles * a.nkv) : 0u;
+    first[e] = at;
+    plan->cum[e + 1] = a.kind[en.kind].tile == tile ? units_of(en, pages) * (uint32_t)(en.tiles * a.nkv) : 0u;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -156,12 +170,27 @@ __device__ void make_plan(const Args& a, Plan* plan, int tile, uint32_t shares) 
     }
     if (threadIdx.x == 0) {
       plan->cum[0] = 0;
-      plan->shares = min(shares, run);  // every share holds a unit
+      // Every share holds a unit.  Of the stream kernel three: a short segment spends more on its start and its partial
+      // (GPU time of a call with 4 sequences of about 1,000 positions, 8 kv heads, head_dim 128, with at least 2, 3, 4 or 6
+      // units a share: 14.5, 12.9, 13.6, 16.4 us).
+      plan->shares = min(shares, tile ? run : (run + 2) / 3);
       plan->q = run ? run / plan->shares : 0u;
       plan->r = run ? run % plan->shares : 0u;
     }
   }
   __syncthreads();
+}
+
+// The entry that holds unit w (the last one that begins at or before it), found by the warp's lanes together.
+__device__ __forceinline__ int entry_at(const Plan& plan, int entries, uint32_t w) {
+  const int lane = threadIdx.x % 32;
+  int e = 0;
+  for (int at = 0; at < entries; at += 32) {
+    const uint32_t n = __popc(__ballot_sync(0xffffffffu, at + lane < entries && plan.cum[at + lane] <= w));
+    e += n;
+    if (n < 32) break;
+  }
+  return e - 1;
 }
 
 // The combining kernel's copy of the plan.
@@ -362,7 +391,9 @@ struct Tile {
   static constexpr uint32_t kHalf = kPageTokens * HD * 2;  // bytes of K, or V, of a page and kv head
   static constexpr uint32_t kQ = 128 * HD * 2;             // bytes of a query tile
   static constexpr int kRow = HD + kSegPad;
-  static constexpr size_t kSmem = 2 * (size_t)kQ + (size_t)kSlots * 2 * kHalf;
+  // two query tiles; slots [K][V]; a staging tile of 32 x 16 floats per warp
+  static constexpr uint32_t kStage = 32 * 64;
+  static constexpr size_t kSmem = 2 * (size_t)kQ + (size_t)kSlots * 2 * kHalf + 8 * kStage;
 };
 
 constexpr int kSoftWarps = 4;  // softmax warps of a stream of the tile kernel
@@ -404,27 +435,18 @@ struct Segment {
 struct Walk {
   const Args& a;
   const Plan& plan;
+  const int* first;
   uint32_t w, end;
   int e;
-  __device__ __forceinline__ Walk(const Args& args, const Plan& p, uint32_t begin, uint32_t finish)
-      : a(args), plan(p), w(begin), end(finish), e(0) {
-    int lo = 0, hi = args.groups.n + args.seqs.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (plan.cum[mid] <= begin)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    e = lo;
-  }
+  __device__ __forceinline__ Walk(const Args& args, const Plan& p, const int* firsts, uint32_t begin, uint32_t finish)
+      : a(args), plan(p), first(firsts), w(begin), end(finish), e(entry_at(p, args.groups.n + args.seqs.n, begin)) {}
   __device__ __forceinline__ bool next(Segment& s) {
     while (w < end) {
       while (plan.cum[e + 1] <= w) ++e;
       const Entry en = entry_of(a, e);
-      const uint32_t pages = plan.pages[e], wt = en.weight, units = pages * wt;
+      const uint32_t units = units_of(en, plan.pages[e]);
       const uint32_t tile = (w - plan.cum[e]) / units, u0 = plan.cum[e] + tile * units;
-      const uint32_t b0 = (w - u0 + wt - 1) / wt, b1 = min(pages, (end - u0 + wt - 1) / wt);
+      const uint32_t b0 = pages_before(en, w - u0), b1 = pages_before(en, min(units, end - u0));
       w = min(u0 + units, end);
       if (b0 >= b1) continue;
       s.item = items_before(a, e) + (int)tile;
@@ -434,7 +456,7 @@ struct Walk {
       s.x0 = (int)tile % en.tiles * kRowTile;
       s.rows = min(en.rows - s.x0, kRowTile);
       s.pair = s.rows > 128;
-      s.page0 = (s.group ? 0 : shared_pages(a, en.s0)) + (int)b0;
+      s.page0 = first[e] + (int)b0;
       s.pages = (int)(b1 - b0);
       s.streams = s.pair || s.pages > 1 ? 2 : 1;
       return true;
@@ -444,7 +466,7 @@ struct Walk {
 };
 
 // ---------------------------------------------------------------------------------------------------
-// tile kernel: entries of more than 64 rows per kv head
+// tile kernel: entries of more than 16 rows per kv head
 //
 // Two streams of four softmax warps each own 128 rows, one thread a row: no reductions across lanes.  With more than 128
 // rows the streams take a row tile each of every page; with fewer they take alternate pages of the same rows and give
@@ -462,6 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
   constexpr int SL = TL::kSlots;
   extern __shared__ __align__(1024) uint8_t smem[];  // [2 query tiles][slots of [K block][V block]]
   __shared__ Plan plan;
+  __shared__ int s_first[kMaxEntries];
   __shared__ __align__(8) uint64_t copied_k[SL], copied_v[SL], free_k[SL], free_v[SL];
   __shared__ __align__(8) uint64_t full_k[2][SL], full_v[2][SL];  // by a stream's own count of pages
   __shared__ __align__(8) uint64_t q_ready[2], drained[2];
@@ -502,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
   }
   griddep_wait();
   griddep_launch();
-  make_plan(a, &plan, 1, gridDim.x);
+  make_plan(a, &plan, s_first, 1, gridDim.x);
   if (a.parent != nullptr) make_ancestors(a, s_anc);
   publish(a, plan, 1);
   const Shares shares = plan.cut();
@@ -533,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
     return false;
   };
 
-  Walk walk(a, plan, shares.begin(blockIdx.x), shares.begin(blockIdx.x + 1));
+  Walk walk(a, plan, s_first, shares.begin(blockIdx.x), shares.begin(blockIdx.x + 1));
   Segment g;
   if (warp == kRelay) {
     // ---------------- relay: copies that have landed become visible to the tensor cores (the copies are generic writes;
@@ -690,31 +713,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
     const uint32_t lanes = tmem + ((uint32_t)(warp % 4) * 32 << 16);
     const uint32_t ts = lanes + 256 * s, to = ts + 128;
     uint8_t* qs = smem + s * TL::kQ;
-    uint32_t idx0 = 0, done = 0;  // pages before the segment, pages of the stream
+    uint8_t* stage = smem + 2 * TL::kQ + SL * 2 * TL::kHalf + warp * TL::kStage;
+    uint32_t before = 0, idx0 = 0, done = 0;  // pages so far; before the segment; of the stream
     bool ok = true;
-    for (; walk.next(g); idx0 += g.pages) {
-      if (s >= g.streams) continue;
-      const int nrows = g.stream_rows(s), x = g.x0 + (g.pair ? 128 * s : 0) + r;
-      const bool work = (warp % 4) * 32 < nrows;  // the warp has a row
-      bool valid = r < nrows;
-      int i = 0;  // window row
-      long long base = 0;
+    auto advance = [&]() {  // the stream's next segment
+      while (walk.next(g)) {
+        idx0 = before;
+        before += g.pages;
+        if (s < g.streams) return true;
+      }
+      return false;
+    };
+    // the segment's rows: the thread's window row and its base, the query row to shared memory
+    int nrows = 0, i = 0;
+    long long base = 0;
+    bool work = false, valid = false;  // the warp has a row; the thread has one
+    auto load = [&]() {
+      const int x = g.x0 + (g.pair ? 128 * s : 0) + r;
+      nrows = g.stream_rows(s);
+      work = (warp % 4) * 32 < nrows;
+      valid = r < nrows;
       if (work) {
         const int srow = valid ? x / a.group : 0, head = g.kvh * a.group + (valid ? x % a.group : 0);
         const int b = g.s0 + srow / a.positions;
         i = srow % a.positions;
         base = a.seqs.base(b);
-        valid = valid && base >= 0;
         const uint4* q = reinterpret_cast<const uint4*>(
             static_cast<const T*>(a.q) + ((long long)b * a.positions + i) * a.ld_q + (long long)head * HD);
+        uint4 v[HD / 8];  // (asked for before the base is known)
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) v[c] = __ldg(q + c);
+        valid = valid && base >= 0;
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c)
-          *reinterpret_cast<uint4*>(qs + (c / 8) * (128 * 128) + sw128(r, c % 8)) =
-              valid ? __ldg(q + c) : make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(qs + (c / 8) * (128 * 128) + sw128(r, c % 8)) = valid ? v[c] : make_uint4(0u, 0u, 0u, 0u);
         fence_smem_async();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[s]);
+    };
+    bool more = advance();
+    if (more) load();
+    while (more) {
       float m = -INFINITY, l = 0.0f;  // m: the reference of the weights so far (scaled scores)
       const int np = g.stream_pages(s);
       for (int t = 0; t < np; ++t, ++done) {
@@ -792,53 +832,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[s][done & 1u]);
       }
-      // the stream's partial rows, once its last products are complete
+      // The next segment's query rows (the scores that read this one's are complete), then this one's partial rows, once
+      // its last products are complete.
+      const Segment was = g;
+      const int was_i = i, left = nrows - (warp % 4) * 32;
+      const long long was_base = base;
+      const bool was_work = work, was_valid = valid;
+      if ((more = advance())) load();
       ok = ok && wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
-      if (work) {
+      if (was_work) {
         tc_after();
-        const int seg = g.item + (int)blockIdx.x;
-        const Args::Kind& kind = a.kind[g.group ? 0 : 1];
-        float* dst = kind.part + ((size_t)(2 * seg + s) * kind.rows + r) * TL::kRow;
-        const bool odd = s_odd && !g.group;
+        const int seg = was.item + (int)blockIdx.x;
+        const Args::Kind& kind = a.kind[was.group ? 0 : 1];
+        float* rows = kind.part + ((size_t)(2 * seg + s) * kind.rows + (warp % 4) * 32) * TL::kRow;
+        const bool odd = s_odd && !was.group;
 #pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          tc_ld32(to + 32 * c, o);
+        for (int c = 0; c < HD / 16; ++c) {
+          uint32_t o[16];
+          tc_ld16(to + 16 * c, o);
           tc_wait_ld();
-          if (odd && valid)  // values that are not finite, of window positions of these pages that the row sees
+          if (odd && was_valid)  // values that are not finite, of window positions of these pages that the row sees
             for (int j = 0; j < a.positions; ++j) {
-              const long long pos = base + j, at = pos / kPageTokens - g.page0;
-              if (!win.sees(i, j) || at < 0 || at >= g.pages) continue;
-              const int32_t page = a.seqs.table(g.s0)[pos / kPageTokens];
+              const long long pos = was_base + j, at = pos / kPageTokens - was.page0;
+              if (!win.sees(was_i, j) || at < 0 || at >= was.pages) continue;
+              const int32_t page = a.seqs.table(was.s0)[pos / kPageTokens];
               if (page < 0 || page >= a.seqs.pool_pages) continue;
               const int pp = (int)(pos % kPageTokens);
 #pragma unroll
-              for (int d = 0; d < 32; ++d) {
-                const int dim = 32 * c + d;
-                const float v = to_f32(static_cast<const T*>(a.v)[(((size_t)page * a.nkv + g.kvh) * HD + dim) * kPageTokens +
+              for (int d = 0; d < 16; ++d) {
+                const int dim = 16 * c + d;
+                const float v = to_f32(static_cast<const T*>(a.v)[(((size_t)page * a.nkv + was.kvh) * HD + dim) * kPageTokens +
                                                                   8 * kv_v_chunk(pp / 8, dim) + pp % 8]);
                 if (!(fabsf(v) <= FLT_MAX)) o[d] = __float_as_uint(NAN);
               }
             }
-          // through the warp's rows of the query tile (read for the last time), so that eight lanes write 128 bytes of a row
-          uint8_t* stage = qs + (warp % 4) * 32 * 128;
+          // through shared memory, so that four lanes write 64 bytes of a row
+          auto at = [&](int row, int j) { return reinterpret_cast<uint4*>(stage + row * 64 + ((j ^ (row / 2 % 4)) << 4)); };
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(stage + sw128(lane, j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          for (int j = 0; j < 4; ++j) *at(lane, j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           __syncwarp();
-          float* rows = dst - (size_t)lane * TL::kRow + 32 * c;
-          const int left = nrows - (warp % 4) * 32;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int rr = 4 * j + lane / 8;
-            if (rr < left)
-              *reinterpret_cast<uint4*>(rows + (size_t)rr * TL::kRow + 4 * (lane % 8)) =
-                  *reinterpret_cast<const uint4*>(stage + sw128(rr, lane % 8));
+          for (int j = 0; j < 4; ++j) {
+            const int row = 8 * j + lane / 4;
+            if (row < left)
+              *reinterpret_cast<uint4*>(rows + (size_t)row * TL::kRow + 16 * c + 4 * (lane % 4)) = *at(row, lane % 4);
           }
           __syncwarp();
         }
         // a copy that never arrived: the rows say so
-        if (r < nrows) *reinterpret_cast<float2*>(dst + HD) = make_float2(m, ok ? l : NAN);
+        if (lane < left) *reinterpret_cast<float2*>(rows + (size_t)lane * TL::kRow + HD) = make_float2(m, ok ? l : NAN);
         tc_before();
       }
     }
@@ -851,12 +893,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------------------------------------------
-// stream kernel: entries of up to 64 rows per kv head
+// stream kernel: entries of up to 16 rows per kv head
 //
-// A team of TM warps (1, 2 or 4: a row tile of 16 each) takes a share of the line; the teams of a CTA, and the warps of
-// a team, share nothing: a warp reads its operands from global memory in the fragments' order (every K and V chunk is
-// used by one lane of a row tile; a team's further warps find it in the L1 cache), keeps its state in registers and
-// writes its own partial.  Eight warps a CTA, each with 8 to 16 KB of loads in flight, cover the memory's latency.
+// A warp takes a share of the line and a row tile of 16; warps share nothing: a warp reads its operands from global
+// memory in the fragments' order (every K and V chunk is used by one lane), keeps its state in registers and writes its
+// own partial.  Eight warps a CTA, each with 8 to 16 KB of loads in flight, cover the memory's latency.
 //
 // Fragment mapping (mma m16n8k16, lane = 4 g + t): column n of S's n-tile jj is position 8 (n / 2) + 2 jj + n % 2 of the
 // half page, so a lane's scores are positions 8 t + 2 jj + {0, 1}; the weights of n-tiles 2 kk and 2 kk + 1 are then the A
@@ -877,20 +918,29 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// 16 bytes of the cache, in program order with the products
+__device__ __forceinline__ uint4 load16(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 template <typename T>
 constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x3C00u : 0x3F80u;
 
-template <typename T, int HD, int TM>
+template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const __grid_constant__ Args a, int second) {
   constexpr int KW = HD / 32;  // 16-byte words of a K row per lane
   constexpr int kRow = HD + kSegPad;
+  constexpr bool kAhead = HD == 64;
   __shared__ Plan plan;
+  __shared__ int s_first[kMaxEntries];
   __shared__ uint32_t s_anc[kKvMaxWindow * 8];
+  __shared__ uint4 s_query[kStreamWarps][2 * KW][32];
   // After the tile kernel this one starts early: what it reads was complete before the tile kernel let it start.  The
   // combining kernel waits for this one alone, so this one waits for the tile kernel before it ends.
   if (!second) griddep_wait();
   griddep_launch();
-  make_plan(a, &plan, 0, gridDim.x * (kStreamWarps / TM));
+  make_plan(a, &plan, s_first, 0, gridDim.x * kStreamWarps);
   if (a.parent != nullptr) {
     make_ancestors(a, s_anc);
     __syncthreads();
@@ -900,96 +950,120 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
   const int E = a.groups.n + a.seqs.n;
   const Shares shares = plan.cut();
   // consecutive shares go to different SMs: short lines use all of them
-  const uint32_t share = (warp / TM) * gridDim.x + blockIdx.x;
-  const int j = warp % TM;  // row tile
+  const uint32_t share = warp * gridDim.x + blockIdx.x;
   const Window win{a.parent ? s_anc : nullptr, a.positions};
   uint32_t w = 0, end = 0;
   int e = 0;
   if (share < shares.C) {
     w = shares.begin(share);
     end = shares.begin(share + 1);
-    int lo = 0, hi = E - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (plan.cum[mid] <= w)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    e = lo;
+    e = entry_at(plan, E, w);
   }
   while (w < end) {
     while (plan.cum[e + 1] <= w) ++e;
     const Entry en = entry_of(a, e);
-    const uint32_t L = plan.pages[e];
-    const uint32_t kvh = (w - plan.cum[e]) / L, off = w - plan.cum[e] - kvh * L;
-    const int np = (int)min(L - off, end - w);
-    w += np;
-    if (16 * j >= en.rows) continue;
-    const int first = (en.kind == 0 ? 0 : shared_pages(a, en.s0)) + (int)off;
+    const uint32_t units = units_of(en, plan.pages[e]);
+    const uint32_t kvh = (w - plan.cum[e]) / units, u0 = plan.cum[e] + kvh * units;
+    const uint32_t off = pages_before(en, w - u0), upto = pages_before(en, min(units, end - u0));
+    w = min(u0 + units, end);
+    if (off >= upto) continue;
+    const int halves = (int)(upto - off);
+    const int half0 = (int)off % 2, first = s_first[e] + (int)off / 2;
     const int32_t* table = a.seqs.table(en.s0) + first;
-    // rows r0 = 16 j + g and r0 + 8: window row and head
+    int32_t page = 0, coming = __ldg(table);  // this page, the next entry
+    // rows g and g + 8: window row and head
     int i0, i1;
     long long b0, b1;
     bool v0, v1;
-    uint4 qw0[KW], qw1[KW];
-    auto row = [&](int r, int& i, long long& base, bool& valid, uint4(&qw)[KW]) {
+    // (the warp's queries lie in shared memory: with them in registers the loop would spill)
+    auto s_q = [&](int which, int u) { return &s_query[warp][which * KW + u][lane]; };
+    auto row = [&](int which, int& i, long long& base, bool& valid) {
+      const int r = g + 8 * which;
       valid = r < en.rows;
       const int srow = valid ? r / a.group : 0, head = (int)kvh * a.group + (valid ? r % a.group : 0);
       const int b = en.s0 + srow / a.positions;
       i = srow % a.positions;
       base = a.seqs.base(b);
-      valid = valid && base >= 0;
       const uint4* p = reinterpret_cast<const uint4*>(
           static_cast<const T*>(a.q) + ((long long)b * a.positions + i) * a.ld_q + (long long)head * HD + (HD / 4) * t);
+      uint4 v[KW];  // (asked for before the base is known)
 #pragma unroll
-      for (int u = 0; u < KW; ++u) qw[u] = valid ? __ldg(p + u) : make_uint4(0u, 0u, 0u, 0u);
+      for (int u = 0; u < KW; ++u) v[u] = __ldg(p + u);
+      valid = valid && base >= 0;
+#pragma unroll
+      for (int u = 0; u < KW; ++u) *s_q(which, u) = valid ? v[u] : make_uint4(0u, 0u, 0u, 0u);
     };
-    row(16 * j + g, i0, b0, v0, qw0);
-    row(16 * j + g + 8, i1, b1, v1, qw1);
-    auto word = [](const uint4(&v)[KW], int k) {
-      const uint4& u = v[k / 4];
-      return (k % 4 == 0) ? u.x : (k % 4 == 1) ? u.y : (k % 4 == 2) ? u.z : u.w;
-    };
+    row(0, i0, b0, v0);
+    row(1, i1, b1, v1);
     float O[HD / 8][4];
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.0f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-    int32_t page = __ldg(table);
-    for (int pj = 0; pj < np; ++pj) {
-      const int32_t now = page;
-      if (pj + 1 < np) page = __ldg(table + pj + 1);
-      if (now < 0 || now >= a.seqs.pool_pages) continue;
-      const size_t at = ((size_t)now * a.nkv + kvh) * (size_t)(kPageTokens * HD);
-      const T* ks = static_cast<const T*>(a.k) + at;
-      const T* vs = static_cast<const T*>(a.v) + at;
-      const long long p_begin = (long long)(first + pj) * kPageTokens;
-      // every position visible to every valid row of the tile
-      const bool plain = __all_sync(0xffffffffu, (!v0 || p_begin + kPageTokens <= b0) && (!v1 || p_begin + kPageTokens <= b1));
+    // K of the next half page (of table entry `pj`; of existing pages only) is asked for once the products with this one's
+    // are made, V after the weights' products, so that loads are in flight while the warp computes.
+    int pj = -1;
+    const T *ks = nullptr, *vs = nullptr;
+    auto advance = [&]() {  // to the next existing page, if there is one
+      while (2 * ++pj < half0 + halves) {
+        page = coming;
+        if (2 * pj + 2 < half0 + halves) coming = __ldg(table + pj + 1);
+        if (page >= 0 && page < a.seqs.pool_pages) {
+          const size_t at = ((size_t)page * a.nkv + kvh) * (size_t)(kPageTokens * HD);
+          ks = static_cast<const T*>(a.k) + at;
+          vs = static_cast<const T*>(a.v) + at;
+          return true;
+        }
+      }
+      return false;
+    };
+    uint4 kw[4][KW], va[HD / 8];
+    auto load_k = [&](int half) {
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        const int pos = 32 * half + 8 * (g / 2) + 2 * jj + (g % 2);
+        const uint4* kr = reinterpret_cast<const uint4*>(ks + (size_t)pos * HD);
+#pragma unroll
+        for (int u = 0; u < KW; ++u) kw[jj][u] = load16(kr + kv_k_chunk(KW * t + u, pos));
+      }
+    };
+    auto load_v = [&](int half) {
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) {
+        const int vrow = 8 * n + g;
+        va[n] = load16(reinterpret_cast<const uint4*>(vs + (size_t)vrow * kPageTokens) + kv_v_chunk(4 * half + t, vrow));
+      }
+    };
+    bool more = advance();
+    int half = pj == 0 ? half0 : 0;
+    if (kAhead && more) {
+      load_k(half);
+      load_v(half);
+    }
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        uint4 kw[4][KW], va[HD / 8];
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          const int pos = 32 * half + 8 * (g / 2) + 2 * jj + (g % 2);
-          const uint4* kr = reinterpret_cast<const uint4*>(ks + (size_t)pos * HD);
-#pragma unroll
-          for (int u = 0; u < KW; ++u) kw[jj][u] = __ldg(kr + kv_k_chunk(KW * t + u, pos));
-        }
-#pragma unroll
-        for (int n = 0; n < HD / 8; ++n) {
-          const int vrow = 8 * n + g;
-          va[n] = __ldg(reinterpret_cast<const uint4*>(vs + (size_t)vrow * kPageTokens) + kv_v_chunk(4 * half + t, vrow));
-        }
+    while (more) {
+      if (!kAhead) {
+        load_k(half);
+        load_v(half);
+      }
+      const long long p_begin = (long long)(first + pj) * kPageTokens;
+      {
         float S[4][4];
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          S[jj][0] = S[jj][1] = S[jj][2] = S[jj][3] = 0.0f;
+        for (int jj = 0; jj < 4; ++jj) S[jj][0] = S[jj][1] = S[jj][2] = S[jj][3] = 0.0f;
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            mma16<T>(S[jj], word(qw0, 2 * kk), word(qw1, 2 * kk), word(qw0, 2 * kk + 1), word(qw1, 2 * kk + 1),
-                     word(kw[jj], 2 * kk), word(kw[jj], 2 * kk + 1));
+        for (int u = 0; u < KW; ++u) {
+          const uint4 q0 = *s_q(0, u), q1 = *s_q(1, u);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            mma16<T>(S[jj], q0.x, q1.x, q0.y, q1.y, kw[jj][u].x, kw[jj][u].y);
+            mma16<T>(S[jj], q0.z, q1.z, q0.w, q1.w, kw[jj][u].z, kw[jj][u].w);
+          }
         }
+        const bool second_half = half == 0 && 2 * pj + 1 < half0 + halves;
+        more = second_half || advance();
+        if (kAhead && more) load_k(second_half);
+        // every position visible to every valid row of the tile
+        const bool plain = __all_sync(0xffffffffu, (!v0 || p_begin + kPageTokens <= b0) && (!v1 || p_begin + kPageTokens <= b1));
         // bit x of a row's word: it sees position 8 t + x of the half page
         uint32_t see0 = v0 ? 0xffu : 0u, see1 = v1 ? 0xffu : 0u;
         if (!plain) {
@@ -1072,6 +1146,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
           mma16<T>(O[n], pa[0][0], pa[0][1], pa[1][0], pa[1][1], va[n].x, va[n].y);
           mma16<T>(O[n], pa[2][0], pa[2][1], pa[3][0], pa[3][1], va[n].z, va[n].w);
         }
+        if (kAhead && more) load_v(second_half);
+        half = second_half;
       }
     }
     // the segment's partial rows
@@ -1082,13 +1158,13 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
     }
     const Args::Kind& kind = a.kind[en.kind];
     const int seg = items_before(a, e) + (int)kvh + (int)share;
-    float* dst = kind.part + ((size_t)seg * kind.rows + 16 * j + g) * kRow;
-    if (16 * j + g < en.rows) {
+    float* dst = kind.part + ((size_t)seg * kind.rows + g) * kRow;
+    if (g < en.rows) {
 #pragma unroll
       for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) = make_float2(O[n][0], O[n][1]);
       if (t == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(m0, l0);
     }
-    if (16 * j + g + 8 < en.rows) {
+    if (g + 8 < en.rows) {
       dst += 8 * kRow;
 #pragma unroll
       for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) = make_float2(O[n][2], O[n][3]);
@@ -1098,8 +1174,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
   if (second) griddep_wait();
 }
 
-// One warp per (row, head): the row's partials of its group's item (found by lanes 0..15) and of its own (lanes 16..31),
-// combined by their maxima.  A lane looks up a partial and its maximum and sum; then the lanes share the outputs' columns.
+// One warp per (row, head): the row's partials of its group's item (found by lanes 0..15) and of its own (lanes 16..31, or
+// all where it has no group), combined by their maxima.  A lane looks up a partial and its maximum and sum; then the lanes share the outputs' columns.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constant__ Args a) {
   using TL = Tile<HD>;
@@ -1109,14 +1185,15 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
   if (id >= (uint32_t)(a.seqs.n * a.positions) * a.nh) return;
   const int head = (int)(id % a.nh), row = (int)(id / a.nh);
   const int b = row / a.positions, kvh = head / a.group;
-  const int k = lane / 16;  // kind
-  const int e = k == 0 ? group_of(a, b) : a.groups.n + b;
+  const int its_group = group_of(a, b), width = its_group < 0 ? 32 : 16;  // lanes of a kind
+  const int k = lane / width + width / 32;  // kind
+  const int e = k == 0 ? its_group : a.groups.n + b;
   const Args::Kind& kind = a.kind[k];
   // the item of the row, and its row in a segment
   Entry en;
   int tile = 0, r = 0;
   bool pair = false;
-  if (e >= 0) {
+  {
     en = entry_of(a, e);
     const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
     tile = kind.tile ? kvh * en.tiles + x / kRowTile : kvh;
@@ -1126,28 +1203,27 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
     if (pair) r += x % kRowTile / 128 * kind.rows;
   }
   const uint32_t per = kind.tile && !pair ? 2 : 1, seg_rows = kind.tile ? 2 * kind.rows : kind.rows;
-  const uint32_t item = e >= 0 ? items_before(a, e) + tile : 0;
+  const uint32_t item = items_before(a, e) + tile;
   griddep_wait();
   griddep_launch();
-  uint32_t n = 0, c0 = 0, u0 = 0, pages = 0, wt = 1;
+  uint32_t n = 0, c0 = 0, u0 = 0, units = 0;
   Shares shares{0, 1, 0};
-  if (e >= 0 && a.seqs.base(b) >= 0) {
-    pages = kind.plan->pages[e];
+  if (a.seqs.base(b) >= 0) {
+    units = units_of(en, kind.plan->pages[e]);
     const uint32_t cum = kind.plan->cum[e];
     shares = kind.plan->cut();
-    if (pages > 0) {
-      wt = en.weight;
-      u0 = cum + tile * pages * wt;
+    if (units > 0) {
+      u0 = cum + tile * units;
       c0 = shares.of(u0);
-      n = (shares.of(u0 + (pages - 1) * wt) - c0 + 1) * per;
+      n = (shares.of(u0 + units - 1) - c0 + 1) * per;
     }
   }
-  const uint32_t rounds = __reduce_max_sync(0xffffffffu, (n + 15) / 16);
+  const uint32_t rounds = __reduce_max_sync(0xffffffffu, (n + width - 1) / width);
   float M = -INFINITY, l = 0.0f, acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.0f;
   for (uint32_t round = 0; round < rounds; ++round) {
-    const uint32_t i = 16 * round + lane % 16;
+    const uint32_t i = width * round + lane % width;
     float2 ml = make_float2(-INFINITY, 0.0f);
     uint32_t src = 0;  // the partial's row
     bool have = false;
@@ -1155,8 +1231,8 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
       const uint32_t c = c0 + i / per, s = i % per;
       // pages of the item that share c holds (none, where it is narrower than a page's units; the second stream has
       // some where there are two or more)
-      const uint32_t w0 = max(shares.begin(c), u0) - u0, w1 = shares.begin(c + 1) - u0;
-      have = min(pages, (w1 + wt - 1) / wt) - min(pages, (w0 + wt - 1) / wt) > s;
+      const uint32_t w0 = max(shares.begin(c), u0) - u0, w1 = min(units, shares.begin(c + 1) - u0);
+      have = pages_before(en, w1) - pages_before(en, w0) > s;
       src = (item + c) * seg_rows + s * kind.rows + r;
       if (have) ml = *reinterpret_cast<const float2*>(kind.part + (size_t)src * TL::kRow + HD);
     }
@@ -1176,7 +1252,8 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
       for (int q = 0; q < 4; ++q) {  // four partials' loads in flight
         const int from = todo ? __ffs(todo) - 1 : 0;
         w[q] = todo ? __shfl_sync(0xffffffffu, f, from) : 0.0f;
-        const float* p = (from < 16 ? a.kind[0].part : a.kind[1].part) + (size_t)__shfl_sync(0xffffffffu, src, from) * TL::kRow;
+        const float* p = (width == 16 && from < 16 ? a.kind[0].part : a.kind[1].part) +
+                         (size_t)__shfl_sync(0xffffffffu, src, from) * TL::kRow;
         if (todo) {
           if constexpr (N == 4) {
             const float4 v = *reinterpret_cast<const float4*>(p + 4 * lane);
@@ -1215,7 +1292,6 @@ size_t al256(size_t n) { return (n + 255) & ~(size_t)255; }
 // How a call is laid out: which kernel takes the groups and which the sequences, and the workspace.
 struct Layout {
   bool tile[2];     // groups, sequences: the tile kernel
-  int team[2];      // warps of a team of the stream kernel
   int tiles;        // row tiles of a sequence
   int rows[2];      // row capacity of a segment (tile kernel: of half of one)
   int shares[2];
@@ -1237,10 +1313,6 @@ Layout layout_of(int n, int positions, int nh, int nkv, int hd, const KvGroups& 
   const int widest[2] = {most, rows};
   s.tile[1] = rows > kStreamRows;
   s.tile[0] = any ? most > kStreamRows : s.tile[1];  // without shared pages there is one kernel
-  auto team_of = [](int r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; };
-  s.team[1] = team_of(rows);
-  s.team[0] = any ? team_of(most) : s.team[1];
-  if (!s.tile[0] && !s.tile[1]) s.team[0] = s.team[1] = std::max(s.team[0], s.team[1]);  // one launch, one team size
   s.tiles = s.tile[1] ? (rows + kRowTile - 1) / kRowTile : 1;
   size_t items[2] = {0, (size_t)n * s.tiles * nkv};
   for (int g = 0; g < groups.n; ++g)
@@ -1249,20 +1321,12 @@ Layout layout_of(int n, int positions, int nh, int nkv, int hd, const KvGroups& 
   s.plan = al256(sizeof(Plan));
   for (int k = 0; k < 2; ++k) {
     s.rows[k] = s.tile[k] ? std::min(k ? rows : 128, 128) : std::max(1, widest[k]);
-    s.shares[k] = s.tile[k] ? sm_count : sm_count * kStreamWarps / s.team[k];
+    s.shares[k] = s.tile[k] ? sm_count : sm_count * kStreamWarps;
     s.part[k] = k == 0 && !any ? 0
                                : al256((items[k] + s.shares[k]) * (s.tile[k] ? 2 : 1) * s.rows[k] * (size_t)(hd + kSegPad) *
                                        sizeof(float));
   }
   return s;
-}
-
-template <typename T, int HD>
-int launch_stream(const Args& a, int team, bool second, int sm_count, cudaStream_t st) {
-  const dim3 grid((unsigned)sm_count), block(32 * kStreamWarps);
-  if (team == 1) return launch_pdl(kv_stream_kernel<T, HD, 1>, grid, block, 0, st, a, (int)second);
-  if (team == 2) return launch_pdl(kv_stream_kernel<T, HD, 2>, grid, block, 0, st, a, (int)second);
-  return launch_pdl(kv_stream_kernel<T, HD, 4>, grid, block, 0, st, a, (int)second);
 }
 
 template <typename T, typename O, int HD>
@@ -1275,7 +1339,7 @@ int launch_typed(const Args& a, const Layout& s, int sm_count, cudaStream_t st) 
   }
   // (on the default streams launches do not overlap, and the second one need not wait)
   if (!s.tile[0] || !s.tile[1])
-    CLM_TRY((launch_stream<T, HD>(a, s.team[s.tile[0] ? 1 : 0], tiled, sm_count, st)));
+    CLM_TRY(launch_pdl(kv_stream_kernel<T, HD>, dim3((unsigned)sm_count), dim3(32 * kStreamWarps), 0, st, a, (int)tiled));
   const uint64_t rows = (uint64_t)a.seqs.n * a.positions * a.nh;
   return launch_pdl(kv_combine_kernel<O, HD>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, a);
 }
@@ -1288,7 +1352,7 @@ size_t kv_attention_work(int n, int positions, int nh, int nkv, int hd, const Kv
 
 int launch_kv_attention(const KvAttnArgs& in, cudaStream_t st) {
   const Layout s = layout_of(in.seqs.n, in.positions, in.nh, in.nkv, in.hd, in.groups, in.sm_count);
-  CLM_CHECK(s.items * (size_t)(in.seqs.max_pages + 2) < (1ull << 31), CLM_OUT_OF_RANGE,
+  CLM_CHECK(s.items * (size_t)(in.seqs.max_pages + kSwitch) < (1ull << 31), CLM_OUT_OF_RANGE,
             "attention: too many pages in one call (narrower page tables, or fewer sequences)");
   CLM_CHECK(in.work != nullptr && in.work_bytes >= s.total(), CLM_RESOURCE_EXHAUSTED, "attention workspace too small");
   Args a;

@@ -16,13 +16,19 @@ namespace clm {
 // P f is formed and reduced modulo 2 pi in double (at P = 10^6 an f32 angle is off by 0.03 rad); the reduced angle's
 // sine and cosine are f32.  Products are f32 and round once to the cache's type.
 //
-// One CTA per (sequence, page its rows touch, kv head): the angles of the page's rows are evaluated once into shared
-// memory and serve the kv head's query heads and its key head; the value rows are transposed through shared memory,
-// because a V page keeps a dimension's 64 positions together (128 bytes): eight threads write such a line.
+// One CTA per (sequence, quarter page that its rows touch, range of kv heads): the rows' angles are evaluated once into
+// shared memory and serve all its heads; the value rows are transposed through shared memory, because a V page keeps a
+// dimension's 64 positions together: two threads write a quarter's 32 bytes.
+//
+// Bound by memory.  4,096 rows of 64 + 8 + 8 heads of 128, f32 to fp16 (252 MB): 47 us, 5.4 TB/s; with 256 threads a CTA
+// 56 us, with 64 58 us; with a CTA per (page, kv head), whose angles are evaluated once per kv head, 65 us.  16 sequences
+// of 4 rows (1.6 MB): 6 us, a launch and three dependent reads.
 // ---------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
+constexpr int kAppendRows = 16;   // positions of a CTA: a quarter page
+constexpr int kAppendHeads = 8;   // kv heads of a CTA at most
 
 struct AppendArgs {
   KvSeqs seqs;
@@ -32,7 +38,7 @@ struct AppendArgs {
   const double* freq;
   const int32_t* parent;
   float scale;
-  int positions, nh, nkv, hd, rot, interleaved, chunks;
+  int positions, nh, nkv, hd, rot, interleaved, blocks, heads;  // CTAs of a sequence; kv heads of a CTA
   int vec_q, vec_k, vec_v;  // rows start 16-byte aligned: vector loads
 };
 
@@ -63,46 +69,21 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
 }
 
-// Elements [d0, d0 + 8) of a head's row `p` after the rotation; cs[j] = (cos, sin) of the row's pair j.
+// Elements [d0, d0 + 8) of a head's row `p` after the rotation; cs[j] = (cos, sin) of the row's pair j.  (Rotations whose
+// halves are not whole chunks; rotate_rows has the others.)
 template <typename S>
 __device__ __forceinline__ void rotate8(const S* p, int d0, const AppendArgs& a, bool vec, const float2* cs,
                                         float (&o)[8]) {
   float x[8];
   load8(p + d0, vec, x);
-  if (d0 >= a.rot) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = x[i];
-    return;
-  }
-  if (a.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (d0 + 2 * i < a.rot) {
-        const float2 c = cs[d0 / 2 + i];
-        o[2 * i] = x[2 * i] * c.x - x[2 * i + 1] * c.y;
-        o[2 * i + 1] = x[2 * i] * c.y + x[2 * i + 1] * c.x;
-      } else {
-        o[2 * i] = x[2 * i];
-        o[2 * i + 1] = x[2 * i + 1];
-      }
-    }
-    return;
-  }
-  const int half = a.rot / 2;
-  if (half % 8 == 0) {  // the eight elements lie in one half, their partners are eight consecutive elements
-    float y[8];
-    const bool low = d0 < half;
-    load8(p + (low ? d0 + half : d0 - half), vec, y);
-    const float2* c8 = cs + (low ? d0 : d0 - half);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = low ? x[i] * c8[i].x - y[i] * c8[i].y : y[i] * c8[i].y + x[i] * c8[i].x;
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int d = d0 + i;
+    const int d = d0 + i, half = a.rot / 2;
     if (d >= a.rot) {
       o[i] = x[i];
+    } else if (a.interleaved) {
+      const float2 c = cs[d / 2];
+      o[i] = i % 2 == 0 ? x[i] * c.x - x[i + 1 & 7] * c.y : x[i - 1 & 7] * c.y + x[i] * c.x;
     } else if (d < half) {
       const float2 c = cs[d];
       o[i] = x[i] * c.x - to_f32(p[d + half]) * c.y;
@@ -113,36 +94,118 @@ __device__ __forceinline__ void rotate8(const S* p, int d0, const AppendArgs& a,
   }
 }
 
+// Runs over the (row, head, unit)s of a page's rows, a thread every kAppendThreads-th: carried along, not divided for.
+struct RowWalk {
+  int r, h, u;
+  int heads, units, dr, dh, du;
+  __device__ __forceinline__ RowWalk(int n_heads, int n_units) : heads(n_heads), units(n_units) {
+    const int per = heads * units;
+    r = threadIdx.x / per, dr = kAppendThreads / per;
+    const int x = threadIdx.x % per, y = kAppendThreads % per;
+    h = x / units, dh = y / units;
+    u = x % units, du = y % units;
+  }
+  __device__ __forceinline__ void next() {
+    u += du, h += dh, r += dr;
+    if (u >= units) u -= units, ++h;
+    if (h >= heads) h -= heads, ++r;
+  }
+};
+
+// Rotates the heads' rows [0, nr) of `src` and gives their chunks to store(row, head, first element, values).  With halves
+// of whole chunks a unit is a chunk of the first half and its partner: each element is read once, and two units'
+// loads are in flight.
+template <typename S, typename F>
+__device__ __forceinline__ void rotate_rows(const S* src, long long ld, int heads, int nr, const AppendArgs& a, bool vec,
+                                            const float2* cs, F&& store) {
+  const int half = a.rot / 2, hd = a.hd;
+  if (a.interleaved ? a.rot % 8 == 0 : half % 8 == 0) {
+    const int pairs = a.interleaved ? a.rot / 8 : half / 8;  // units that rotate; the rest are chunks that stay
+    RowWalk w(heads, pairs + (hd - a.rot) / 8);
+    while (w.r < nr) {
+      float x[2][8], y[2][8];
+      int r[2], h[2], d[2];
+      bool turn[2], two[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        r[q] = w.r, h[q] = w.h;
+        turn[q] = w.u < pairs;
+        two[q] = turn[q] && !a.interleaved;
+        d[q] = turn[q] ? 8 * w.u : a.rot + 8 * (w.u - pairs);
+        if (r[q] < nr) {
+          const S* p = src + (long long)r[q] * ld + h[q] * hd + d[q];
+          load8(p, vec, x[q]);
+          if (two[q]) load8(p + half, vec, y[q]);
+        }
+        w.next();
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (r[q] >= nr) continue;
+        float o[8];
+        if (two[q]) {
+          const float2* c8 = cs + r[q] * half + d[q];
+          float o2[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 c = c8[i];
+            o[i] = x[q][i] * c.x - y[q][i] * c.y;
+            o2[i] = x[q][i] * c.y + y[q][i] * c.x;
+          }
+          store(r[q], h[q], d[q] + half, o2);
+        } else if (turn[q]) {
+          const float2* c4 = cs + r[q] * half + d[q] / 2;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 c = c4[i];
+            o[2 * i] = x[q][2 * i] * c.x - x[q][2 * i + 1] * c.y;
+            o[2 * i + 1] = x[q][2 * i] * c.y + x[q][2 * i + 1] * c.x;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = x[q][i];
+        }
+        store(r[q], h[q], d[q], o);
+      }
+    }
+    return;
+  }
+  for (RowWalk w(heads, hd / 8); w.r < nr; w.next()) {
+    float o[8];
+    rotate8(src + (long long)w.r * ld + w.h * hd, 8 * w.u, a, vec, cs + w.r * half, o);
+    store(w.r, w.h, 8 * w.u, o);
+  }
+}
+
 template <typename S, typename T>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
   extern __shared__ __align__(16) uint8_t ap_smem[];
-  __shared__ int s_depth[kPageTokens];
+  __shared__ int s_depth[kAppendRows];
   griddep_wait();
   griddep_launch();
-  const int b = blockIdx.x / a.chunks, c = blockIdx.x % a.chunks, kvh = blockIdx.y;
-  const int group = a.nh / a.nkv, hd = a.hd, hv = hd / 8, half = a.rot / 2;
-  float2* cs = reinterpret_cast<float2*>(ap_smem);  // [64][half]
-  const int vld = hd + 2;                           // padded row of the value tile, elements
-  T* vt = reinterpret_cast<T*>(ap_smem + (size_t)kPageTokens * half * sizeof(float2));
+  const int b = blockIdx.x / a.blocks, c = blockIdx.x % a.blocks, kv0 = blockIdx.y * a.heads;
+  const int kvn = min(a.heads, a.nkv - kv0), group = a.nh / a.nkv, hd = a.hd, half = a.rot / 2;
+  float2* cs = reinterpret_cast<float2*>(ap_smem);  // [16][half]
+  const int vld = hd + 2;                           // padded row of the value tiles, elements
+  T* vt = reinterpret_cast<T*>(ap_smem + (size_t)kAppendRows * half * sizeof(float2));  // [heads][16][vld]
   const long long base = a.seqs.base(b);
   const S* q = static_cast<const S*>(a.q);
   T* q_out = static_cast<T*>(a.q_out);
   const int g0 = b * a.positions;  // the sequence's first row
   if (base < 0) {                  // an idle sequence: nothing enters the cache, its query rows become zero
-    const int r0 = c * kPageTokens, nr = min(kPageTokens, a.positions - r0);
+    const int r0 = c * kAppendRows, nr = min(kAppendRows, a.positions - r0), per = kvn * group * hd / 8;
     if (q != nullptr)
-      for (int i = threadIdx.x; i < nr * group * hv; i += kAppendThreads) {
-        const int r = i / (group * hv), x = i % (group * hv);
-        *reinterpret_cast<uint4*>(q_out + ((size_t)(g0 + r0 + r) * a.nh + kvh * group) * hd + 8 * x) =
+      for (int i = threadIdx.x; i < nr * per; i += kAppendThreads)
+        *reinterpret_cast<uint4*>(q_out + ((size_t)(g0 + r0 + i / per) * a.nh + kv0 * group) * hd + 8 * (i % per)) =
             make_uint4(0u, 0u, 0u, 0u);
-      }
     return;
   }
-  const long long pg = base / kPageTokens + c;
-  const long long lo = max(base, pg * kPageTokens), hi = min(base + a.positions, (pg + 1) * kPageTokens);
-  const int r0 = (int)(lo - base), nr = (int)(hi - lo);  // rows r0 .. r0 + nr - 1 of the window lie in this page
+  const long long block = base / kAppendRows + c, pg = block / (kPageTokens / kAppendRows);
+  const long long lo = max(base, block * kAppendRows), hi = min(base + a.positions, (block + 1) * kAppendRows);
+  const int r0 = (int)(lo - base), nr = (int)(hi - lo);  // rows r0 .. r0 + nr - 1 of the window lie in this block
   if (nr <= 0) return;
-  const int p0 = (int)(lo % kPageTokens);  // the first one's place in the page
+  const int at0 = (int)(block % (kPageTokens / kAppendRows)) * kAppendRows;  // the block's first position in the page
+  const int p0 = (int)(lo % kAppendRows);                                    // the first row's place in the block
   int32_t page = pg < a.seqs.max_pages ? a.seqs.table(b)[pg] : -1;
   if (page >= a.seqs.pool_pages) page = -1;  // no page: the rows are rotated but not kept
   for (int r = threadIdx.x; r < nr; r += kAppendThreads) {
@@ -168,52 +231,48 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     sincosf((float)red, &sn, &cn);
     cs[i] = make_float2(cn * a.scale, sn * a.scale);
   }
-  // the value tile, rows at their place in the page (with the angles: one barrier for both)
+  // the value tiles, rows at their place in the block (with the angles: one barrier for both)
   if (page >= 0) {
-    const S* v = static_cast<const S*>(a.v);
-    for (int i = threadIdx.x; i < nr * hv; i += kAppendThreads) {
-      const int r = i / hv, d0 = 8 * (i % hv);
+    const S* v = static_cast<const S*>(a.v) + (long long)(g0 + r0) * a.ld_v + kv0 * hd;
+#pragma unroll 2
+    for (RowWalk w(kvn, hd / 8); w.r < nr; w.next()) {
       float x[8];
-      load8(v + (long long)(g0 + r0 + r) * a.ld_v + kvh * hd + d0, a.vec_v, x);
-      uint32_t* t = reinterpret_cast<uint32_t*>(vt + (size_t)(p0 + r) * vld + d0);
+      load8(v + (long long)w.r * a.ld_v + w.h * hd + 8 * w.u, a.vec_v, x);
+      uint32_t* t = reinterpret_cast<uint32_t*>(vt + (size_t)(w.h * kAppendRows + p0 + w.r) * vld + 8 * w.u);
 #pragma unroll
       for (int k = 0; k < 4; ++k) t[k] = pack2<T>(x[2 * k], x[2 * k + 1]);
     }
   }
   __syncthreads();
   if (q != nullptr)
-    for (int i = threadIdx.x; i < nr * group * hv; i += kAppendThreads) {
-      const int r = i / (group * hv), x = i % (group * hv), d0 = 8 * (x % hv);
-      const int head = kvh * group + x / hv;
-      float o[8];
-      rotate8(q + (long long)(g0 + r0 + r) * a.ld_q + (long long)head * hd, d0, a, a.vec_q, cs + r * half, o);
-      *reinterpret_cast<uint4*>(q_out + ((size_t)(g0 + r0 + r) * a.nh + head) * hd + d0) = pack8<T>(o);
-    }
+    rotate_rows(q + (long long)(g0 + r0) * a.ld_q + kv0 * group * hd, a.ld_q, kvn * group, nr, a, a.vec_q, cs,
+                [&](int r, int h, int d, const float(&o)[8]) {
+                  *reinterpret_cast<uint4*>(q_out + ((size_t)(g0 + r0 + r) * a.nh + kv0 * group + h) * hd + d) = pack8<T>(o);
+                });
   if (page < 0) return;
-  const size_t at = ((size_t)page * a.nkv + kvh) * kPageTokens * hd;
+  const size_t at = ((size_t)page * a.nkv + kv0) * kPageTokens * hd;
   T* kp = static_cast<T*>(a.kpool) + at;
   T* vp = static_cast<T*>(a.vpool) + at;
-  const S* k = static_cast<const S*>(a.k);
-  for (int i = threadIdx.x; i < nr * hv; i += kAppendThreads) {
-    const int r = i / hv, ch = i % hv, pos = p0 + r;
-    float o[8];
-    rotate8(k + (long long)(g0 + r0 + r) * a.ld_k + kvh * hd, 8 * ch, a, a.vec_k, cs + r * half, o);
-    *reinterpret_cast<uint4*>(kp + (size_t)pos * hd + 8 * kv_k_chunk(ch, pos)) = pack8<T>(o);
-  }
-  const int c_lo = p0 / 8, c_n = (p0 + nr - 1) / 8 - c_lo + 1;  // position chunks the rows touch
-  for (int i = threadIdx.x; i < hd * c_n; i += kAppendThreads) {
-    const int d = i / c_n, pc = c_lo + i % c_n;
-    T* dst = vp + (size_t)d * kPageTokens + 8 * kv_v_chunk(pc, d);
+  rotate_rows(static_cast<const S*>(a.k) + (long long)(g0 + r0) * a.ld_k + kv0 * hd, a.ld_k, kvn, nr, a, a.vec_k, cs,
+              [&](int r, int h, int d, const float(&o)[8]) {
+                const int pos = at0 + p0 + r;
+                *reinterpret_cast<uint4*>(kp + (size_t)(h * kPageTokens + pos) * hd + 8 * kv_k_chunk(d / 8, pos)) = pack8<T>(o);
+              });
+  // chunks of 8 positions of a dimension, two a block
+  for (int i = threadIdx.x; i < 2 * kvn * hd; i += kAppendThreads) {
+    const int pc = i % 2, d = i / 2 % hd, h = i / 2 / hd;
+    const T* from = vt + (size_t)(h * kAppendRows + 8 * pc) * vld + d;
+    T* dst = vp + (size_t)(h * hd + d) * kPageTokens + 8 * kv_v_chunk(at0 / 8 + pc, d);
     if (8 * pc >= p0 && 8 * pc + 8 <= p0 + nr) {
       T e[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = vt[(size_t)(8 * pc + j) * vld + d];
+      for (int j = 0; j < 8; ++j) e[j] = from[(size_t)j * vld];
       uint4 w;
       memcpy(&w, e, 16);
       *reinterpret_cast<uint4*>(dst) = w;
     } else {  // a chunk that other rows share: the other positions stay as they are
       for (int j = 0; j < 8; ++j)
-        if (8 * pc + j >= p0 && 8 * pc + j < p0 + nr) dst[j] = vt[(size_t)(8 * pc + j) * vld + d];
+        if (8 * pc + j >= p0 && 8 * pc + j < p0 + nr) dst[j] = from[(size_t)j * vld];
     }
   }
 }
@@ -429,9 +488,9 @@ bool aligned16(const void* p, long long ld, size_t es) {
 
 template <typename S, typename T>
 int launch_append(const AppendArgs& a, cudaStream_t st) {
-  const size_t smem = (size_t)kPageTokens * (a.rot / 2) * sizeof(float2) + (size_t)kPageTokens * (a.hd + 2) * sizeof(T);
-  CLM_TRY(ensure_smem(kv_append_kernel<S, T>, smem + kPageTokens * sizeof(int)));  // (the limit counts static memory too)
-  return launch_pdl(kv_append_kernel<S, T>, dim3((unsigned)(a.seqs.n * a.chunks), (unsigned)a.nkv),
+  const size_t smem = (size_t)kAppendRows * (a.rot / 2) * sizeof(float2) + (size_t)a.heads * kAppendRows * (a.hd + 2) * sizeof(T);
+  CLM_TRY(ensure_smem(kv_append_kernel<S, T>, smem + kAppendRows * sizeof(int)));  // (the limit counts static memory too)
+  return launch_pdl(kv_append_kernel<S, T>, dim3((unsigned)(a.seqs.n * a.blocks), (unsigned)ceil_div(a.nkv, a.heads)),
                     dim3(kAppendThreads), smem, st, a);
 }
 
@@ -490,9 +549,13 @@ int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t
   a.hd = (int)pool->head_dim;
   a.rot = (int)rot;
   a.interleaved = rope && rope->layout == CLM_ROPE_INTERLEAVED;
-  // pages that `positions` rows starting anywhere touch at most
-  a.chunks = positions == 1 ? 1 : (int)((positions - 2) / kPageTokens + 2);
-  CLM_CHECK((uint64_t)n * a.chunks <= 0x7fffffffull, CLM_OUT_OF_RANGE, "too many rows");
+  // blocks that `positions` rows starting anywhere touch at most
+  a.blocks = positions == 1 ? 1 : (int)((positions - 2) / kAppendRows + 2);
+  CLM_CHECK((uint64_t)n * a.blocks <= 0x7fffffffull, CLM_OUT_OF_RANGE, "too many rows");
+  // As few splits of the kv heads as fill the GPU (the angles are evaluated in each).
+  uint64_t splits = ceil_div((uint64_t)a.nkv, kAppendHeads);
+  splits = std::max(splits, std::min((uint64_t)a.nkv, ceil_div(6ull * ctx->sm_count, (uint64_t)n * a.blocks)));
+  a.heads = (int)ceil_div((uint64_t)a.nkv, splits);
   const size_t es = dtype_size(src_dtype);
   a.vec_q = aligned16(d_q, a.ld_q, es);
   a.vec_k = aligned16(d_k, a.ld_k, es);

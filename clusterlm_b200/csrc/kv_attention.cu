@@ -1236,24 +1236,16 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
       src = (item + c) * seg_rows + s * kind.rows + r;
       if (have) ml = *reinterpret_cast<const float2*>(kind.part + (size_t)src * TL::kRow + HD);
     }
-    float m = fmaxf(M, ml.x);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const float keep = ex2(M - ref), f = ex2(ml.x - ref);
-    float add = ml.y * f;
-    for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
-    M = m;
-    l = l * keep + add;
+    // four partials' loads at a time in flight, the first ones before the maxima are here
+    uint32_t todo = __ballot_sync(0xffffffffu, have);
+    float o[4][N];
+    int from[4];
+    auto load = [&]() {
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] *= keep;
-    for (uint32_t todo = __ballot_sync(0xffffffffu, have); todo;) {
-      float o[4][N], w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {  // four partials' loads in flight
-        const int from = todo ? __ffs(todo) - 1 : 0;
-        w[q] = todo ? __shfl_sync(0xffffffffu, f, from) : 0.0f;
-        const float* p = (width == 16 && from < 16 ? a.kind[0].part : a.kind[1].part) +
-                         (size_t)__shfl_sync(0xffffffffu, src, from) * TL::kRow;
+      for (int q = 0; q < 4; ++q) {
+        from[q] = todo ? __ffs(todo) - 1 : -1;
+        const float* p = (width == 16 && from[q] < 16 ? a.kind[0].part : a.kind[1].part) +
+                         (size_t)__shfl_sync(0xffffffffu, src, from[q] & 31) * TL::kRow;
         if (todo) {
           if constexpr (N == 4) {
             const float4 v = *reinterpret_cast<const float4*>(p + 4 * lane);
@@ -1268,10 +1260,27 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
         }
         todo &= todo - 1;
       }
+    };
+    load();
+    float m = fmaxf(M, ml.x);
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const float keep = ex2(M - ref), f = ex2(ml.x - ref);
+    float add = ml.y * f;
+    for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+    M = m;
+    l = l * keep + add;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+    for (int j = 0; j < N; ++j) acc[j] *= keep;
+    for (;;) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += o[q][j] * w[q];
+      for (int q = 0; q < 4; ++q) {
+        const float w = __shfl_sync(0xffffffffu, f, from[q] & 31);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += o[q][j] * (from[q] < 0 ? 0.0f : w);
+      }
+      if (todo == 0) break;
+      load();
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;

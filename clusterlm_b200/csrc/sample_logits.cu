@@ -16,7 +16,7 @@
 //      with them: the row's whole mass and a histogram of the entries over 64 bins per octave of e, whose counts bound
 //      the cumulative mass within 1.1%: the cut falls into known bins.  Entries above these are allowed (their exact
 //      mass is summed), entries below are not, and the few in them are ranked: their key range in 64 parts with exact
-//      masses, then the members of the cut's part one against the other.  Where more than kCand entries share those
+//      masses, then the members of the cut's part one against the other.  Where kCand or more entries share those
 //      bins (a flat row, or equal logits, as from 16-bit types), their key range is divided again; where one key value
 //      is left, its lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
@@ -39,7 +39,7 @@ constexpr int kWrp = kThr / 32;    // warp segments of a CTA's slice
 constexpr int kBinsOct = 64;       // histogram bins per octave
 constexpr int kBins = 44 * kBinsOct;
 constexpr int kOwn = kBins / kCl;  // bins whose row totals a CTA forms
-constexpr int kCand = 1024;        // candidates of a row that are ranked
+constexpr int kCand = 1024;        // candidates of a row that are ranked are fewer
 constexpr int kMine = 384;         // of one CTA
 constexpr int kSub = 64;           // parts of the candidates' key range
 constexpr int kFrac = 44;          // fraction bits of a mass
@@ -50,6 +50,17 @@ typedef unsigned long long u64;
 struct Cand {
   uint32_t u, idx;  // |d| (ascends as the order does) and index
   u64 w;
+};
+
+// A sum of fewer than 1,024 masses (of up to 2^44 each), by two 32-bit atomic additions: shared memory has them in
+// hardware, where a 64-bit one is a loop.
+struct Split {
+  uint32_t hi, lo;
+  __device__ __forceinline__ void add(u64 w) {
+    atomicAdd(&hi, (uint32_t)(w >> 22));
+    atomicAdd(&lo, (uint32_t)w & 0x3fffffu);
+  }
+  __device__ __forceinline__ u64 sum() const { return ((u64)hi << 22) + lo; }
 };
 
 struct SampleArgs {
@@ -105,8 +116,8 @@ struct Shared {
   u64 red[kWrp];
   uint32_t redc[kWrp];
   float redf[2][kWrp];
-  u64 sub_mass[kSub];
   uint32_t sub_cnt[kSub];
+  Split sub_mass[kSub], seg_add[kWrp];
   uint32_t cand_n, cut_n;
   double table[64];     // 2^(j / 64)
   float few[kWrp][192];  // entries whose masses a warp has yet to sum
@@ -505,7 +516,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         ul = nl;
         uh = umax = nh;
       }
-      return all_allowed || (cand <= kCand && most <= kMine);
+      return all_allowed || (cand < kCand && most <= kMine);
     };
     bool done = look(std::true_type{});
     for (int level = 1; !done; ++level) {
@@ -573,15 +584,14 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       done = look(std::false_type{});
     }
     seg_mass = warp_sum(seg_mass);
-    __syncthreads();
-    if (lane == 0) s.seg[warp] = seg_mass;
     if (!struck && cand > 0) {
       // The candidates' key range in kSub parts, with exact counts and masses: the cut falls into one part, and only its
       // members are ranked one against the other.
       for (int i = tid; i < kSub; i += kThr) {
-        s.sub_mass[i] = 0;
+        s.sub_mass[i] = Split{0, 0};
         s.sub_cnt[i] = 0;
       }
+      if (tid < kWrp) s.seg_add[tid] = Split{0, 0};
       if (tid == 0) s.cut_n = 0;
       __syncthreads();
       const uint32_t u0 = ul;
@@ -602,7 +612,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           if (!direct) {
             const int p = part_of(x.u);
             atomicAdd(&s.sub_cnt[p], 1u);
-            atomicAdd(&s.sub_mass[p], x.w);
+            s.sub_mass[p].add(x.w);
           }
         }
       }
@@ -610,7 +620,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       // every warp: two parts a lane, cumulative; the first part that reaches top-k or top-p holds the cut
       static_assert(kSub == 64, "two parts a lane");
       const uint32_t c0 = s.sub_cnt[2 * lane], c1 = s.sub_cnt[2 * lane + 1];
-      const u64 w0 = s.sub_mass[2 * lane], w1 = s.sub_mass[2 * lane + 1];
+      const u64 w0 = s.sub_mass[2 * lane].sum(), w1 = s.sub_mass[2 * lane + 1].sum();
       uint32_t cx = c0 + c1;
       u64 wx = w0 + w1;
       for (int o = 1; o < 32; o <<= 1) {
@@ -667,11 +677,11 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         if (!allowed)
           key[me.idx - v0] = -INFINITY;
         else
-          atomicAdd(&s.seg[(me.idx - v0) / seg], me.w);
+          s.seg_add[(me.idx - v0) / seg].add(me.w);
       }
+      __syncthreads();
+      seg_mass += s.seg_add[warp].sum();
     }
-    __syncthreads();
-    seg_mass = s.seg[warp];
   }
 
   // ---- 3. the token

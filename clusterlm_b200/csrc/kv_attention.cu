@@ -4,16 +4,23 @@
 // its sequence shares with its group and the sequence's own pages; both parts (and any further split of them) give a
 // partial (unnormalised o, running maximum m, sum l), and partials combine by their maxima.
 //
-// An "entry" is a group's shared pages (rows: all query heads of a kv head of all the group's window rows) or a sequence's
-// own pages (rows: its own).  Entries of up to kStreamRows rows per kv head are bound by reading the pages: the stream
-// kernel, whose warps load the operands of mma.sync straight from global memory.  Entries of more rows are bound by the
-// products: the tile kernel, on the tensor cores' accumulators in TMEM.  All groups of a call go to one of the two, and
-// all sequences; so a call is one or two launches and the combining one.
+// An "entry" is a group's shared pages (rows: all query heads of a kv head of all the group's window rows) or a
+// sequence's own pages (rows: its own).  Entries of up to kStreamRows rows per kv head are bound by reading the
+// pages: the stream kernel, whose warps load the operands of mma.sync straight from global memory.  Entries of more
+// rows are bound by the products: the tile kernel, on the tensor cores' accumulators in TMEM.  All groups of a call
+// go to one of the two, and all sequences; so a call is one or two launches and the combining one.
 //
-// Work of a kernel is one line of units: per entry, per item (kv head, and row tile in the tile kernel), its pages (tile
-// kernel: counted double for more than 128 rows; stream kernel: half pages), and some for the item's own start and end.  The line is cut into
-// equal shares, one per CTA (stream kernel: per warp), so ragged lengths balance without any host knowledge of
-// them.  A share's part of an item is a segment, numbered by (item + share): both only grow along the line.
+// Work of a kernel is one line of units: per entry, per item (kv head, and row tile in the tile kernel), its pages
+// (tile kernel: counted double for more than 128 rows; stream kernel: half pages), and some units for an item's own
+// start and end.  The line is cut into equal shares, one per CTA (stream kernel: per warp), so ragged lengths balance
+// without any host knowledge of them.  A share's part of an item is a segment, numbered by (item + share): both only
+// grow along the line.
+//
+// GPU time of a call (fp16, head_dim 128, 32 heads over 8 unless said): 4 sequences of about 1,000 positions 13 us; 8
+// tree windows of 16 rows over 4,096 shared positions 34 us; 64 windows of 4 rows, 16,384 shared and about 500 own
+// positions each, 140 us (tile kernel 83 us, 0.83 PFLOP/s; stream kernel 36 us, 3.7 TB/s; combining kernel 13 us);
+// 256 rows over 8,192 positions (bf16) 105 us (0.72 PFLOP/s in the tile kernel); 64 sequences of 2,048 positions, 8
+// rows a kv head, 94 us (5.7 TB/s).
 #include <algorithm>
 #include <cfloat>
 
@@ -26,12 +33,18 @@ namespace clm {
 namespace {
 
 constexpr int kMaxEntries = kKvMaxGroups + kKvMaxSeqs;
-constexpr int kStreamRows = 16;  // entries of up to this many rows per kv head: the stream kernel
+// Entries of up to this many rows per kv head: the stream kernel.  (Whole calls with 17 to 64 rows, stream kernel
+// with up to four row tiles against tile kernel, head_dim 128: 8 sequences of 8,192 positions 72-118 against 62-65
+// us, 64 of 2,048 134-247 against 123-146, 4 of 512 12-15 against 16-17; up to 16 rows the stream kernel: 8 x 8,192
+// 58-60 us.)
+constexpr int kStreamRows = 16;
 constexpr int kStreamWarps = 8;  // warps of a stream CTA
 constexpr int kRowTile = 256;    // rows of an item of the tile kernel: two tiles of 128
 constexpr int kSegPad = 8;     // floats after a partial row's hd outputs: m, l, padding to 32 bytes
 constexpr int kStreamSwitch = 2;  // stream kernel: a segment's start and end take as long as this many half pages
-constexpr int kSwitch = 12;    // tile kernel: a segment's start and end take as long as this many units
+// Tile kernel: a segment's start and end take as long as this many units.  (8 tree windows of 16 rows over 4,096 shared
+// positions, both kinds of entries in the tile kernel: 0 units 81 us, 6 39 us, 12 34 us.)
+constexpr int kSwitch = 12;
 
 struct Plan {
   uint32_t cum[kMaxEntries + 1];  // work units before entry e (below 2^31, checked by the host)
@@ -135,8 +148,8 @@ struct Shares {
 
 __device__ __forceinline__ Shares Plan::cut() const { return Shares{shares, q, r}; }
 
-// Fills the plan of the tile (or stream) kernel from the device-side positions: pages per item, then the running work of
-// its entries (the other kernel's have none).  first: the entries' first pages.
+// Fills the plan of the tile (or stream) kernel from the device-side positions: pages per item, then the running work
+// of its entries (the other kernel's have none).  first: the entries' first pages.
 __device__ void make_plan(const Args& a, Plan* plan, int* first, int tile, uint32_t shares) {
   const int E = a.groups.n + a.seqs.n;
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
@@ -171,8 +184,8 @@ __device__ void make_plan(const Args& a, Plan* plan, int* first, int tile, uint3
     if (threadIdx.x == 0) {
       plan->cum[0] = 0;
       // Every share holds a unit.  Of the stream kernel three: a short segment spends more on its start and its partial
-      // (GPU time of a call with 4 sequences of about 1,000 positions, 8 kv heads, head_dim 128, with at least 2, 3, 4 or 6
-      // units a share: 14.5, 12.9, 13.6, 16.4 us).
+      // (GPU time of a call with 4 sequences of about 1,000 positions, 8 kv heads, head_dim 128, with at least 2, 3,
+      // 4 or 6 units a share: 14.5, 12.9, 13.6, 16.4 us).
       plan->shares = min(shares, tile ? run : (run + 2) / 3);
       plan->q = run ? run / plan->shares : 0u;
       plan->r = run ? run % plan->shares : 0u;
@@ -259,8 +272,8 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                : "memory");
 }
-// One lane of the warp.  (The compiler knows that a single lane runs what this guards: the products' operands then need no
-// loop over lanes.  Guarded by a comparison of the lane's number an instruction took 95 clocks to issue.)
+// One lane of the warp.  (The compiler knows that a single lane runs what this guards: the products' operands then
+// need no loop over lanes.  Guarded by a comparison of the lane's number an instruction took 95 clocks to issue.)
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
@@ -468,15 +481,21 @@ struct Walk {
 // ---------------------------------------------------------------------------------------------------
 // tile kernel: entries of more than 16 rows per kv head
 //
-// Two streams of four softmax warps each own 128 rows, one thread a row: no reductions across lanes.  With more than 128
-// rows the streams take a row tile each of every page; with fewer they take alternate pages of the same rows and give
-// two partials.  A stream has two score buffers, so the scores of its next page are computed while it weighs this one's;
-// its weights go back to TMEM as the first operand of their product with V.  O is rescaled only when a row's maximum
-// grows by more than 2^8 (weights stay below 2^8, far inside the types' range); the first maximum of a segment sets
-// the reference.
+// Two streams of four softmax warps each own 128 rows, one thread a row: no reductions across lanes.  With more than
+// 128 rows the streams take a row tile each of every page; with fewer they take alternate pages of the same rows and
+// give two partials.  A stream has two score buffers, so the scores of its next page are computed while it weighs
+// this one's; its weights go back to TMEM as the first operand of their product with V.  O is rescaled only when a
+// row's maximum grows by more than 2^8 (weights stay below 2^8, far inside the types' range); the first maximum of a
+// segment sets the reference.
 //
-// The producer warp copies the pages with 16-byte asynchronous copies, because the cache's chunk order is not the tensor
-// cores' (128-byte swizzle): each chunk goes straight to its place, where a bulk copy would need a reordering pass.
+// Bound by the tensor pipe: a page of both streams takes 2,230 clocks, of which 16 score products (M 128, N 64, K 16,
+// both operands in shared memory) take 107 each and 8 products with V 64 each.  (Score products of two pages, N 128,
+// take no longer, but their scores leave no room for a second buffer: a page of both streams then waits for its own
+// softmax, 3,100 clocks.  With half the query in TMEM, one score buffer: 2,750.)
+//
+// The producer warp copies the pages with 16-byte asynchronous copies, because the cache's chunk order is not the
+// tensor cores' (128-byte swizzle): each chunk goes straight to its place, where a bulk copy would need a reordering
+// pass.
 // ---------------------------------------------------------------------------------------------------
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_constant__ Args a) {
@@ -559,8 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
   Walk walk(a, plan, s_first, shares.begin(blockIdx.x), shares.begin(blockIdx.x + 1));
   Segment g;
   if (warp == kRelay) {
-    // ---------------- relay: copies that have landed become visible to the tensor cores (the copies are generic writes;
-    // the fence would cost a product warp its time), for the streams that use the page ----------------
+    // ---------------- relay: copies that have landed become visible to the tensor cores, for the streams that use the
+    // page (the copies are generic writes; the fence would cost a product warp its time) ----------------
     if (lane == 0) {
       uint32_t idx = 0, count[2] = {0, 0};
       bool ok = true;
@@ -832,8 +851,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[s][done & 1u]);
       }
-      // The next segment's query rows (the scores that read this one's are complete), then this one's partial rows, once
-      // its last products are complete.
+      // The next segment's query rows (the scores that read this one's are complete), then this one's partial rows,
+      // once its last products are complete.
       const Segment was = g;
       const int was_i = i, left = nrows - (warp % 4) * 32;
       const long long was_base = base;
@@ -897,12 +916,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
 //
 // A warp takes a share of the line and a row tile of 16; warps share nothing: a warp reads its operands from global
 // memory in the fragments' order (every K and V chunk is used by one lane), keeps its state in registers and writes its
-// own partial.  Eight warps a CTA, each with 8 to 16 KB of loads in flight, cover the memory's latency.
+// own partial.  Eight warps a CTA, each with 8 to 16 KB of loads in flight, cover the memory's latency: a half page of
+// head_dim 128 takes about 6,400 clocks with all warps at it, 5.7 TB/s.  The start (launch, plan, first rows and
+// pages: four dependent reads) takes 8,000, which is most of a short call.
 //
-// Fragment mapping (mma m16n8k16, lane = 4 g + t): column n of S's n-tile jj is position 8 (n / 2) + 2 jj + n % 2 of the
-// half page, so a lane's scores are positions 8 t + 2 jj + {0, 1}; the weights of n-tiles 2 kk and 2 kk + 1 are then the A
-// fragment of P V's k-step kk, whose B fragment is the lane's one chunk of V (positions 8 t .. 8 t + 7).  The dims of a
-// score are summed in the lane's order of K chunks (any order, alike in Q and K).
+// Fragment mapping (mma m16n8k16, lane = 4 g + t): column n of S's n-tile jj is position 8 (n / 2) + 2 jj + n % 2 of
+// the half page, so a lane's scores are positions 8 t + 2 jj + {0, 1}; the weights of n-tiles 2 kk and 2 kk + 1 are
+// then the A fragment of P V's k-step kk, whose B fragment is the lane's one chunk of V (positions 8 t .. 8 t + 7).
+// The dims of a score are summed in the lane's order of K chunks (any order, alike in Q and K).
 // ---------------------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -931,6 +952,8 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const __grid_constant__ Args a, int second) {
   constexpr int KW = HD / 32;  // 16-byte words of a K row per lane
   constexpr int kRow = HD + kSegPad;
+  // loads of the next half page before this one's products are done: head_dim 64 8 x 8,192 positions 36.1 -> 35.3 us;
+  // with 128 the registers do not hold them (98.9 -> 104.8 us, 64 sequences of 2,048)
   constexpr bool kAhead = HD == 64;
   __shared__ Plan plan;
   __shared__ int s_first[kMaxEntries];
@@ -999,8 +1022,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.0f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-    // K of the next half page (of table entry `pj`; of existing pages only) is asked for once the products with this one's
-    // are made, V after the weights' products, so that loads are in flight while the warp computes.
+    // K of the next half page (of table entry `pj`; of existing pages only) is asked for once the products with this
+    // one's are made, V after the weights' products, so that loads are in flight while the warp computes.
     int pj = -1;
     const T *ks = nullptr, *vs = nullptr;
     auto advance = [&]() {  // to the next existing page, if there is one
@@ -1112,8 +1135,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
           pa[jj][1] = pack2<T>(p10, p11);
         }
         if (!plain) {
-          // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  Such values
-          // are replaced by zero, and a second product of indicators finds the outputs they reach.
+          // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  Such
+          // values are replaced by zero, and a second product of indicators finds the outputs they reach.
           bool odd = false;
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n)
@@ -1174,8 +1197,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
   if (second) griddep_wait();
 }
 
-// One warp per (row, head): the row's partials of its group's item (found by lanes 0..15) and of its own (lanes 16..31, or
-// all where it has no group), combined by their maxima.  A lane looks up a partial and its maximum and sum; then the lanes share the outputs' columns.
+// One warp per (row, head): the row's partials of its group's item (found by lanes 0..15) and of its own (lanes
+// 16..31, or all where it has no group), combined by their maxima.  A lane looks up a partial and its maximum and
+// sum; then the lanes share the outputs' columns.  Bound by three dependent reads (plan; maxima, with the first four
+// partials; the others): 8,192 rows of 128 with six partials each 13 us, 25 MB.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constant__ Args a) {
   using TL = Tile<HD>;

@@ -20,6 +20,11 @@
 //      bins (a flat row, or equal logits, as from 16-bit types), their key range is divided again; where one key value
 //      is left, its lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
+//
+// Bound by instructions, and by the cluster's barriers where there are few rows: 1 row of 128,256 17 us (30,000
+// clocks, of which eight barriers and what waits for them take 15,000); 64 of 151,936 with top-p 77 us (two rows'
+// slices on an SM at a time: 1.7 waves of 58,000 clocks, half the issue slots used); 256 of 128,256 with mixed
+// settings 170 us.  A row on sixteen CTAs takes as long alone, and 138 and 317 us in those batches.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -219,7 +224,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   const float cf = (float)c;
   const bool need_k = k_in > 0 && (uint32_t)k_in < a.V, need_p = p_in < 1.0f;
   const uint32_t k = need_k ? (uint32_t)k_in : 0xffffffffu;
-  // entries below dcut have no mass (y < -45: it rounds to zero); entries below dlow are not allowed: dcut, or the first float whose y is log2(min_p) or more
+  // entries below dcut have no mass (y < -45: it rounds to zero); entries below dlow are not allowed: dcut, or the
+  // first float whose y is log2(min_p) or more
   const float dcut = fmaxf(-FLT_MAX, (float)(-45.5 / c));
   float dlow = dcut;
   if (m_in > 0.0f && !greedy) {
@@ -277,8 +283,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     seg_mass = warp_sum(seg_mass);
   } else {
     // The cut is located level by level.  A level looks at the entries with keys in [ul, uh]: those before are allowed
-    // (cnt_above of them, with the mass `above`), those behind are not.  Level 0 has all entries in bins of 1/64 octave of
-    // e; the others divide what is left evenly.
+    // (cnt_above of them, with the mass `above`), those behind are not.  Level 0 has all entries in bins of 1/64
+    // octave of e; the others divide what is left evenly.
     uint32_t ul = 0, uh = umax, span = umax, cand = 0, before = 0, cnt_above = 0, most = 0;
     uint32_t in[kCl];  // candidates of each CTA
     u64 above = 0, thr = ~0ull;
@@ -408,8 +414,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       __syncthreads();
       const int lo = s.lo, hi = s.hi;
       if (lo_mine == lo && lo < kBins) s.cnt_before = before_lo;  // (one thread)
-      // Bins ascend with u: the first u of a bin or a later one, by a search of 32 parts a step (the same in every warp),
-      // so that the entries need no bins again.
+      // Bins ascend with u: the first u of a bin or a later one, by a search of 32 parts a step (the same in every
+      // warp), so that the entries need no bins again.
       auto first_of = [&](int bin) -> uint32_t {
         uint32_t at = ul, left = uh - ul + 1;  // the first is in [at, at + left]
         while (left > 0) {
@@ -425,7 +431,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       const float dtop = -__uint_as_float(ul);
       // before the cut's bins: dtop >= d > dlo (and d >= dlow); in them: dlo >= d >= dhi
       const float dlo = -__uint_as_float(ulo), dhi = uhi > ul ? fmaxf(dlow, -__uint_as_float(uhi - 1)) : INFINITY;
-      // the masses of entries before the cut's bins (gathered, so that every lane has one to evaluate), and the candidates
+      // the masses of entries before the cut's bins (gathered, so that every lane has one to evaluate), and the
+      // candidates
       uint32_t waiting = 0, least = 0xffffffffu, largest = 0;
       float* few = s.few[warp];
       auto add_up = [&](uint32_t count) {
@@ -585,8 +592,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     }
     seg_mass = warp_sum(seg_mass);
     if (!struck && cand > 0) {
-      // The candidates' key range in kSub parts, with exact counts and masses: the cut falls into one part, and only its
-      // members are ranked one against the other.
+      // The candidates' key range in kSub parts, with exact counts and masses: the cut falls into one part, and only
+      // its members are ranked one against the other.
       for (int i = tid; i < kSub; i += kThr) {
         s.sub_mass[i] = Split{0, 0};
         s.sub_cnt[i] = 0;

@@ -221,7 +221,6 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   cluster.barrier_arrive();
   // (the row's settings, while the maxima arrive)
   const double c = 1.4426950408889634 / (double)T;  // y = c d: e = 2^y
-  const float cf = (float)c;
   const bool need_k = k_in > 0 && (uint32_t)k_in < a.V, need_p = p_in < 1.0f;
   const uint32_t k = need_k ? (uint32_t)k_in : 0xffffffffu;
   // entries below dcut have no mass (y < -45: it rounds to zero); entries below dlow are not allowed: dcut, or the
@@ -346,7 +345,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       auto edge = [&](int bin) {  // e at a bin's upper edge, in units of 2^-44
         if (kFirst) return exp2f((float)kFrac - ((float)bin - 0.5f) * (1.0f / kBinsOct));
         const float step = ((float)(uh - ul) + 1.0f) * (1.0f / kBins);
-        return exp2f((float)kFrac - __uint_as_float(min(uh, ul + (uint32_t)((float)bin * step) + (bin > 0))) * cf);
+        // (in double: a tiny temperature's c is no float)
+        return exp2f((float)(kFrac - (double)__uint_as_float(min(uh, ul + (uint32_t)((float)bin * step) + (bin > 0))) * c));
       };
       uint32_t n[kPer];
       float up[kPer], down[kPer];

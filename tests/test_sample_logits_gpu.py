@@ -119,6 +119,17 @@ def test_masks_infinities_and_nan(ctx, sample):
         assert tok[:2].tolist() == [-1, -1]
 
 
+def test_denormal_logits_at_a_denormal_temperature(ctx, sample):
+    """Differences below 2^-126 with weights of every size, and more of them than a row ranks at once."""
+    g = torch.Generator().manual_seed(3)
+    steps = torch.randint(0, 4000, (3, 9000), generator=g)
+    steps[:, :3000] %= 5  # thousands of equal ones near the top
+    logits = (-steps.double() * 2.0**-149).float().cuda()
+    for kw in (dict(temp=1e-42), dict(temp=1e-42, top_p=0.5), dict(temp=1e-42, top_p=0.9, top_k=4000), dict(temp=1e-43, top_p=0.99),
+               dict(temp=1e-42, min_p=0.5, top_k=1500)):
+        check(ctx, sample, logits, uniforms(3, 8), **kw)
+
+
 def test_zeros_of_both_signs_are_one_value(ctx, sample):
     logits = torch.zeros(2, 100, device="cuda")
     logits[:, ::2] = -0.0

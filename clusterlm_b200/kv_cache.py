@@ -79,6 +79,14 @@ def _rows(ctx: Context, name: str, t: torch.Tensor, heads, head_dim: int):
     return p, n, positions, h, ld
 
 
+def _result(ctx: Context, out, dtype, like: torch.Tensor, shape):
+    """The caller's output tensor, or a new one, and its address."""
+    if out is not None:
+        return out, _operand(ctx, "out", out, dtype, shape)
+    out = torch.empty_like(like) if like.dtype is dtype and like.is_contiguous() else like.new_empty(shape, dtype=dtype)
+    return out, out.data_ptr()
+
+
 def _parents(ctx: Context, parents, positions: int):
     return None if parents is None else _operand(ctx, "parents", parents, torch.int32, (positions,))
 
@@ -129,9 +137,7 @@ def kv_append(ctx: Context, k_pool, v_pool, tables, pos, q, k, v, rope: Rope | N
         qp, qn, qpos, heads, ldq = _rows(ctx, "q", q, None, hd)
         if (qn, qpos) != (n, positions) or q.dtype != k.dtype:
             raise ValueError("q: expected the rows and type of k")
-        if out is None:
-            out = torch.empty((n, positions, heads, hd), dtype=k_pool.dtype, device=k_pool.device)
-        op = _operand(ctx, "out", out, k_pool.dtype, (n, positions, heads, hd))
+        out, op = _result(ctx, out, k_pool.dtype, q, (n, positions, heads, hd))
     r = rope._c(ctx) if rope is not None else None
     check(lib.clm_b200_kv_append(ctx.h, C.byref(pool), 0, C.byref(seqs), n, positions, heads, DTYPES[k.dtype], qp, ldq, kp,
                                  ldk, vp, ldv, None if r is None else C.byref(r), _parents(ctx, parents, positions), op,
@@ -157,9 +163,7 @@ def kv_attention(ctx: Context, k_pool, v_pool, tables, pos, q, groups=None, scal
             if not (0 <= c < 2**32 and 0 <= p < 2**32):
                 raise ValueError("groups: expected (sequences, pages) of zero or more")
         counts, pages = (C.c_uint32 * g)(*[c for c, _ in groups]), (C.c_uint32 * g)(*[p for _, p in groups])
-    if out is None:
-        out = torch.empty((n, positions, heads, hd), dtype=q.dtype, device=q.device)
-    op = _operand(ctx, "out", out, q.dtype, (n, positions, heads, hd))
+    out, op = _result(ctx, out, q.dtype, q, (n, positions, heads, hd))
     need = C.c_uint64()
     check(lib.clm_b200_kv_attention_workspace(ctx.h, n, positions, heads, pool.n_kv_heads, hd, g, counts, pages,
                                               C.byref(need)))

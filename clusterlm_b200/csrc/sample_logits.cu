@@ -46,6 +46,7 @@ constexpr int kBins = 44 * kBinsOct;
 constexpr int kOwn = kBins / kCl;  // bins whose row totals a CTA forms
 constexpr int kCand = 1024;        // candidates of a row that are ranked are fewer
 constexpr int kMine = 384;         // of one CTA
+constexpr int kFew = 192;          // entries that a warp puts aside
 constexpr int kSub = 64;           // parts of the candidates' key range
 constexpr int kFrac = 44;          // fraction bits of a mass
 constexpr uint32_t kMaxVocab = 8 * 48128;  // a slice and the tables fit in 227 KB
@@ -125,7 +126,8 @@ struct Shared {
   Split sub_mass[kSub], seg_add[kWrp];
   uint32_t cand_n, cut_n;
   double table[64];     // 2^(j / 64)
-  float few[kWrp][192];  // entries whose masses a warp has yet to sum
+  float few[kWrp][kFew];  // entries whose masses a warp has yet to sum
+  uint32_t few_n[kWrp];
   int lo, hi;
   uint32_t cnt_before;
 };
@@ -414,9 +416,16 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       __syncthreads();
       const int lo = s.lo, hi = s.hi;
       if (lo_mine == lo && lo < kBins) s.cnt_before = before_lo;  // (one thread)
-      // Bins ascend with u: the first u of a bin or a later one, by a search of 32 parts a step (the same in every
-      // warp), so that the entries need no bins again.
+      // Bins ascend with u: the first u of a bin or a later one, so that the entries need no bins again.  Of level 0 it lies
+      // at the bin's edge but for a few units, which the lanes try; else (and for bins past the last one) by a search of
+      // 32 parts a step.  (The same in every warp.)
       auto first_of = [&](int bin) -> uint32_t {
+        if (kFirst && bin < kBins) {
+          if (bin <= 0) return ul;
+          const uint32_t from = max(__float_as_uint((float)(((double)bin - 0.5) / (kBinsOct * c))), 16u) - 16u;
+          const uint32_t under = __ballot_sync(0xffffffffu, bin_of(-__uint_as_float(from + lane)) < bin);
+          if ((under & 1u) && !(under >> 31)) return from + __popc(under);
+        }
         uint32_t at = ul, left = uh - ul + 1;  // the first is in [at, at + left]
         while (left > 0) {
           const uint32_t step = (left + 31) / 32, probe = at + min(left, (lane + 1) * step) - 1;
@@ -431,64 +440,50 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       const float dtop = -__uint_as_float(ul);
       // before the cut's bins: dtop >= d > dlo (and d >= dlow); in them: dlo >= d >= dhi
       const float dlo = -__uint_as_float(ulo), dhi = uhi > ul ? fmaxf(dlow, -__uint_as_float(uhi - 1)) : INFINITY;
-      // the masses of entries before the cut's bins (gathered, so that every lane has one to evaluate), and the
+      // the masses of entries before the cut's bins (put aside, so that every lane has one to evaluate), and the
       // candidates
-      uint32_t waiting = 0, least = 0xffffffffu, largest = 0;
+      uint32_t least = 0xffffffffu, largest = 0;
       float* few = s.few[warp];
-      auto add_up = [&](uint32_t count) {
-        waiting -= count;
-        __syncwarp();
-        const bool one = lane < count, two = lane + 32 < count;
-        const u64 w0 = mass(one ? few[waiting + lane] : 0.0f), w1 = mass(two ? few[waiting + lane + 32] : 0.0f);
-        seg_mass += (one ? w0 : 0ull) + (two ? w1 : 0ull);
-        __syncwarp();
-      };
-      for (uint32_t i0 = s0; i0 < s1; i0 += 128) {
+      if (lane == 0) s.few_n[warp] = 0;
+      __syncwarp();
+      bool full = false;
+      for (uint32_t i0 = s0; i0 < s1; i0 += 256) {
         const uint32_t i = i0 + 4 * lane;
-        const float4 x = i < s1 ? *reinterpret_cast<const float4*>(key + i)
-                                : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        const float d[4] = {d_of(x.x), d_of(x.y), d_of(x.z), d_of(x.w)};
-        bool in_cut[4], some = false, any = false;
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool in = d[j] >= dhi && d[j] <= dtop;
-          any |= in;
-          in_cut[j] = in && d[j] <= dlo;
-          some |= in_cut[j];
+        for (int h = 0; h < 2; ++h) {
+          const float4 v = i + 128 * h < s1 ? *reinterpret_cast<const float4*>(key + i + 128 * h)
+                                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
         }
-        if (!__any_sync(0xffffffffu, any)) continue;
-        uint32_t early[4];
+        if (d_of(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])))) < dhi) continue;
+        uint32_t counts = 0;  // a bit per entry
 #pragma unroll
-        for (int j = 0; j < 4; ++j) early[j] = __ballot_sync(0xffffffffu, d[j] > dlo && d[j] >= dhi && d[j] <= dtop);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (early[j] >> lane & 1u) few[waiting + __popc(early[j] & ((1u << lane) - 1u))] = d[j];
-          waiting += __popc(early[j]);
-        }
-        while (waiting >= 64) add_up(64);
-        if (__any_sync(0xffffffffu, some)) {
-          uint32_t mates[4], at = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mates[j] = __ballot_sync(0xffffffffu, in_cut[j]);
-            at += __popc(mates[j]);
-          }
-          if (lane == 0) at = atomicAdd(&s.cand_n, at);
-          at = __shfl_sync(0xffffffffu, at, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (in_cut[j]) {
-              const uint32_t u = u_of(d[j]), to = at + __popc(mates[j] & ((1u << lane) - 1u));
-              least = min(least, u);
-              largest = max(largest, u);
-              // (in the place of the histograms, which every CTA has read; its mass follows)
-              if (to < kMine) mine[to] = Cand{u, v0 + i + j, 0ull};
+        for (int j = 0; j < 8; ++j)
+          if (d_of(x[j]) >= dhi && (kFirst || d_of(x[j]) <= dtop)) counts |= 1u << j;
+        for (; counts; counts &= counts - 1) {
+          const int j = __ffs(counts) - 1;
+          const uint32_t e = i + 128 * (j / 4) + j % 4;
+          const float d = d_of(key[e]);
+          if (d > dlo) {
+            const uint32_t at = full ? kFew : atomicAdd(&s.few_n[warp], 1u);
+            if (at < kFew) {
+              few[at] = d;
+            } else {  // a dense row: most lanes have some
+              full = true;
+              seg_mass += mass(d);
             }
-            at += __popc(mates[j]);
+          } else {
+            const uint32_t u = u_of(d), at = atomicAdd(&s.cand_n, 1u);
+            least = min(least, u);
+            largest = max(largest, u);
+            // (in the place of the histograms, which every CTA has read; its mass follows)
+            if (at < kMine) mine[at] = Cand{u, v0 + e, 0ull};
           }
         }
       }
-      if (waiting) add_up(waiting);
+      __syncwarp();
+      for (uint32_t i = lane; i < min(s.few_n[warp], (uint32_t)kFew); i += 32) seg_mass += mass(few[i]);
       const u64 level_mass = warp_sum(seg_mass);  // with the levels before
       const u64 x = cta_sum(level_mass, s.seg, warp, lane);
       for (uint32_t i = tid; i < min(s.cand_n, (uint32_t)kMine); i += kThr) mine[i].w = mass(-__uint_as_float(mine[i].u));

@@ -46,7 +46,6 @@ constexpr int kBins = 44 * kBinsOct;
 constexpr int kOwn = kBins / kCl;  // bins whose row totals a CTA forms
 constexpr int kCand = 1024;        // candidates of a row that are ranked are fewer
 constexpr int kMine = 384;         // of one CTA
-constexpr int kFew = 192;          // entries that a warp puts aside
 constexpr int kSub = 64;           // parts of the candidates' key range
 constexpr int kFrac = 44;          // fraction bits of a mass
 constexpr uint32_t kMaxVocab = 8 * 48128;  // a slice and the tables fit in 227 KB
@@ -126,8 +125,6 @@ struct Shared {
   Split sub_mass[kSub], seg_add[kWrp];
   uint32_t cand_n, cut_n;
   double table[64];     // 2^(j / 64)
-  float few[kWrp][kFew];  // entries whose masses a warp has yet to sum
-  uint32_t few_n[kWrp];
   int lo, hi;
   uint32_t cnt_before;
 };
@@ -440,13 +437,9 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       const float dtop = -__uint_as_float(ul);
       // before the cut's bins: dtop >= d > dlo (and d >= dlow); in them: dlo >= d >= dhi
       const float dlo = -__uint_as_float(ulo), dhi = uhi > ul ? fmaxf(dlow, -__uint_as_float(uhi - 1)) : INFINITY;
-      // the masses of entries before the cut's bins (put aside, so that every lane has one to evaluate), and the
+      // the masses of entries before the cut's bins and the
       // candidates
       uint32_t least = 0xffffffffu, largest = 0;
-      float* few = s.few[warp];
-      if (lane == 0) s.few_n[warp] = 0;
-      __syncwarp();
-      bool full = false;
       for (uint32_t i0 = s0; i0 < s1; i0 += 256) {
         const uint32_t i = i0 + 4 * lane;
         float x[8];
@@ -466,13 +459,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           const uint32_t e = i + 128 * (j / 4) + j % 4;
           const float d = d_of(key[e]);
           if (d > dlo) {
-            const uint32_t at = full ? kFew : atomicAdd(&s.few_n[warp], 1u);
-            if (at < kFew) {
-              few[at] = d;
-            } else {  // a dense row: most lanes have some
-              full = true;
-              seg_mass += mass(d);
-            }
+            seg_mass += mass(d);
           } else {
             const uint32_t u = u_of(d), at = atomicAdd(&s.cand_n, 1u);
             least = min(least, u);
@@ -482,8 +469,6 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
           }
         }
       }
-      __syncwarp();
-      for (uint32_t i = lane; i < min(s.few_n[warp], (uint32_t)kFew); i += 32) seg_mass += mass(few[i]);
       const u64 level_mass = warp_sum(seg_mass);  // with the levels before
       const u64 x = cta_sum(level_mass, s.seg, warp, lane);
       for (uint32_t i = tid; i < min(s.cand_n, (uint32_t)kMine); i += kThr) mine[i].w = mass(-__uint_as_float(mine[i].u));

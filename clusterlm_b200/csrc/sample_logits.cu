@@ -440,23 +440,32 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       // the masses of entries before the cut's bins and the
       // candidates
       uint32_t least = 0xffffffffu, largest = 0;
-      for (uint32_t i0 = s0; i0 < s1; i0 += 256) {
-        const uint32_t i = i0 + 4 * lane;
-        float x[8];
+      // first which entries of up to 2,048 (a bit for each of a lane's 64), then one after the other: lanes have unlike
+      // numbers of them, which even out over many
+      for (uint32_t c0 = s0; c0 < s1; c0 += 2048) {
+        u64 counts = 0;
+        const uint32_t c1 = min(s1, c0 + 2048);
+#pragma unroll 1
+        for (uint32_t k = 0; c0 + 256 * k < c1; ++k) {
+          const uint32_t i = c0 + 256 * k + 4 * lane;
+          float x[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 v = i + 128 * h < s1 ? *reinterpret_cast<const float4*>(key + i + 128 * h)
-                                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-          x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
+          for (int h = 0; h < 2; ++h) {
+            const float4 v = i + 128 * h < c1 ? *reinterpret_cast<const float4*>(key + i + 128 * h)
+                                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
+          }
+          if (d_of(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])))) < dhi)
+            continue;
+          uint32_t bits = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (d_of(x[j]) >= dhi && (kFirst || d_of(x[j]) <= dtop)) bits |= 1u << j;
+          counts |= (u64)bits << (8 * k);
         }
-        if (d_of(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])))) < dhi) continue;
-        uint32_t counts = 0;  // a bit per entry
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (d_of(x[j]) >= dhi && (kFirst || d_of(x[j]) <= dtop)) counts |= 1u << j;
         for (; counts; counts &= counts - 1) {
-          const int j = __ffs(counts) - 1;
-          const uint32_t e = i + 128 * (j / 4) + j % 4;
+          const int j = __ffsll((long long)counts) - 1;
+          const uint32_t e = c0 + 128 * (j / 4) + 4 * lane + j % 4;
           const float d = d_of(key[e]);
           if (d > dlo) {
             seg_mass += mass(d);

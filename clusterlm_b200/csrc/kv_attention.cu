@@ -18,8 +18,8 @@
 //
 // GPU time of a call (fp16, head_dim 128, 32 heads over 8 unless said): 4 sequences of about 1,000 positions 13 us; 8
 // tree windows of 16 rows over 4,096 shared positions 34 us; 64 windows of 4 rows, 16,384 shared and about 500 own
-// positions each, 140 us (tile kernel 83 us, 0.83 PFLOP/s; stream kernel 36 us, 3.7 TB/s; combining kernel 13 us);
-// 256 rows over 8,192 positions (bf16) 105 us (0.72 PFLOP/s in the tile kernel); 64 sequences of 2,048 positions, 8
+// positions each, 138 us (tile kernel 83 us, 0.83 PFLOP/s; stream kernel 36 us, 3.7 TB/s; combining kernel 10 us);
+// 256 rows over 8,192 positions (bf16) 101 us (0.72 PFLOP/s in the tile kernel); 64 sequences of 2,048 positions, 8
 // rows a kv head, 94 us (5.7 TB/s).
 #include <algorithm>
 #include <cfloat>
@@ -1197,36 +1197,32 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
   if (second) griddep_wait();
 }
 
-// One warp per (row, head): the row's partials of its group's item (found by lanes 0..15) and of its own (lanes
-// 16..31, or all where it has no group), combined by their maxima.  A lane looks up a partial and its maximum and
-// sum; then the lanes share the outputs' columns.  Bound by three dependent reads (plan; maxima, with the first four
-// partials; the others): 8,192 rows of 128 with six partials each 13 us, 25 MB.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constant__ Args a) {
+// One warp per row and HP heads of a kv head (whose rows lie together in a segment): their partials of the group's item
+// (found by lanes 0..15) and of the sequence's own (lanes 16..31, or all where it has no group), combined by their maxima.
+// A lane looks up a partial and its maxima and sums; then the lanes share the outputs' columns.  Bound by the look-up's
+// instructions and three dependent reads (plan; maxima, with the first partials; the others).
+template <typename T, int HD, int HP>
+__global__ void __launch_bounds__(256, HP == 1 ? 4 : 2) kv_combine_kernel(const __grid_constant__ Args a) {
   using TL = Tile<HD>;
   constexpr int N = HD / 32;  // outputs per lane
+  constexpr int B = HP == 4 ? 2 : 4;  // partials whose loads are in flight
   const int lane = threadIdx.x % 32;
-  const uint32_t id = blockIdx.x * 8 + threadIdx.x / 32;
-  if (id >= (uint32_t)(a.seqs.n * a.positions) * a.nh) return;
-  const int head = (int)(id % a.nh), row = (int)(id / a.nh);
+  const uint32_t id = blockIdx.x * 8 + threadIdx.x / 32, blocks = a.nh / HP;
+  if (id >= (uint32_t)(a.seqs.n * a.positions) * blocks) return;
+  const int head = (int)(id % blocks) * HP, row = (int)(id / blocks);
   const int b = row / a.positions, kvh = head / a.group;
   const int its_group = group_of(a, b), width = its_group < 0 ? 32 : 16;  // lanes of a kind
-  const int k = lane / width + width / 32;  // kind
+  const int k = lane / width + width / 32;                                // kind
   const int e = k == 0 ? its_group : a.groups.n + b;
   const Args::Kind& kind = a.kind[k];
-  // the item of the row, and its row in a segment
-  Entry en;
-  int tile = 0, r = 0;
-  bool pair = false;
-  {
-    en = entry_of(a, e);
-    const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
-    tile = kind.tile ? kvh * en.tiles + x / kRowTile : kvh;
-    r = kind.tile ? x % 128 : x;
-    // in a tile of more than 128 rows a row has one partial a segment, that of its stream; else one of each stream
-    pair = kind.tile && min(en.rows - x / kRowTile * kRowTile, kRowTile) > 128;
-    if (pair) r += x % kRowTile / 128 * kind.rows;
-  }
+  // the item of the rows, and the first one's place in a segment
+  const Entry en = entry_of(a, e);
+  const int x = (row - en.s0 * a.positions) * a.group + head % a.group;
+  const int tile = kind.tile ? kvh * en.tiles + x / kRowTile : kvh;
+  int r = kind.tile ? x % 128 : x;
+  // in a tile of more than 128 rows a row has one partial a segment, that of its stream; else one of each stream
+  const bool pair = kind.tile && min(en.rows - x / kRowTile * kRowTile, kRowTile) > 128;
+  if (pair) r += x % kRowTile / 128 * kind.rows;
   const uint32_t per = kind.tile && !pair ? 2 : 1, seg_rows = kind.tile ? 2 * kind.rows : kind.rows;
   const uint32_t item = items_before(a, e) + tile;
   griddep_wait();
@@ -1244,13 +1240,18 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
     }
   }
   const uint32_t rounds = __reduce_max_sync(0xffffffffu, (n + width - 1) / width);
-  float M = -INFINITY, l = 0.0f, acc[N];
+  float M[HP], l[HP], acc[HP][N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+  for (int h = 0; h < HP; ++h) {
+    M[h] = -INFINITY;
+    l[h] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[h][i] = 0.0f;
+  }
   for (uint32_t round = 0; round < rounds; ++round) {
     const uint32_t i = width * round + lane % width;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    uint32_t src = 0;  // the partial's row
+    float2 ml[HP];
+    uint32_t src = 0;  // the partials' first row
     bool have = false;
     if (i < n) {
       const uint32_t c = c0 + i / per, s = i % per;
@@ -1259,65 +1260,81 @@ __global__ void __launch_bounds__(256, 4) kv_combine_kernel(const __grid_constan
       const uint32_t w0 = max(shares.begin(c), u0) - u0, w1 = min(units, shares.begin(c + 1) - u0);
       have = pages_before(en, w1) - pages_before(en, w0) > s;
       src = (item + c) * seg_rows + s * kind.rows + r;
-      if (have) ml = *reinterpret_cast<const float2*>(kind.part + (size_t)src * TL::kRow + HD);
     }
-    // four partials' loads at a time in flight, the first ones before the maxima are here
+#pragma unroll
+    for (int h = 0; h < HP; ++h)
+      ml[h] = have ? *reinterpret_cast<const float2*>(kind.part + (size_t)(src + h) * TL::kRow + HD)
+                   : make_float2(-INFINITY, 0.0f);
+    // the first partials' loads start before the maxima are here
     uint32_t todo = __ballot_sync(0xffffffffu, have);
-    float o[4][N];
-    int from[4];
+    float o[B][HP][N];
+    int from[B];
     auto load = [&]() {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < B; ++q) {
         from[q] = todo ? __ffs(todo) - 1 : -1;
         const float* p = (width == 16 && from[q] < 16 ? a.kind[0].part : a.kind[1].part) +
-                         (size_t)__shfl_sync(0xffffffffu, src, from[q] & 31) * TL::kRow;
-        if (todo) {
-          if constexpr (N == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + 4 * lane);
-            o[q][0] = v.x, o[q][1] = v.y, o[q][2] = v.z, o[q][3] = v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(p + 2 * lane);
-            o[q][0] = v.x, o[q][1] = v.y;
-          }
-        } else {
+                         (size_t)__shfl_sync(0xffffffffu, src, from[q] & 31) * TL::kRow + N * lane;
 #pragma unroll
-          for (int j = 0; j < N; ++j) o[q][j] = 0.0f;
+        for (int h = 0; h < HP; ++h) {
+          if (todo) {
+            if constexpr (N == 4) {
+              const float4 v = *reinterpret_cast<const float4*>(p + h * TL::kRow);
+              o[q][h][0] = v.x, o[q][h][1] = v.y, o[q][h][2] = v.z, o[q][h][3] = v.w;
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(p + h * TL::kRow);
+              o[q][h][0] = v.x, o[q][h][1] = v.y;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[q][h][j] = 0.0f;
+          }
         }
         todo &= todo - 1;
       }
     };
     load();
-    float m = fmaxf(M, ml.x);
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const float keep = ex2(M - ref), f = ex2(ml.x - ref);
-    float add = ml.y * f;
-    for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-    M = m;
-    l = l * keep + add;
+    float f[HP];
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] *= keep;
+    for (int h = 0; h < HP; ++h) {
+      float m = fmaxf(M[h], ml[h].x);
+      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const float keep = ex2(M[h] - ref);
+      f[h] = ex2(ml[h].x - ref);
+      float add = ml[h].y * f[h];
+      for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+      M[h] = m;
+      l[h] = l[h] * keep + add;
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[h][j] *= keep;
+    }
     for (;;) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float w = __shfl_sync(0xffffffffu, f, from[q] & 31);
+      for (int q = 0; q < B; ++q)
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += o[q][j] * (from[q] < 0 ? 0.0f : w);
-      }
+        for (int h = 0; h < HP; ++h) {
+          const float w = __shfl_sync(0xffffffffu, f[h], from[q] & 31);
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[h][j] += o[q][h][j] * (from[q] < 0 ? 0.0f : w);
+        }
       if (todo == 0) break;
       load();
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) + ((size_t)row * a.nh + head) * HD + N * lane;
-  if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = acc[i] * inv;
-  } else if constexpr (N == 4) {
-    *reinterpret_cast<uint2*>(out) =
-        make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
-  } else {
-    *reinterpret_cast<uint32_t*>(out) = pack2<T>(acc[0] * inv, acc[1] * inv);
+  for (int h = 0; h < HP; ++h) {
+    const float inv = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
+    T* out = static_cast<T*>(a.out) + ((size_t)row * a.nh + head + h) * HD + N * lane;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) out[i] = acc[h][i] * inv;
+    } else if constexpr (N == 4) {
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack2<T>(acc[h][0] * inv, acc[h][1] * inv), pack2<T>(acc[h][2] * inv, acc[h][3] * inv));
+    } else {
+      *reinterpret_cast<uint32_t*>(out) = pack2<T>(acc[h][0] * inv, acc[h][1] * inv);
+    }
   }
 }
 
@@ -1375,7 +1392,15 @@ int launch_typed(const Args& a, const Layout& s, int sm_count, cudaStream_t st) 
   if (!s.tile[0] || !s.tile[1])
     CLM_TRY(launch_pdl(kv_stream_kernel<T, HD>, dim3((unsigned)sm_count), dim3(32 * kStreamWarps), 0, st, a, (int)tiled));
   const uint64_t rows = (uint64_t)a.seqs.n * a.positions * a.nh;
-  return launch_pdl(kv_combine_kernel<O, HD>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, a);
+  auto combine = [&](auto kernel, int heads) {
+    return launch_pdl(kernel, dim3((unsigned)ceil_div(rows / heads, 8)), dim3(256), 0, st, a);
+  };
+  // Several heads a warp where one each would be more than the GPU holds at once: the look-up is done once for them (8,192
+  // rows and heads of 128 with six partials each: 13 -> 9 us; but 1,024 of 64 with twenty: 10 -> 16).
+  const bool many = rows > 32ull * sm_count;
+  if (many && a.group % 4 == 0) return combine(kv_combine_kernel<O, HD, 4>, 4);
+  if (many && a.group % 2 == 0) return combine(kv_combine_kernel<O, HD, 2>, 2);
+  return combine(kv_combine_kernel<O, HD, 1>, 1);
 }
 
 }  // namespace

@@ -15,6 +15,7 @@ sequence state is private to a domain (runtime/domain/src/reference_domain.cpp:2
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 import torch
@@ -175,39 +176,47 @@ def kv_attention(ctx: Context, k_pool, v_pool, tables, pos, q, groups=None, scal
     return out
 
 
-def _ints(name: str, a, dtype) -> np.ndarray:
+def _ints(name: str, a, dtype):
+    """(address, entries, their owner) of integers: a list, or an array that is copied unless it has the type."""
+    if isinstance(a, (list, tuple, range)):
+        try:
+            a = array("I" if dtype is np.uint32 else "i", a)
+            return a.buffer_info()[0], len(a), a
+        except (TypeError, OverflowError):
+            pass  # (said below)
     a = np.asarray(a)
     if a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:
-        return a
+        return a.ctypes.data, a.size, a
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise ValueError(f"{name}: expected a list of integers")
     lim = np.iinfo(dtype)
     if a.size and (int(a.min()) < lim.min or int(a.max()) > lim.max):
         raise ValueError(f"{name}: an entry is out of range")
-    return np.ascontiguousarray(a, dtype=dtype)
+    a = np.ascontiguousarray(a, dtype=dtype)
+    return a.ctypes.data, a.size, a
 
 
 def kv_fork(ctx: Context, k_pools, v_pools, tables, pos, parents, children, new_pages) -> None:
     """Row children[i] of the tables becomes a continuation of row parents[i]: the full pages shared, the last page
     copied into new_pages[i] in every layer (pools with a leading layers dim), the position taken over."""
     pool, seqs = _pool(ctx, k_pools, v_pools, True), _seqs(ctx, tables, pos)
-    p, c, g = _ints("parents", parents, np.uint32), _ints("children", children, np.uint32), _ints("new_pages", new_pages, np.int32)
-    if not p.size == c.size == g.size:
+    (p, n, _p), (c, nc, _c), (g, ng, _g) = (_ints("parents", parents, np.uint32), _ints("children", children, np.uint32),
+                                            _ints("new_pages", new_pages, np.int32))
+    if not n == nc == ng:
         raise ValueError("parents, children and new_pages: expected one entry per fork")
-    check(lib.clm_b200_kv_fork(ctx.h, C.byref(pool), C.byref(seqs), p.size, p.ctypes.data, c.ctypes.data, g.ctypes.data,
-                               _stream_on(ctx.device)))
+    check(lib.clm_b200_kv_fork(ctx.h, C.byref(pool), C.byref(seqs), n, p, c, g, _stream_on(ctx.device)))
 
 
 def kv_copy_pages(ctx: Context, k_pools, v_pools, src, dst, tables=None) -> None:
     """Copies page src[i] to dst[i] in every layer (pools with a leading layers dim); with tables, entries that name
     src[i] then name dst[i]."""
     pool = _pool(ctx, k_pools, v_pools, True)
-    s, d = _ints("src", src, np.int32), _ints("dst", dst, np.int32)
-    if s.size != d.size:
+    (s, n, _s), (d, nd, _d) = _ints("src", src, np.int32), _ints("dst", dst, np.int32)
+    if n != nd:
         raise ValueError("src and dst: expected one entry per page")
     tp = None if tables is None else _operand(ctx, "tables", tables, torch.int32)
-    check(lib.clm_b200_kv_copy_pages(ctx.h, C.byref(pool), s.size, s.ctypes.data, d.ctypes.data, tp,
-                                     0 if tables is None else tables.numel(), _stream_on(ctx.device)))
+    check(lib.clm_b200_kv_copy_pages(ctx.h, C.byref(pool), n, s, d, tp, 0 if tables is None else tables.numel(),
+                                     _stream_on(ctx.device)))
 
 
 class Pages:
@@ -237,12 +246,12 @@ class Pages:
         return ids.tolist()
 
     def retain(self, ids) -> None:
-        a = _ints("ids", ids, np.int32)
-        call("clm_b200_pages_retain", self.h, a.size, a.ctypes.data_as(_vp))
+        a, n, _a = _ints("ids", ids, np.int32)
+        call("clm_b200_pages_retain", self.h, n, a)
 
     def release(self, ids) -> None:
-        a = _ints("ids", ids, np.int32)
-        call("clm_b200_pages_release", self.h, a.size, a.ctypes.data_as(_vp))
+        a, n, _a = _ints("ids", ids, np.int32)
+        call("clm_b200_pages_release", self.h, n, a)
 
     def holders(self, page: int) -> int:
         r = C.c_uint32()

@@ -21,10 +21,10 @@
 //      is left, its lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
 //
-// Bound by instructions, and by the cluster's barriers where there are few rows: 1 row of 128,256 17 us (30,000
-// clocks, of which eight barriers and what waits for them take 15,000); 64 of 151,936 with top-p 77 us (two rows'
-// slices on an SM at a time: 1.7 waves of 58,000 clocks, half the issue slots used); 256 of 128,256 with mixed
-// settings 170 us.  A row on sixteen CTAs takes as long alone, and 138 and 317 us in those batches.
+// Bound by instructions, and by the cluster's barriers where there are few rows: 1 row of 128,256 16 us (27,000
+// clocks, of which eight barriers and what waits for them take half); 64 of 151,936 with top-p 69 us (two rows' slices on
+// an SM at a time: two waves of 52,000 clocks, half the issue slots used); 256 of 128,256 with mixed settings 158 us.
+// On sixteen CTAs a row was 10% faster alone and 1.7 times slower in those batches.
 #include <cooperative_groups.h>
 
 #include <cfloat>

@@ -530,6 +530,11 @@ int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t
             CLM_INVALID_ARGUMENT, "a row stride is smaller than a row");
   CLM_CHECK(!d_q || (reinterpret_cast<uintptr_t>(d_q_out) & 15) == 0, CLM_INVALID_ARGUMENT,
             "the rotated queries must be 16-byte aligned");
+  if (d_q) {  // rotated pairs are read by several threads
+    const uint64_t rows = (uint64_t)n * positions, q = reinterpret_cast<uintptr_t>(d_q), o = reinterpret_cast<uintptr_t>(d_q_out);
+    CLM_CHECK(o >= q + ((rows - 1) * ld_q + qd) * dtype_size(src_dtype) || q >= o + rows * qd * 2, CLM_INVALID_ARGUMENT,
+              "the rotated queries must not overlap the rows");
+  }
   AppendArgs a{};
   a.seqs = make_kv_seqs(pool, seqs, n);
   const uint64_t off = (uint64_t)layer * pool->pages * kv_page_bytes(pool);

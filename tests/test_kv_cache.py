@@ -184,6 +184,13 @@ def test_append_refuses(kw, code):
     assert append(**kw) == code
 
 
+@pytest.mark.parametrize("q,out,ld_q,src", [(A, A, 1024, 1), (A, A + 8192, 1024, 1), (A + 6128, A, 512, 1), (A, A + 22512, 1024, 0)])
+def test_append_refuses_to_rotate_in_place(q, out, ld_q, src):
+    """Six rows of 512 elements: the rows from q on (5 strides and a row), the result's 6,144 bytes."""
+    assert append(q=q, out=out, ld_q=ld_q, src=src) == INVALID
+    assert b"overlap" in _native.lib.clm_b200_last_error()
+
+
 def attention(ctx=CTX, p=None, layer=0, s=None, n=3, positions=2, heads=4, q=A, ld_q=512, groups=(), parents=0, out=A,
               work=A, work_bytes=1 << 40, null_groups=False, scale=0.1):
     p, s = pool() if p is None else p, seqs() if s is None else s

@@ -9,10 +9,10 @@
 // integers do not depend on their order, so a row's result is the same whatever computed it, every comparison is
 // exact on the w_i, and an entry below 2^-45 of the largest has no mass.
 //
-// A cluster of eight CTAs holds a row in shared memory (a slice each), so the logits are read from memory once however
-// many passes the row needs:
+// A cluster of eight CTAs (sixteen for few rows) holds a row in shared memory, a slice each, so the logits are read from
+// memory once however many passes the row needs:
 //   1. load, maximum (and its lowest index: greedy rows end here);
-//   2. without top-k / top-p: the masses of the CTAs' sixteen warp segments;
+//   2. without top-k / top-p: the masses of the CTAs' warp segments;
 //      with them: the row's whole mass and a histogram of the entries over 64 bins per octave of e, whose counts bound
 //      the cumulative mass within 1.1%: the cut falls into known bins.  Entries above these are allowed (their exact
 //      mass is summed), entries below are not, and the few in them are ranked: their key range in 64 parts with exact
@@ -21,10 +21,10 @@
 //      is left, its lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
 //
-// Bound by instructions, and by the cluster's barriers where there are few rows: 1 row of 128,256 16 us (27,000
-// clocks, of which eight barriers and what waits for them take half); 64 of 151,936 with top-p 69 us (two rows' slices on
-// an SM at a time: two waves of 52,000 clocks, half the issue slots used); 256 of 128,256 with mixed settings 158 us.
-// On sixteen CTAs a row was 10% faster alone and 1.7 times slower in those batches.
+// Bound by instructions, and by the cluster's barriers where there are few rows: 1 row of 128,256 15 us (27,000
+// clocks on eight CTAs, of which eight barriers and what waits for them take half); 64 of 151,936 with top-p 69 us (two
+// rows' slices on an SM at a time: two waves of 52,000 clocks, half the issue slots used); 256 of 128,256 with mixed
+// settings 158 us.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -38,12 +38,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kCl = 8;             // CTAs of a row
+constexpr int kCl = 8, kWide = 16;  // CTAs of a row; of few rows
 constexpr int kThr = 512;
 constexpr int kWrp = kThr / 32;    // warp segments of a CTA's slice
 constexpr int kBinsOct = 64;       // histogram bins per octave
 constexpr int kBins = 44 * kBinsOct;
-constexpr int kOwn = kBins / kCl;  // bins whose row totals a CTA forms
 constexpr int kCand = 1024;        // candidates of a row that are ranked are fewer
 constexpr int kMine = 384;         // of one CTA
 constexpr int kSub = 64;           // parts of the candidates' key range
@@ -110,13 +109,14 @@ __device__ __forceinline__ u64 warp_sum(u64 x) {
   return x;
 }
 
+template <int CL>  // CTAs of a row
 struct Shared {
-  u64 top[kCl];       // (ordered maximum, ~index) of each CTA's slice
-  u64 total[kCl];     // whole mass (pass 2)
-  u64 above[kCl];     // mass above the candidates
-  u64 kept[kCl];      // allowed mass
-  uint32_t ncand[kCl], umin[kCl], umax[kCl];  // candidates: how many, their key range
-  uint32_t ties[kCl];
+  u64 top[CL];       // (ordered maximum, ~index) of each CTA's slice
+  u64 total[CL];     // whole mass (pass 2)
+  u64 above[CL];     // mass above the candidates
+  u64 kept[CL];      // allowed mass
+  uint32_t ncand[CL], umin[CL], umax[CL];  // candidates: how many, their key range
+  uint32_t ties[CL];
   u64 seg[kWrp];      // allowed mass of the warp segments
   u64 red[kWrp];
   uint32_t redc[kWrp];
@@ -143,11 +143,11 @@ __device__ __forceinline__ uint32_t cta_sum(uint32_t warp_value, uint32_t* slots
   return __reduce_add_sync(0xffffffffu, lane < kWrp ? slots[lane] : 0u);
 }
 
-template <typename S>
-__global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
+template <typename S, int CL>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kThr, CL == kCl ? 2 : 1)
     sample_logits_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint8_t sl_smem[];
-  __shared__ Shared s;
+  __shared__ Shared<CL> s;
   cg::cluster_group cluster = cg::this_cluster();
   float* key = reinterpret_cast<float*>(sl_smem);  // [slice], padded with -inf
   uint32_t* hist = reinterpret_cast<uint32_t*>(key + a.slice);
@@ -157,11 +157,11 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   Cand* mine = all + kCand;
   static_assert(sizeof(Cand) * (kCand + kMine) <= 2 * kBins * sizeof(uint32_t), "the candidates fit over the histograms");
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const uint32_t rank = cluster.block_rank(), row = blockIdx.x / kCl;
+  const uint32_t rank = cluster.block_rank(), row = blockIdx.x / CL;
   const uint32_t v0 = min(a.V, rank * a.slice), cnt = min(a.V, v0 + a.slice) - v0;
   // a value of this CTA goes to every CTA of the row
   auto push = [&](auto* slot, auto value) {
-    if (tid < kCl) *cluster.map_shared_rank(slot + rank, tid) = value;
+    if (tid < CL) *cluster.map_shared_rank(slot + rank, tid) = value;
   };
   for (int i = tid; i < kBins; i += kThr) hist[i] = 0;
   if (tid < 64) s.table[tid] = exp2(tid / 64.0);
@@ -236,7 +236,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   cluster.barrier_wait();
   u64 best = 0;
 #pragma unroll
-  for (int r = 0; r < kCl; ++r) best = max(best, s.top[r]);
+  for (int r = 0; r < CL; ++r) best = max(best, s.top[r]);
   const float M = of_ord((uint32_t)(best >> 32));
   if (greedy || M == -INFINITY) {  // the same for the whole cluster
     if (rank == 0 && tid == 0) {
@@ -284,7 +284,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
     // (cnt_above of them, with the mass `above`), those behind are not.  Level 0 has all entries in bins of 1/64
     // octave of e; the others divide what is left evenly.
     uint32_t ul = 0, uh = umax, span = umax, cand = 0, before = 0, cnt_above = 0, most = 0;
-    uint32_t in[kCl];  // candidates of each CTA
+    uint32_t in[CL];  // candidates of each CTA
     u64 above = 0, thr = ~0ull;
     bool struck = false;
     auto look = [&](auto level0) {  // (two copies of the code: level 0 reads every entry)
@@ -312,15 +312,15 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       }
       push(s.total, cta_sum(warp_sum(sum), s.red, warp, lane));
       cluster.sync();
-      for (int b = tid; b < kOwn; b += kThr) {
-        const int bin = (int)rank * kOwn + b;
-        uint32_t part[kCl], n = 0;
+      for (int b = tid; b < (kBins / CL); b += kThr) {
+        const int bin = (int)rank * (kBins / CL) + b;
+        uint32_t part[CL], n = 0;
 #pragma unroll
-        for (int r = 0; r < kCl; ++r) part[r] = cluster.map_shared_rank(hist, r)[bin];
+        for (int r = 0; r < CL; ++r) part[r] = cluster.map_shared_rank(hist, r)[bin];
 #pragma unroll
-        for (int r = 0; r < kCl; ++r) n += part[r];
+        for (int r = 0; r < CL; ++r) n += part[r];
 #pragma unroll
-        for (int r = 0; r < kCl; ++r) cluster.map_shared_rank(tot, r)[bin] = n;
+        for (int r = 0; r < CL; ++r) cluster.map_shared_rank(tot, r)[bin] = n;
       }
       if (tid == 0) {
         s.lo = kBins;
@@ -332,7 +332,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         // allowed by top-p: entries with less than `thr` mass before them (p in units of 2^-40, rounded up)
         u64 total = 0;
 #pragma unroll
-        for (int r = 0; r < kCl; ++r) total += s.total[r];
+        for (int r = 0; r < CL; ++r) total += s.total[r];
         const u64 pi = (u64)ceil(fmax((double)p_in, 0.0) * 0x1p40);
         const u64 ph = __umul64hi(pi, total), pl = pi * total;
         thr = (ph << 24 | pl >> 40) + ((pl & 0xffffffffffull) != 0);
@@ -498,7 +498,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       cand = before = most = 0;
       uint32_t nl = 0xffffffffu, nh = 0;
 #pragma unroll
-      for (int r = 0; r < kCl; ++r) {
+      for (int r = 0; r < CL; ++r) {
         above += s.above[r];
         in[r] = s.ncand[r];
         if (r < (int)rank) before += in[r];
@@ -560,7 +560,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
         uint32_t count = 0;
         u64 sum = 0;
 #pragma unroll
-        for (int r = 0; r < kCl; ++r) {
+        for (int r = 0; r < CL; ++r) {
           count += s.ncand[r];
           sum += s.total[r];
         }
@@ -598,11 +598,11 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
       const bool direct = cand <= 64;  // few enough to be ranked at once
       {
         uint32_t at = 0;
-        const int from = warp % kCl;
+        const int from = warp % CL;
 #pragma unroll
-        for (int r = 0; r < kCl; ++r) at += r < from ? in[r] : 0u;
+        for (int r = 0; r < CL; ++r) at += r < from ? in[r] : 0u;
         const Cand* theirs = cluster.map_shared_rank(mine, from);
-        for (uint32_t i = warp / kCl * 32 + lane; i < s.ncand[from]; i += 32 * (kWrp / kCl)) {
+        for (uint32_t i = warp / CL * 32 + lane; i < s.ncand[from]; i += 32 * (kWrp / CL)) {
           const Cand x = theirs[i];
           all[at + i] = x;
           if (!direct) {
@@ -685,7 +685,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   cluster.sync();
   u64 W = 0;
 #pragma unroll
-  for (int r = 0; r < kCl; ++r) W += s.kept[r];
+  for (int r = 0; r < CL; ++r) W += s.kept[r];
   // floor(u W), exactly: u = m 2^-e with a 53-bit m
   const double u = a.u[row];
   u64 r = 0;
@@ -700,7 +700,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
   u64 base = 0;
   uint32_t owner = 0;
-  for (; owner + 1 < (uint32_t)kCl && base + s.kept[owner] <= r; ++owner) base += s.kept[owner];
+  for (; owner + 1 < (uint32_t)CL && base + s.kept[owner] <= r; ++owner) base += s.kept[owner];
   if (owner != rank) return;
   int ws = 0;
   for (; ws + 1 < kWrp && base + s.seg[ws] <= r; ++ws) base += s.seg[ws];
@@ -734,15 +734,49 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThr, 2)
   }
 }
 
+// Few rows: kWide CTAs each, if that many clusters run at once, one CTA on an SM.  (A cluster of more than eight needs
+// the kernel's leave, and its SMs in one part of the GPU, so it is asked how many there can be.  1 row of 128,256 with
+// top-k and top-p 15.6 -> 14.7 us, with top-p alone 22 -> 18 us; 64 and 256 rows would take 1.7 times as long.)
 template <typename S>
-int launch_sample_logits(SampleArgs a, uint32_t rows, cudaStream_t st) {
+bool wide_clusters(uint32_t rows, size_t smem, int sm_count) {
+  if ((uint64_t)rows * kWide > (uint64_t)sm_count) return false;
+  auto kernel = sample_logits_kernel<S, kWide>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows * kWide);
+  cfg.blockDim = dim3(kThr);
+  cfg.dynamicSmemBytes = smem;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return n >= (int)rows;
+}
+
+template <typename S, int CL>
+int launch_sample_logits(SampleArgs a, uint32_t rows, size_t smem, cudaStream_t st) {
+  return launch_pdl(sample_logits_kernel<S, CL>, dim3(rows * CL), dim3(kThr), smem, st, a);
+}
+
+template <typename S>
+int launch_sample_logits(SampleArgs a, uint32_t rows, int sm_count, cudaStream_t st) {
   constexpr int N = 16 / sizeof(S);
-  a.slice = (uint32_t)((ceil_div(a.V, kCl) + N - 1) / N * N);
-  a.slice = (a.slice + 3) / 4 * 4;  // four entries a lane, and the tables after the keys stay 16-byte aligned
   a.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.ld % N == 0;
-  const size_t smem = (size_t)a.slice * 4 + 2 * kBins * sizeof(uint32_t);
-  CLM_TRY(ensure_smem(sample_logits_kernel<S>, smem + sizeof(Shared)));  // (the limit counts static memory too)
-  return launch_pdl(sample_logits_kernel<S>, dim3(rows * kCl), dim3(kThr), smem, st, a);
+  auto memory = [&](int ctas) {
+    a.slice = (uint32_t)((ceil_div(a.V, ctas) + N - 1) / N * N);
+    a.slice = (a.slice + 3) / 4 * 4;  // four entries a lane, and the tables after the keys stay 16-byte aligned
+    return (size_t)a.slice * 4 + 2 * kBins * sizeof(uint32_t);
+  };
+  size_t smem = memory(kWide);
+  CLM_TRY(ensure_smem(sample_logits_kernel<S, kWide>, smem + sizeof(Shared<kWide>)));  // (the limit counts static memory)
+  if (wide_clusters<S>(rows, smem, sm_count)) return launch_sample_logits<S, kWide>(a, rows, smem, st);
+  smem = memory(kCl);
+  CLM_TRY(ensure_smem(sample_logits_kernel<S, kCl>, smem + sizeof(Shared<kCl>)));
+  return launch_sample_logits<S, kCl>(a, rows, smem, st);
 }
 
 }  // namespace
@@ -776,7 +810,7 @@ extern "C" int clm_b200_sample_logits(clm_b200_ctx* ctx, const void* d_logits, i
   a.prob = d_probs;
   CLM_SCOPE(ctx);
   cudaStream_t st = pick_stream(ctx, stream);
-  if (dtype == CLM_DTYPE_F32) return launch_sample_logits<float>(a, rows, st);
-  if (dtype == CLM_DTYPE_F16) return launch_sample_logits<__half>(a, rows, st);
-  return launch_sample_logits<__nv_bfloat16>(a, rows, st);
+  if (dtype == CLM_DTYPE_F32) return launch_sample_logits<float>(a, rows, ctx->sm_count, st);
+  if (dtype == CLM_DTYPE_F16) return launch_sample_logits<__half>(a, rows, ctx->sm_count, st);
+  return launch_sample_logits<__nv_bfloat16>(a, rows, ctx->sm_count, st);
 }

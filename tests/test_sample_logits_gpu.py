@@ -168,6 +168,20 @@ def test_a_row_does_not_depend_on_its_batch(ctx, sample):
         assert int(one) == int(whole[r]) and float(po) == float(pw[r])
 
 
+@pytest.mark.parametrize("vocab", [1, 130, 3001, 128256])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=7), dict(top_p=0.8), dict(min_p=0.03), dict(top_k=900, top_p=0.97),
+                                dict(temperature=0.0), dict(temperature=2.5, top_p=0.99)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_rows_and_many_agree(ctx, sample, vocab, kw, dtype):
+    """Rows alone, whose parts are halves of those that rows of a batch have."""
+    logits, u = gaussian(24, vocab, 21, dtype=dtype), uniforms(24, 21)
+    tok, prob = sample(ctx, logits, u, with_probs=True, **kw)
+    for r in range(0, 24, 5):
+        one, p = sample(ctx, logits[r:r + 2], u[r:r + 2], with_probs=True, **kw)
+        assert torch.equal(one, tok[r:r + 2]) and torch.equal(p, prob[r:r + 2])
+    check(ctx, sample, logits, u, **{"temp" if k == "temperature" else k: x for k, x in kw.items()})
+
+
 def test_frequencies_follow_the_distribution(ctx, sample):
     """100,000 draws of a 12-token row: every token within 5 standard deviations of its share."""
     row = torch.tensor([[2.0, 1.5, 1.0, 0.5, 0.0, -0.5, -1.0, -2.0, -3.0, 1.9, 1.4, 0.9]], device="cuda")

@@ -117,6 +117,8 @@ struct Shared {
   u64 kept[CL];      // allowed mass
   uint32_t ncand[CL], umin[CL], umax[CL];  // candidates: how many, their key range
   uint32_t ties[CL];
+  u64 half_mass[CL];       // of the lower half of the keys that are left, where a level halves them: slots that look()
+  uint32_t half_count[CL];  // does not write, so that its barriers lie between two uses of them
   u64 seg[kWrp];      // allowed mass of the warp segments
   u64 red[kWrp];
   uint32_t redc[kWrp];
@@ -554,15 +556,17 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kThr, CL == kCl ? 2
           ++cl;
           ml += mass(d);
         });
-        push(s.ncand, cta_sum(__reduce_add_sync(0xffffffffu, cl), s.redc, warp, lane));
-        push(s.total, cta_sum(warp_sum(ml), s.red, warp, lane));
+        // Every CTA has read what the look before left in ncand and total only once it passes the barrier below, and may
+        // still read these sums while a faster one is in the next look, which writes both: hence their own slots.
+        push(s.half_count, cta_sum(__reduce_add_sync(0xffffffffu, cl), s.redc, warp, lane));
+        push(s.half_mass, cta_sum(warp_sum(ml), s.red, warp, lane));
         cluster.sync();
         uint32_t count = 0;
         u64 sum = 0;
 #pragma unroll
         for (int r = 0; r < CL; ++r) {
-          count += s.ncand[r];
-          sum += s.total[r];
+          count += s.half_count[r];
+          sum += s.half_mass[r];
         }
         if (cnt_above + count >= k || above + sum >= thr) {
           uh = umax = mid;

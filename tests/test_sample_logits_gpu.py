@@ -100,6 +100,28 @@ def test_one_entry_outweighs_thousands(ctx, sample):
         check(ctx, sample, logits, torch.tensor([0.0, 0.5, 1 - 1e-6, 1 - 1e-7, 1 - 2.0**-53], dtype=torch.float64).cuda(), top_p=p)
 
 
+@pytest.mark.parametrize("rows", [1, 5, 64])
+@pytest.mark.parametrize("spread", ["first eighth", "last sixteenth", "everywhere"])
+def test_halving_with_uneven_slices(ctx, sample, rows, spread):
+    """One entry outweighs thousands, several levels are halved by exact sums, and the parts of a row have unlike work: all the
+    others in one part, so that the rest of the row's CTAs run ahead of it.  Every repetition gives the same tokens."""
+    vocab = 48000
+    first, last = {"first eighth": (0, vocab // 8), "last sixteenth": (vocab - vocab // 16, vocab), "everywhere": (0, vocab)}[spread]
+    g = torch.Generator(device="cuda").manual_seed(31)
+    logits = torch.full((rows, vocab), -math.inf, device="cuda")
+    logits[:, first:last] = torch.rand(rows, last - first, device="cuda", generator=g) - 20.0
+    logits[:, first + 11] = 0.0
+    rest = float(torch.exp(logits[0].double()).sum() - 1.0)
+    u = uniforms(rows, 31)
+    u[::2] = 1 - 2.0**-53 * (1 + torch.arange(len(u[::2]), dtype=torch.float64, device="cuda"))
+    for part in (0.03, 0.5, 0.98):
+        p = np.float32((1.0 + part * rest) / (1.0 + rest))
+        want = check(ctx, sample, logits, u, top_p=p)
+        top_p = torch.full((rows,), float(p), device="cuda")
+        for _ in range(50):
+            assert torch.equal(sample(ctx, logits, u, top_p=top_p), want)
+
+
 def test_masks_infinities_and_nan(ctx, sample):
     logits = gaussian(9, 3001, 6)
     logits[0] = -math.inf                       # nothing left

@@ -1737,7 +1737,9 @@ int llama_session_close(LlamaEngine* e, uint64_t id) {
   CLM_TRY(engine_enter(e));
   Session* s = find_session(e, id);
   if (!s) return CLM_OK;  // idempotent cleanup (WindowLedger::abort_session)
-  CLM_CUDA(cudaStreamSynchronize(e->ctx->stream));
+  // Work that was queued for the session on any stream ends before its slot and pages go to the next session: tables,
+  // states and pages are rows of the engine's arrays, so nothing here frees memory and waits on that account.
+  CLM_CUDA(cudaDeviceSynchronize());
   e->drop_batch_graphs();
   e->release_session(*s);
   e->sessions.erase(id);

@@ -345,6 +345,8 @@ CLM_API int clm_b200_engine_prepare(clm_b200_engine* e);
 CLM_API int clm_b200_engine_info(const clm_b200_engine* e, uint64_t* weight_bytes, uint64_t* state_bytes_per_session,
                                  uint32_t* floats_per_position);
 CLM_API int clm_b200_session_open(clm_b200_engine* e, uint64_t session);
+/* Waits for the work queued on the device (the session's windows and rounds on any stream), then gives the session's
+ * pages and its place back. */
 CLM_API int clm_b200_session_close(clm_b200_engine* e, uint64_t session);
 /* Opens `child` as a continuation of `parent` at its committed position: the full pages of the parent's KV cache are
  * shared (each holds until its last session closes), the last page is copied, and the state of speculative rounds (next

@@ -47,6 +47,8 @@ struct Gemv {
   const GemvPlan& for_q(int q) const { return plan[q <= 8 ? 0 : (q <= 16 ? 1 : 2)]; }
 };
 
+constexpr int kBatchChainMax = 4;  // sessions of a batched window on the GEMV chain
+
 struct Session {
   uint64_t id = 0;
   std::vector<int32_t> pages;     // of its context; the leading ones may be shared (clm_b200_session_fork)
@@ -65,6 +67,8 @@ struct Session {
   std::map<int, FlowPhase*> flow_phases;  // dataflow window kernel phase tables by q (device arrays)
   int32_t* d_win = nullptr;    // pipeline tail: this session's current window tokens [W + 1]
   float* d_dprobs = nullptr;   // pipeline tail: draft distributions of the current window [W][V]
+  cudaEvent_t queued = nullptr;  // after what the last call queued for it on a caller's stream
+  bool has_queued = false;       // such a call was made since the context's stream last waited for it
   bool own_links = false;      // pipeline: the session's messages use lin / lout below (clm_b200_pipe_attach_session)
   LinkDev lin, lout;
 };
@@ -1141,7 +1145,48 @@ struct LlamaEngine : clm_b200_engine {
     return CLM_OK;
   }
 
+  // Notes the end of what a call queues for its sessions on a caller's stream (at the end of the call, whatever it returns).
+  // An engine's calls share its buffers, so callers order them: the last one's end is the end of all of them.
+  struct Queued {
+    LlamaEngine* e;
+    cudaStream_t st;
+    Session* s[kBatchChainMax];
+    int n = 1;
+    Queued(LlamaEngine* engine, cudaStream_t stream, Session* one) : e(engine), st(stream), s{one} {}
+    Queued(LlamaEngine* engine, cudaStream_t stream, const std::vector<WideSeg>& segs) : e(engine), st(stream), s{}, n(0) {
+      for (const WideSeg& g : segs) s[n++] = g.s;
+    }
+    Queued(const Queued&) = delete;
+    Queued& operator=(const Queued&) = delete;
+    ~Queued() {
+      cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+      if (st == e->ctx->stream || cudaStreamIsCapturing(st, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone)
+        return;
+      for (int i = 0; i < n; ++i) {
+        Session& x = *s[i];
+        x.has_queued = true;
+        if (x.queued == nullptr && cudaEventCreateWithFlags(&x.queued, cudaEventDisableTiming) != cudaSuccess) x.queued = nullptr;
+        if (x.queued != nullptr && cudaEventRecord(x.queued, st) != cudaSuccess) {
+          cudaEventDestroy(x.queued);
+          x.queued = nullptr;  // (after_queued then waits for the device)
+        }
+      }
+    }
+  };
+  // Orders the context's stream behind the session's work on callers' streams.
+  int after_queued(Session& s) {
+    if (!s.has_queued) return CLM_OK;
+    if (s.queued != nullptr)
+      CLM_CUDA(cudaStreamWaitEvent(ctx->stream, s.queued, 0));
+    else
+      CLM_CUDA(cudaDeviceSynchronize());
+    s.has_queued = false;
+    return CLM_OK;
+  }
+
   void release_session(Session& s) {
+    if (s.queued != nullptr) cudaEventDestroy(s.queued);
+    s.queued = nullptr;
     for (auto& kv : s.graphs) cudaGraphExecDestroy(kv.second);
     s.graphs.clear();
     for (auto& kv : s.flow_phases) cudaFree(kv.second);
@@ -1764,6 +1809,7 @@ int llama_session_fork(LlamaEngine* e, uint64_t parent_id, uint64_t id) {
   CLM_CHECK(parent != nullptr, CLM_NOT_FOUND, "session not open");
   CLM_CHECK(find_session(e, id) == nullptr, CLM_ALREADY_EXISTS, "session already open");
   CLM_CHECK(parent->outstanding == 0, CLM_FAILED_PRECONDITION, "a window is outstanding for the parent session");
+  CLM_TRY(e->after_queued(*parent));  // rounds in flight on a caller's stream
   CLM_TRY(sync_pos(e, parent));
   return add_session(e, id, parent);
 }
@@ -1790,6 +1836,7 @@ int llama_run_window_device(LlamaEngine* e, uint64_t id, uint64_t base, uint32_t
   cudaStream_t st = pick_stream(e->ctx, stream);
   Session* s = nullptr;
   CLM_TRY(run_window_common(e, id, base, q, st, &s));
+  LlamaEngine::Queued mark(e, st, s);
   const size_t rec = (size_t)q * e->floats_per_position() * sizeof(float);
   if (e->has_tokens) {
     CLM_CHECK(d_tokens != nullptr, CLM_INVALID_ARGUMENT, "this stage consumes tokens");
@@ -1816,6 +1863,7 @@ int llama_run_tree_device(LlamaEngine* e, uint64_t id, uint64_t base, uint32_t q
   cudaStream_t st = pick_stream(e->ctx, stream);
   Session* s = nullptr;
   CLM_TRY(run_window_common(e, id, base, q, st, &s));
+  LlamaEngine::Queued mark(e, st, s);
   const size_t rec = (size_t)q * e->floats_per_position() * sizeof(float);
   if (e->has_tokens) {
     CLM_CHECK(d_tokens != nullptr, CLM_INVALID_ARGUMENT, "this stage consumes tokens");
@@ -1948,7 +1996,7 @@ int llama_run_batch_device(LlamaEngine* e, uint32_t n, const uint64_t* ids, cons
                            const int32_t* d_tokens, const float* d_in, float* d_out, float* d_logits, void* stream) {
   CLM_TRY(engine_enter(e));
   CLM_CHECK(e->prepared, CLM_FAILED_PRECONDITION, "engine not prepared");
-  CLM_CHECK(ids != nullptr && bases != nullptr && n >= 1 && n <= 4 && q >= 1 && q <= 8, CLM_INVALID_ARGUMENT,
+  CLM_CHECK(ids != nullptr && bases != nullptr && n >= 1 && n <= (uint32_t)kBatchChainMax && q >= 1 && q <= 8, CLM_INVALID_ARGUMENT,
             "batched GEMV window: 1..4 sessions of 1..8 rows");
   const uint32_t Q = n * q;
   CLM_CHECK(Q <= e->spec.max_window, CLM_RESOURCE_EXHAUSTED, "batched window exceeds max_window");
@@ -1964,6 +2012,7 @@ int llama_run_batch_device(LlamaEngine* e, uint32_t n, const uint64_t* ids, cons
     CLM_TRY(run_window_common(e, ids[b], bases[b], q, st, &s));
     segs.push_back({s, (int)(b * q), (int)q});
   }
+  LlamaEngine::Queued mark(e, st, segs);
   const size_t rec = (size_t)Q * e->floats_per_position() * sizeof(float);
   if (e->has_tokens)
     CLM_CUDA(cudaMemcpyAsync(e->win, d_tokens, Q * sizeof(int32_t), cudaMemcpyDeviceToDevice, st));
@@ -2190,6 +2239,7 @@ int llama_spec_round_device(LlamaEngine* e, uint64_t id, const clm_b200_spec_par
   CLM_CHECK((uint64_t)s->pos_bound + p->q <= e->spec.max_context, CLM_RESOURCE_EXHAUSTED,
             "speculative round would exceed max_context");
   cudaStream_t st = pick_stream(e->ctx, stream);
+  LlamaEngine::Queued mark(e, st, s);
   const bool stochastic = p->temperature > 0.0f;
   // the round's inputs (temperature, seed) go host -> device each round; the graph reads them there
   RoundCtl c{p->temperature, 0u, (unsigned long long)p->seed};
@@ -2268,6 +2318,7 @@ int llama_pipe_prefill(LlamaEngine* e, uint64_t id, const int32_t* h_tokens, uin
   Session* s = nullptr;
   CLM_TRY(pipe_session(e, id, q, &s));
   cudaStream_t st = pick_stream(e->ctx, stream);
+  LlamaEngine::Queued mark(e, st, s);
   if (e->spec.role == CLM_ROLE_PREFIX) {
     CLM_CHECK(h_tokens != nullptr, CLM_INVALID_ARGUMENT, "the prefix consumes tokens");
     for (uint32_t i = 0; i < q; ++i)
@@ -2288,6 +2339,7 @@ int llama_pipe_begin(LlamaEngine* e, uint64_t id, uint32_t row, const clm_b200_s
   CLM_TRY(pipe_session(e, id, p->q, &s));
   CLM_CHECK(row < e->spec.max_window, CLM_OUT_OF_RANGE, "row outside the last window");
   cudaStream_t st = pick_stream(e->ctx, stream);
+  LlamaEngine::Queued mark(e, st, s);
   const bool stochastic = p->temperature > 0.0f;
   RoundCtl c{p->temperature, 0u, (unsigned long long)p->seed};
   CLM_CUDA(cudaMemcpyAsync(e->ctl, &c, sizeof(c), cudaMemcpyHostToDevice, st));
@@ -2306,6 +2358,7 @@ int llama_pipe_round(LlamaEngine* e, uint64_t id, const clm_b200_spec_params* p,
   Session* s = nullptr;
   CLM_TRY(pipe_session(e, id, p->q, &s));
   cudaStream_t st = pick_stream(e->ctx, stream);
+  LlamaEngine::Queued mark(e, st, s);
   const bool stochastic = p->temperature > 0.0f;
   if (e->spec.role == CLM_ROLE_TAIL) {
     RoundCtl c{p->temperature, 0u, (unsigned long long)p->seed};

@@ -1,4 +1,4 @@
-"""Sessions that are closed while work of theirs is queued on a caller's stream."""
+"""Sessions that are closed or forked while work of theirs is queued on a caller's stream."""
 import numpy as np
 import pytest
 
@@ -60,3 +60,37 @@ def test_close_waits_for_work_on_another_stream(ctx, kind):
         e.close_session(100 + turn)
         del kept
     e.close()
+
+
+def test_fork_waits_for_rounds_on_another_stream(ctx):
+    """The child continues after the rounds that were queued for its parent when it was forked."""
+    import torch
+
+    geo = small_geo("q4_k")
+    prompt = np.random.default_rng(6).integers(0, geo.vocab, 60).astype(np.int32)  # the rounds pass a page's end
+    side = torch.cuda.Stream()
+
+    def rounds(e, s):
+        return [int(t) for _ in range(6) for t in e.spec_round(s, 4, temperature=1.0, seed=3)]
+
+    for turn in range(3):
+        e = make_engine(ctx, geo, max_context=256, max_window=16, sessions=3)
+        ref = make_engine(ctx, geo, max_context=256, max_window=16, sessions=1)
+        for x in (e, ref):
+            x.open_session(1)
+            x.spec_begin(1, prompt, 4, temperature=1.0, seed=3)
+            for _ in range(turn):
+                x.spec_round(1, 4, temperature=1.0, seed=3)
+        for _ in range(12):
+            ref.spec_round(1, 4, temperature=1.0, seed=3)
+        kept = queue(e, 1, side, "rounds", 0, geo.vocab)
+        e.fork_session(1, 2)
+        assert side.query()
+        assert e.position(2) == ref.position(1) and e.position(1) == ref.position(1)
+        want = rounds(ref, 1)
+        assert rounds(e, 2) == want and rounds(e, 1) == want
+        e.fork_session(1, 3)  # nothing queued since: the position is the parent's now
+        assert e.position(3) == ref.position(1)
+        del kept
+        e.close()
+        ref.close()

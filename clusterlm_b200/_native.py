@@ -67,6 +67,7 @@ _SIGS = {
     "clm_b200_kv_attention_workspace": (_i, [_vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, C.POINTER(_u64)]),
     "clm_b200_kv_attention": (_i, [_vp, _vp, _u32, _vp, _u32, _u32, _u32, _vp, _u64, _u32, _vp, _vp, _vp, _f, _vp, _vp,
                                    _u64, _vp]),
+    "clm_b200_kv_attention_wait_limit": (_i, [_vp, _u32]),
     "clm_b200_kv_fork": (_i, [_vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
     "clm_b200_kv_copy_pages": (_i, [_vp, _vp, _u32, _vp, _vp, _vp, _u64, _vp]),
     "clm_b200_pages_create": (_i, [_u32, C.POINTER(_vp)]),

@@ -38,6 +38,10 @@ int cuda_fail(cudaError_t e, const char* what);
 
 }  // namespace clm
 
+namespace clm {
+constexpr uint32_t kAttentionPolls = 1u << 20;  // polls of a wait in the paged attention's kernels, unless set
+}
+
 // Context: one device, one stream, and a scratch arena reused by calls that need temporaries.
 struct clm_b200_ctx {
   int device = 0;
@@ -50,6 +54,7 @@ struct clm_b200_ctx {
   // while some are alive only marks the context closed; the last object's destruction frees it.
   int refs = 0;
   bool closed = false;
+  uint32_t attention_polls = clm::kAttentionPolls;  // clm_b200_kv_attention_wait_limit
 };
 
 namespace clm {

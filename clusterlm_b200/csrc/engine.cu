@@ -797,6 +797,7 @@ struct LlamaEngine : clm_b200_engine {
     a.work = share_work;
     a.work_bytes = share_bytes;
     a.sm_count = ctx->sm_count;
+    a.polls = ctx->attention_polls;
     return a;
   }
   // Its workspace (grown outside of captures; captured batched windows hold the old one's address and are dropped).

@@ -62,6 +62,7 @@ struct Args {
   const int32_t* parent;
   int positions, nh, nkv, group;
   float scale_log2;
+  uint32_t polls;  // a wait of the tile kernel gives up after so many
   // partials of groups [0] and sequences [1]: segment x rows (tile kernel: 2 x 128, or 2 x rows, one half per stream)
   struct Kind {
     Plan* plan;     // of the kernel that has this kind
@@ -488,6 +489,9 @@ struct Walk {
 // row's maximum grows by more than 2^8 (weights stay below 2^8, far inside the types' range); the first maximum of a
 // segment sets the reference.
 //
+// Every wait is bounded.  When one gives up, all warps do: the rows whose products are missing become NaN, and the
+// CTA ends after its products and copies in flight.
+//
 // Bound by the tensor pipe: a page of both streams takes 2,230 clocks, of which 16 score products (M 128, N 64, K 16,
 // both operands in shared memory) take 107 each and 8 products with V 64 each.  (Score products of two pages, N 128,
 // take no longer, but their scores leave no room for a second buffer: a page of both streams then waits for its own
@@ -561,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
   const uint32_t tmem = s_tmem;
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     const uint32_t addr = smem_addr(bar);
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    for (uint32_t i = 0; i < a.polls; ++i) {
       uint32_t done;
       asm volatile(
           "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -574,6 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
     s_dead = 1;
     return false;
   };
+  // the same for all of a warp, whose lanes vote and elect afterwards
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
   Walk walk(a, plan, s_first, shares.begin(blockIdx.x), shares.begin(blockIdx.x + 1));
   Segment g;
@@ -667,6 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
   } else if (warp >= kMma) {
     // ---------------- products of stream s ----------------
     const int s = warp - kMma;
@@ -683,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
         };
         auto scores = [&](int b) {  // S = Q K^T of page b, the stream's page `asked`
           const int slot = (int)((idx0 + b) % SL);
-          if (!wait(&full_k[s][asked % SL], (asked / SL) & 1u)) return false;
+          if (!warp_wait(&full_k[s][asked % SL], (asked / SL) & 1u)) return false;
           tc_after();
           const uint32_t k = ra + (uint32_t)slot * 2 * TL::kHalf;
           if (elect_one()) {
@@ -701,10 +708,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           return true;
         };
         int b = g.pair ? 0 : s;
-        ok = wait(&q_ready[s], segs++ & 1u) && scores(b) && (b + step >= g.pages || scores(b + step));
+        ok = warp_wait(&q_ready[s], segs++ & 1u) && scores(b) && (b + step >= g.pages || scores(b + step));
         for (bool first = true; ok && b < g.pages; b += step, first = false, ++done) {
           const int slot = (int)((idx0 + b) % SL);
-          if (!(ok = wait(&full_v[s][done % SL], (done / SL) & 1u) && wait(&p_ready[s][done & 1u], (done >> 1) & 1u))) break;
+          if (!(ok = warp_wait(&full_v[s][done % SL], (done / SL) & 1u) &&
+                     warp_wait(&p_ready[s][done & 1u], (done >> 1) & 1u)))
+            break;
           tc_after();
           const uint32_t v = ra + (uint32_t)slot * 2 * TL::kHalf + TL::kHalf;
           if (elect_one()) {
@@ -718,11 +727,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           if (b + 2 * step < g.pages) ok = scores(b + 2 * step);  // over the weights that these products read
         }
       }
-      if (!ok) {  // products may be in flight: the accumulators are freed after them
-        if (elect_one()) tc_commit(&drained[s]);
-        __syncwarp();
-        mbar_wait(&drained[s], 0, nullptr);
-      }
+      // The accumulators are freed after the last products, also where the softmax no longer waits for them.
+      if (elect_one()) tc_commit(&drained[s]);
+      __syncwarp();
+      mbar_wait(&drained[s], 0, nullptr);
     }
     __syncwarp();
   } else {
@@ -777,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
       float m = -INFINITY, l = 0.0f;  // m: the reference of the weights so far (scaled scores)
       const int np = g.stream_pages(s);
       for (int t = 0; t < np; ++t, ++done) {
-        ok = ok && wait(&s_full[s][done & 1u], (done >> 1) & 1u);
+        ok = ok && warp_wait(&s_full[s][done & 1u], (done >> 1) & 1u);
         if (work && ok) {
           tc_after();
           const int b = g.pair ? t : 2 * t + s;
@@ -805,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
             const bool grow = top > m + 8.0f;
             if (__any_sync(0xffffffffu, grow)) {
               // the products of the page before are the last to add to O
-              ok = wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
+              ok = warp_wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
               tc_after();
               const float f = grow ? ex2(m - top) : 1.0f;  // 0 for a row that had seen nothing
               if (grow) m = top;
@@ -858,7 +866,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
       const long long was_base = base;
       const bool was_work = work, was_valid = valid;
       if ((more = advance())) load();
-      ok = ok && wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
+      ok = ok && warp_wait(&o_done[s][(done - 1) & 1u], ((done - 1) >> 1) & 1u);
       if (was_work) {
         tc_after();
         const int seg = was.item + (int)blockIdx.x;
@@ -1429,6 +1437,7 @@ int launch_kv_attention(const KvAttnArgs& in, cudaStream_t st) {
   a.group = in.nh / in.nkv;
   // (a zero scale weighs all positions alike: a product with a masked score of -inf must not become NaN)
   a.scale_log2 = std::max(in.scale * 1.4426950408889634f, FLT_MIN);
+  a.polls = in.polls;
   uint8_t* w = static_cast<uint8_t*>(in.work);
   for (int k = 0; k < 2; ++k) {
     a.kind[k].plan = reinterpret_cast<Plan*>(w + (s.tile[k] ? 0 : s.plan));  // one plan per kernel
@@ -1535,8 +1544,15 @@ int clm_b200_kv_attention(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint3
   a.work = d_work;
   a.work_bytes = work_bytes;
   a.sm_count = ctx->sm_count;
+  a.polls = ctx->attention_polls;
   CLM_SCOPE(ctx);
   return launch_kv_attention(a, pick_stream(ctx, stream));
+}
+
+int clm_b200_kv_attention_wait_limit(clm_b200_ctx* ctx, uint32_t polls) {
+  CLM_CHECK(ctx != nullptr, CLM_INVALID_ARGUMENT, "null context");
+  ctx->attention_polls = polls;
+  return CLM_OK;
 }
 
 }  // extern "C"

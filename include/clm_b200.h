@@ -254,7 +254,7 @@ CLM_API int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, 
  * and sums are f32, the weights round to the pool's type for their product with v; scale >= 0.  Rows that see nothing
  * (idle sequences) become 0.  q rows ld_q elements apart, 16-byte aligned, like d_out; q, pool and out have one type.
  * d_work: clm_b200_kv_attention_workspace bytes, 16-byte aligned, used by this call alone while it runs (a captured
- * graph keeps its own). */
+ * graph keeps its own).  The waits inside are bounded: rows whose operands never arrive become NaN. */
 CLM_API int clm_b200_kv_attention_workspace(clm_b200_ctx* ctx, uint32_t n, uint32_t positions, uint32_t n_heads,
                                             uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_groups,
                                             const uint32_t* h_group_seqs, const uint32_t* h_group_pages,
@@ -264,6 +264,9 @@ CLM_API int clm_b200_kv_attention(clm_b200_ctx* ctx, const clm_b200_kv_pool* poo
                                   const void* d_q, uint64_t ld_q, uint32_t n_groups, const uint32_t* h_group_seqs,
                                   const uint32_t* h_group_pages, const int32_t* d_parents, float scale, void* d_out,
                                   void* d_work, uint64_t work_bytes, void* stream);
+/* Polls after which such a wait gives up (2^20 unless set; each suspends the thread for a moment), for this context's
+ * later calls and its engines' later windows; captured ones keep theirs. */
+CLM_API int clm_b200_kv_attention_wait_limit(clm_b200_ctx* ctx, uint32_t polls);
 /* Forks: child h_children[i] takes over the full pages of h_parents[i] (the table entries), its position, and a copy,
  * in page h_new_pages[i], of the parent's last page in every layer (no copy when the position is a multiple of 64; the
  * entry is set all the same).  n <= 256; a child appears once and is no parent of the same call. */

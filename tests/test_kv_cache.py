@@ -274,3 +274,17 @@ def test_empty_calls_touch_nothing():
     need = C.c_uint64(9)
     assert _native.lib.clm_b200_kv_attention_workspace(CTX, 0, 4, 8, 8, 128, 0, None, None, C.byref(need)) == 0
     assert need.value == 0
+
+
+def test_wait_limit_refuses():
+    from clusterlm_b200.kv_cache import set_wait_limit
+
+    class Ctx:
+        h = None
+
+    with pytest.raises(ClmError) as err:
+        set_wait_limit(Ctx())
+    assert err.value.code == INVALID
+    for polls in (-1, 2**32):
+        with pytest.raises(ValueError):
+            set_wait_limit(Ctx(), polls)

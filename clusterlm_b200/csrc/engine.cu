@@ -798,6 +798,7 @@ struct LlamaEngine : clm_b200_engine {
     a.work_bytes = share_bytes;
     a.sm_count = ctx->sm_count;
     a.polls = ctx->attention_polls;
+    a.err = bad;
     return a;
   }
   // Its workspace (grown outside of captures; captured batched windows hold the old one's address and are dropped).

@@ -63,6 +63,7 @@ struct Args {
   int positions, nh, nkv, group;
   float scale_log2;
   uint32_t polls;  // a wait of the tile kernel gives up after so many
+  int* err;        // and then this flag is raised (or null)
   // partials of groups [0] and sequences [1]: segment x rows (tile kernel: 2 x 128, or 2 x rows, one half per stream)
   struct Kind {
     Plan* plan;     // of the kernel that has this kind
@@ -489,8 +490,8 @@ struct Walk {
 // row's maximum grows by more than 2^8 (weights stay below 2^8, far inside the types' range); the first maximum of a
 // segment sets the reference.
 //
-// Every wait is bounded.  When one gives up, all warps do: the rows whose products are missing become NaN, and the
-// CTA ends after its products and copies in flight.
+// Every wait is bounded.  When one gives up, all warps do: the rows whose products are missing become NaN, the caller's
+// flag is raised, and the CTA ends after its products and copies in flight.
 //
 // Bound by the tensor pipe: a page of both streams takes 2,230 clocks, of which 16 score products (M 128, N 64, K 16,
 // both operands in shared memory) take 107 each and 8 products with V 64 each.  (Score products of two pages, N 128,
@@ -913,6 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0 && s_dead && a.err != nullptr) atomicExch(a.err, kErrWaitTimeout);
   if (warp == kMma) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -1438,6 +1440,7 @@ int launch_kv_attention(const KvAttnArgs& in, cudaStream_t st) {
   // (a zero scale weighs all positions alike: a product with a masked score of -inf must not become NaN)
   a.scale_log2 = std::max(in.scale * 1.4426950408889634f, FLT_MIN);
   a.polls = in.polls;
+  a.err = in.err;
   uint8_t* w = static_cast<uint8_t*>(in.work);
   for (int k = 0; k < 2; ++k) {
     a.kind[k].plan = reinterpret_cast<Plan*>(w + (s.tile[k] ? 0 : s.plan));  // one plan per kernel

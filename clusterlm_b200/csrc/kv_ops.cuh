@@ -61,7 +61,8 @@ struct KvAttnArgs {
   void* work = nullptr;
   size_t work_bytes = 0;
   int sm_count = 148;
-  uint32_t polls = kAttentionPolls;  // a wait inside gives up after so many polls: rows of NaN
+  uint32_t polls = kAttentionPolls;  // a wait inside gives up after so many polls: rows of NaN, and
+  int* err = nullptr;                // (device) kErrWaitTimeout here
 };
 // Workspace bytes of launch_kv_attention (an upper bound over the device-side lengths).
 size_t kv_attention_work(int n, int positions, int nh, int nkv, int hd, const KvGroups& groups, int sm_count);

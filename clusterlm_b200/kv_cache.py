@@ -178,7 +178,7 @@ def kv_attention(ctx: Context, k_pool, v_pool, tables, pos, q, groups=None, scal
 
 def set_wait_limit(ctx: Context, polls: int = 2**20) -> None:
     """Polls after which a device wait inside kv_attention gives up and leaves NaN rows, for later calls of the context
-    and later windows of its engines; captured ones keep theirs."""
+    and later windows of its engines (whose commit then fails); captured ones keep theirs."""
     if not 0 <= polls < 2**32:
         raise ValueError("polls: expected 0 to 2^32 - 1")
     call("clm_b200_kv_attention_wait_limit", ctx.h, polls)

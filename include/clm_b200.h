@@ -254,7 +254,8 @@ CLM_API int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, 
  * and sums are f32, the weights round to the pool's type for their product with v; scale >= 0.  Rows that see nothing
  * (idle sequences) become 0.  q rows ld_q elements apart, 16-byte aligned, like d_out; q, pool and out have one type.
  * d_work: clm_b200_kv_attention_workspace bytes, 16-byte aligned, used by this call alone while it runs (a captured
- * graph keeps its own).  The waits inside are bounded: rows whose operands never arrive become NaN. */
+ * graph keeps its own).  The waits inside are bounded: rows whose operands never arrive become NaN (in an engine's window
+ * the commit then fails with CLM_DEADLINE_EXCEEDED). */
 CLM_API int clm_b200_kv_attention_workspace(clm_b200_ctx* ctx, uint32_t n, uint32_t positions, uint32_t n_heads,
                                             uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_groups,
                                             const uint32_t* h_group_seqs, const uint32_t* h_group_pages,

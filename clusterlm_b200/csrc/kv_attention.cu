@@ -151,7 +151,8 @@ struct Shares {
 __device__ __forceinline__ Shares Plan::cut() const { return Shares{shares, q, r}; }
 
 // Fills the plan of the tile (or stream) kernel from the device-side positions: pages per item, then the running work
-// of its entries (the other kernel's have none).  first: the entries' first pages.
+// of its entries (the other kernel's have none).  first: a sequence's first page of its own; of a group the sequence whose
+// table names its pages, the first that is not idle (an idle one's table may name anything).
 __device__ void make_plan(const Args& a, Plan* plan, int* first, int tile, uint32_t shares) {
   const int E = a.groups.n + a.seqs.n;
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
@@ -159,7 +160,9 @@ __device__ void make_plan(const Args& a, Plan* plan, int* first, int tile, uint3
     const int per = tile ? 1 : 2, unit = kPageTokens / per;
     int pages = 0, at = 0;
     if (e < a.groups.n) {
-      pages = per * min((int)a.groups.pages[e], a.seqs.max_pages);
+      for (at = en.s0; at < en.s1 && a.seqs.base(at) < 0; ++at) {
+      }
+      if (at < en.s1) pages = per * min((int)a.groups.pages[e], a.seqs.max_pages);
     } else {
       const long long base = a.seqs.base(en.s0);
       at = shared_pages(a, en.s0);
@@ -440,6 +443,7 @@ struct Segment {
   int item, kvh, x0, rows;   // item among its kind; kv head, first row, rows (<= kRowTile)
   bool group, pair;          // group entry; more than 128 rows
   int s0;                    // its (first) sequence
+  int named;                 // the sequence whose table names the pages
   int page0, pages;          // table entry of the first page, pages
   int streams;               // streams with work
   __device__ __forceinline__ int stream_pages(int s) const { return pair ? pages : (pages + 1 - s) / 2; }
@@ -471,7 +475,8 @@ struct Walk {
       s.x0 = (int)tile % en.tiles * kRowTile;
       s.rows = min(en.rows - s.x0, kRowTile);
       s.pair = s.rows > 128;
-      s.page0 = first[e] + (int)b0;
+      s.named = s.group ? first[e] : en.s0;
+      s.page0 = (s.group ? 0 : first[e]) + (int)b0;
       s.pages = (int)(b1 - b0);
       s.streams = s.pair || s.pages > 1 ? 2 : 1;
       return true;
@@ -619,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
     uint32_t idx = 0;
     bool ok = true;
     while (ok && walk.next(g)) {
-      const int32_t* table = a.seqs.table(g.s0) + g.page0;
+      const int32_t* table = a.seqs.table(g.named) + g.page0;
       // positions at or after `base` are the window's (or nobody's): their values are checked
       const long long base = g.group ? 0x7fffffffffffffffll : a.seqs.base(g.s0);
       int32_t page = __ldg(table);
@@ -1001,8 +1006,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
     w = min(u0 + units, end);
     if (off >= upto) continue;
     const int halves = (int)(upto - off);
-    const int half0 = (int)off % 2, first = s_first[e] + (int)off / 2;
-    const int32_t* table = a.seqs.table(en.s0) + first;
+    const int half0 = (int)off % 2, first = (en.kind ? s_first[e] : 0) + (int)off / 2;
+    const int32_t* table = a.seqs.table(en.kind ? en.s0 : s_first[e]) + first;
     int32_t page = 0, coming = __ldg(table);  // this page, the next entry
     // rows g and g + 8: window row and head
     int i0, i1;

@@ -150,8 +150,8 @@ def kv_attention(ctx: Context, k_pool, v_pool, tables, pos, q, groups=None, scal
                  out=None):
     """Attention of rows q (n, positions <= 256, heads, head_dim) of sequences 0..n-1 over the cache that kv_append
     filled: row i of sequence b sees the positions below pos[b] and window rows 0..i (with parents: its ancestors and
-    itself).  groups [(sequences, pages), ...]: consecutive sequences whose first `pages` table entries are the same;
-    these pages are read once for the group.  scale: 1 / sqrt(head_dim) by default.  Returns the outputs in q's type."""
+    itself).  groups [(sequences, pages), ...]: consecutive sequences whose first `pages` table entries are the same
+    (or which are idle: their tables are not read); these pages are read once for the group.  scale: 1 / sqrt(head_dim) by default.  Returns the outputs in q's type."""
     pool, seqs = _pool(ctx, k_pool, v_pool, False), _seqs(ctx, tables, pos)
     hd = pool.head_dim
     qp, n, positions, heads, ldq = _rows(ctx, "q", q, None, hd)

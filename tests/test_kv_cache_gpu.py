@@ -239,6 +239,34 @@ def test_attention_of_idle_sequences_and_missing_pages(ctx, kv):
     assert bool((room[0] == 9).all()) and bool((room[6] == 9).all())  # rows before and behind stay as they are
 
 
+@pytest.mark.parametrize("positions,nh", [(1, 2), (1, 16), (6, 8), (3, 64)])  # 1, 8, 24 and 96 rows per kv head of a sequence
+def test_attention_of_a_group_whose_first_sequences_are_idle(ctx, kv, positions, nh):
+    """The group's pages come from the table of a sequence that is not idle; the idle ones' tables name other pages, or none."""
+    shared = [(8, 3), (3, 1)]
+    pos = [200, 330, 192, 250, 400, 193, 300, 201, 64, 70, 65]
+    k, v, tables, p, q = make(11, positions, nh, 2, 128, pos, F16, shared=shared)
+    graph = None
+    for idle in ([0], [0, 1, 2], [0, 3, 8, 9], [1, 10], list(range(8)), [0], list(range(11))):
+        live, entries = p.clone(), tables.clone()
+        for b in idle:
+            live[b] = -1
+            entries[b] = -1 if b % 2 else 0
+        want, bound = ref.attention(k, v, entries, live, q)
+        out = kv.kv_attention(ctx, k, v, entries, live, q, groups=shared)
+        check(out, want, bound)
+        assert not out[idle].any()
+        if graph is None:
+            held, named = live.clone(), entries.clone()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                again = kv.kv_attention(ctx, k, v, named, held, q, groups=shared)
+        held.copy_(live)
+        named.copy_(entries)
+        graph.replay()
+        assert torch.equal(again, out)
+
+
 @pytest.mark.parametrize("hd,dtype,shared", [(64, F16, None), (128, BF16, None), (128, F16, [(3, 2)])])
 def test_attention_ignores_what_is_not_seen(ctx, kv, hd, dtype, shared):
     """Infinities and NaN behind the last row, and in a row of the window: only rows that see them are touched."""

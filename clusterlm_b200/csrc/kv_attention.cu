@@ -245,6 +245,17 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {  // 0xffff at e
   return ((w & kExpMask<T>) == kExpMask<T> ? 0xffffu : 0u) |
          (((w >> 16) & kExpMask<T>) == kExpMask<T> ? 0xffff0000u : 0u);
 }
+// A pair as numbers of the type that count what is not finite in a sum of up to 63: 1 for infinity, 64 for -infinity,
+// 4096 for NaN (0 for finite values).
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_code(uint32_t w) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr uint32_t one = kHalf ? 0x3C00u : 0x3F80u, c64 = kHalf ? 0x5400u : 0x4280u, c4096 = kHalf ? 0x6C00u : 0x4580u;
+  auto code = [](uint32_t h) {
+    return (h & 0x7fffu) < kExpMask<T> ? 0u : (h & 0x7fffu) > kExpMask<T> ? c4096 : h >> 15 ? c64 : one;
+  };
+  return code(w & 0xffffu) | code(w >> 16) << 16;
+}
 
 // ---- tensor-core primitives (kind::f16: f16 or bf16 operands, f32 accumulators in TMEM)
 // K-major operand tiles with the 128-byte swizzle: rows of 64 elements, 8-row atoms of 1024 bytes, 16-byte chunk c of
@@ -523,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
   __shared__ uint32_t s_anc[kKvMaxWindow * 8];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_dead;  // a bounded wait gave up: the others give up too
-  __shared__ volatile int s_odd;   // a value that is not finite lay in a window
+  __shared__ volatile int s_odd;   // a value that is not finite, and that some row sees, became zero
   uint8_t* ring = smem + 2 * TL::kQ;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // warps: 2 x 4 softmax, then a product warp per stream, the producer and the relay
@@ -625,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
     bool ok = true;
     while (ok && walk.next(g)) {
       const int32_t* table = a.seqs.table(g.named) + g.page0;
-      // positions at or after `base` are the window's (or nobody's): their values are checked
+      // positions at or after `base` are the window's (or nobody's): values of their pages are checked
       const long long base = g.group ? 0x7fffffffffffffffll : a.seqs.base(g.s0);
       int32_t page = __ldg(table);
       for (int b = 0; b < g.pages; ++b, ++idx) {
@@ -655,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           cp_async_arrive(&copied_v[slot]);
         } else {
           // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  In a
-          // page with positions that some row does not see, such values (from `base` on) become zero here; those of
-          // window positions reach the rows that see them at the segment's end.
+          // page with positions that some row does not see, such values become zero here, and reach the rows that see
+          // them at the segment's end.
           asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
           for (int i = 0; i < kCopies; ++i) {
@@ -668,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
             for (int k = 0; k < 8; ++k) {
               const uint32_t m = nonfinite_mask<T>(w[k / 2]) & (k & 1 ? 0xffff0000u : 0xffffu);
               const long long pos = first + 8 * vc + k;
-              if (m == 0 || pos < base) continue;
+              if (m == 0) continue;
               w[k / 2] &= ~m;
               if (pos < base + a.positions) s_odd = 1;
             }
@@ -884,10 +895,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           uint32_t o[16];
           tc_ld16(to + 16 * c, o);
           tc_wait_ld();
-          if (odd && was_valid)  // values that are not finite, of window positions of these pages that the row sees
-            for (int j = 0; j < a.positions; ++j) {
+          if (odd && was_valid)  // values that are not finite, which the row sees, in these pages from the window's first on
+            for (int j = -(int)(was_base % kPageTokens); j < a.positions; ++j) {
               const long long pos = was_base + j, at = pos / kPageTokens - was.page0;
-              if (!win.sees(was_i, j) || at < 0 || at >= was.pages) continue;
+              if ((j >= 0 && !win.sees(was_i, j)) || at < 0 || at >= was.pages) continue;
               const int32_t page = a.seqs.table(was.s0)[pos / kPageTokens];
               if (page < 0 || page >= a.seqs.pool_pages) continue;
               const int pp = (int)(pos % kPageTokens);
@@ -896,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
                 const int dim = 16 * c + d;
                 const float v = to_f32(static_cast<const T*>(a.v)[(((size_t)page * a.nkv + was.kvh) * HD + dim) * kPageTokens +
                                                                   8 * kv_v_chunk(pp / 8, dim) + pp % 8]);
-                if (!(fabsf(v) <= FLT_MAX)) o[d] = __float_as_uint(NAN);
+                if (!(fabsf(v) <= FLT_MAX)) o[d] = __float_as_uint(__uint_as_float(o[d]) + v);
               }
             }
           // through shared memory, so that four lanes write 64 bytes of a row
@@ -1151,7 +1162,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
         }
         if (!plain) {
           // 0 * inf and 0 * NaN: a value that is not finite counts only for the rows that see its position.  Such
-          // values are replaced by zero, and a second product of indicators finds the outputs they reach.
+          // values are replaced by zero, and a second product counts those that reach an output: infinities of each
+          // sign (32 positions at most) and NaN.
           bool odd = false;
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n)
@@ -1164,18 +1176,19 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
               in[jj][0] = ((see0 >> (2 * jj)) & 1u ? kOne<T> : 0u) | ((see0 >> (2 * jj + 1)) & 1u ? kOne<T> << 16 : 0u);
               in[jj][1] = ((see1 >> (2 * jj)) & 1u ? kOne<T> : 0u) | ((see1 >> (2 * jj + 1)) & 1u ? kOne<T> << 16 : 0u);
             }
-            constexpr uint32_t one2 = kOne<T> | kOne<T> << 16;
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n) {
-              const uint32_t bx = nonfinite_mask<T>(va[n].x), by = nonfinite_mask<T>(va[n].y),
-                             bz = nonfinite_mask<T>(va[n].z), bw = nonfinite_mask<T>(va[n].w);
               float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma16<T>(hit, in[0][0], in[0][1], in[1][0], in[1][1], bx & one2, by & one2);
-              mma16<T>(hit, in[2][0], in[2][1], in[3][0], in[3][1], bz & one2, bw & one2);
+              mma16<T>(hit, in[0][0], in[0][1], in[1][0], in[1][1], nonfinite_code<T>(va[n].x), nonfinite_code<T>(va[n].y));
+              mma16<T>(hit, in[2][0], in[2][1], in[3][0], in[3][1], nonfinite_code<T>(va[n].z), nonfinite_code<T>(va[n].w));
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                if (hit[x] > 0.0f) O[n][x] = NAN;
-              va[n] = make_uint4(va[n].x & ~bx, va[n].y & ~by, va[n].z & ~bz, va[n].w & ~bw);
+                if (hit[x] > 0.0f) {
+                  const int h = (int)hit[x];
+                  O[n][x] += h >= 4096 || ((h & 63) && h >= 64) ? NAN : h >= 64 ? -INFINITY : INFINITY;
+                }
+              va[n] = make_uint4(va[n].x & ~nonfinite_mask<T>(va[n].x), va[n].y & ~nonfinite_mask<T>(va[n].y),
+                                 va[n].z & ~nonfinite_mask<T>(va[n].z), va[n].w & ~nonfinite_mask<T>(va[n].w));
             }
           }
         }

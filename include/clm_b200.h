@@ -250,9 +250,12 @@ CLM_API int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, 
  * positions below d_pos[b] and the window rows 0..i (or, with d_parents, its ancestors and itself), which
  * clm_b200_kv_append has placed there.  Group g (of n_groups <= 64) is the next h_group_seqs[g] sequences, whose first
  * h_group_pages[g] table entries are the same and whose positions there are all committed, or which are idle (an idle
- * sequence's table is not read): these pages are read once for all of the group's rows.  Sequences after the last group share nothing.  Softmax statistics
- * and sums are f32, the weights round to the pool's type for their product with v; scale >= 0.  Rows that see nothing
- * (idle sequences) become 0.  q rows ld_q elements apart, 16-byte aligned, like d_out; q, pool and out have one type.
+ * sequence's table is not read): these pages are read once for all of the group's rows.  Sequences after the last group
+ * share nothing.  Softmax statistics and sums are f32, the weights round to the pool's type for their product with v;
+ * scale >= 0.  Rows that see nothing (idle sequences) become 0.  A value that is not finite counts only for the rows that
+ * see its position: an infinity gives that infinity, NaN or infinities of both signs give NaN (so does, in a page that is
+ * committed to its end, an infinity whose weight rounds to 0).  q rows ld_q elements apart, 16-byte aligned, like d_out;
+ * q, pool and out have one type.
  * d_work: clm_b200_kv_attention_workspace bytes, 16-byte aligned, used by this call alone while it runs (a captured
  * graph keeps its own).  The waits inside are bounded: rows whose operands never arrive become NaN (in an engine's window
  * the commit then fails with CLM_DEADLINE_EXCEEDED). */

@@ -290,6 +290,57 @@ def test_attention_ignores_what_is_not_seen(ctx, kv, hd, dtype, shared):
     check(kv.kv_attention(ctx, k, v, tables, p, q, groups=shared), want, bound)
 
 
+@pytest.mark.parametrize("hd,dtype,nh,positions,shared,tr", [
+    (128, F16, 4, 3, None, False),       # 6 rows a kv head: the stream kernel
+    (64, BF16, 8, 4, None, True),        # 16
+    (128, BF16, 16, 4, None, False),     # 32 and more: the tile kernel, alternate pages of a row tile
+    (64, F16, 16, 20, None, True),       # 160: both streams' rows
+    (128, F16, 16, 40, None, False),     # 320: two row tiles
+    (128, F16, 4, 3, [(3, 2)], False),   # shared pages in the tile kernel, own ones in the stream kernel
+    (64, BF16, 16, 4, [(2, 1)], False),
+])
+def test_attention_of_values_that_are_not_finite(ctx, kv, hd, dtype, nh, positions, shared, tr):
+    """Infinities of either sign and NaN in a full page, in the last page's committed part and in the window: each row that
+    sees one gets it, whichever kernel has the row."""
+    base = [150, 200, 141]
+    k, v, tables, p, q = make(3, positions, nh, 2, hd, base, dtype, shared=shared)
+    parents = tree(np.random.default_rng(12), positions) if tr else None
+    sees = ref.ancestors(parents, positions)
+    ki, vi = (x.cuda() for x in ref.page_index(hd))
+    odd = torch.zeros(3, positions, 2, hd, dtype=torch.float64, device="cuda")  # what the rows of a kv head see
+    bad = v.clone()
+    for b in range(3):
+        full, partial = 70 + b, base[b] - 2  # of its own full page (a shared one for a group of two pages), and the last page
+        marks = [(full, 3, math.inf), (full, 4, -math.inf), (full, 5, math.nan), (full, 6, math.inf), (full + 1, 6, -math.inf),
+                 (partial, 7, math.inf), (partial, 8, -math.inf), (partial, 9, math.nan), (partial, 10, math.inf)]
+        for j in {1, positions - 1}:
+            slot = base[b] + j
+            marks += [(slot, 11 + j % 3, math.inf), (slot, 14, -math.inf), (slot, 15, math.nan), (slot, 10, -math.inf), (slot, 3, math.inf)]
+        if shared and b < shared[0][0] and shared[0][1] * PAGE > full:
+            marks = [m for m in marks if m[0] > full + 1] if b else marks  # the group's page is marked once
+        for slot, dim, value in marks:
+            page, at = int(tables[b, slot // PAGE]), slot % PAGE
+            k[page].view(2, -1)[:, ki[at]] = 0  # a score of 0: its weight is far from rounding to 0
+            for h in range(2):
+                d = dim + 20 * h
+                bad[page, h].view(-1)[vi[at, d]] = value
+                v[page, h].view(-1)[vi[at, d]] = 0
+                for other in range(3):  # (a shared page is seen by every sequence that names it)
+                    if int(tables[other, slot // PAGE]) != page:
+                        continue
+                    for i in range(positions):
+                        if slot < base[other] or sees[i, slot - base[other]]:
+                            odd[other, i, h, d] += value
+    want, bound = ref.attention(k, v, tables, p, q, parents)
+    want = want + odd.repeat_interleave(nh // 2, dim=2)
+    assert want.isinf().any() and want.isnan().any()
+    out = kv.kv_attention(ctx, k, bad, tables, p, q, groups=shared, parents=parents).double()
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[want.isinf()], want[want.isinf()])
+    finite = want.isfinite()
+    assert out[finite].isfinite().all() and bool(((out - want).abs() <= bound)[finite].all())
+
+
 def test_attention_with_large_scores_and_another_scale(ctx, kv):
     k, v, tables, p, q = make(2, 3, 4, 2, 64, [100, 200], BF16)
     q = q * 40  # a softmax that is nearly one-hot

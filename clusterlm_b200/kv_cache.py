@@ -92,6 +92,13 @@ def _parents(ctx: Context, parents, positions: int):
     return None if parents is None else _operand(ctx, "parents", parents, torch.int32, (positions,))
 
 
+def _count(name: str, x, most: int = 2**32 - 1) -> int:
+    """A count as the C ABI takes it (ctypes would drop the bits above its type)."""
+    if not 0 <= x <= most:
+        raise ValueError(f"{name}: expected 0 to {most}")
+    return x
+
+
 ROPE_KINDS = {"plain": 0, "linear": 1, "bands": 2, "yarn": 3}
 
 
@@ -102,8 +109,9 @@ def rope_frequencies(rot: int, theta: float, kind: str = "plain", factor: float 
     ("bands"), or blended over the pair index with the scale 0.1 ln(factor) + 1 ("yarn")."""
     if kind not in ROPE_KINDS:
         raise ValueError(f"unknown frequency scaling {kind!r}: one of {', '.join(ROPE_KINDS)}")
-    out, scale = np.empty(max(0, rot) // 2, np.float64), C.c_float()
-    call("clm_b200_rope_frequencies", ROPE_KINDS[kind], max(0, rot), theta, factor, low, high, original,
+    rot = _count("rot", max(0, rot), 2**20)
+    out, scale = np.empty(rot // 2, np.float64), C.c_float()
+    call("clm_b200_rope_frequencies", ROPE_KINDS[kind], rot, theta, factor, low, high, original,
          out.ctypes.data_as(_vp), C.byref(scale))
     return out, scale.value
 
@@ -179,9 +187,7 @@ def kv_attention(ctx: Context, k_pool, v_pool, tables, pos, q, groups=None, scal
 def set_wait_limit(ctx: Context, polls: int = 2**20) -> None:
     """Polls after which a device wait inside kv_attention gives up and leaves NaN rows, for later calls of the context
     and later windows of its engines (whose commit then fails); captured ones keep theirs."""
-    if not 0 <= polls < 2**32:
-        raise ValueError("polls: expected 0 to 2^32 - 1")
-    call("clm_b200_kv_attention_wait_limit", ctx.h, polls)
+    call("clm_b200_kv_attention_wait_limit", ctx.h, _count("polls", polls))
 
 
 def _ints(name: str, a, dtype):
@@ -233,7 +239,7 @@ class Pages:
     def __init__(self, pages: int):
         self.h = None
         h = _vp()
-        call("clm_b200_pages_create", pages, C.byref(h))
+        call("clm_b200_pages_create", _count("pages", pages), C.byref(h))
         self.h, self.pages = h, pages
 
     def close(self) -> None:
@@ -249,7 +255,7 @@ class Pages:
 
     def alloc(self, n: int) -> list[int]:
         """The n lowest free pages, one holder each (none is taken when fewer are free)."""
-        ids = np.empty(n, np.int32)
+        ids = np.empty(_count("n", n, 2**31 - 1), np.int32)
         call("clm_b200_pages_alloc", self.h, n, ids.ctypes.data_as(_vp))
         return ids.tolist()
 
@@ -263,7 +269,7 @@ class Pages:
 
     def holders(self, page: int) -> int:
         r = C.c_uint32()
-        call("clm_b200_pages_info", self.h, page, C.byref(r), None)
+        call("clm_b200_pages_info", self.h, _count("page", page, 2**31 - 1) if page >= 0 else -1, C.byref(r), None)
         return r.value
 
     def free(self) -> int:

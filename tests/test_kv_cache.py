@@ -288,3 +288,27 @@ def test_wait_limit_refuses():
     for polls in (-1, 2**32):
         with pytest.raises(ValueError):
             set_wait_limit(Ctx(), polls)
+
+
+def test_counts_that_no_32_bits_hold():
+    """ctypes keeps the low bits of an integer: such counts must not become other, valid ones."""
+    with pytest.raises(ValueError):
+        Pages(2**32 + 5)
+    with pytest.raises(ValueError):
+        Pages(-1)
+    pages = Pages(5)
+    assert pages.alloc(2) == [0, 1]
+    for call, x in ((pages.alloc, 2**32 + 1), (pages.alloc, -1), (pages.holders, 2**32)):
+        with pytest.raises(ValueError):
+            call(x)
+    for page in (-1, -2**32, -2**32 + 1):
+        with pytest.raises(ClmError) as err:
+            pages.holders(page)
+        assert err.value.code == RANGE
+    assert pages.free() == 3
+    for rot in (2**32 + 2, 2**21):
+        with pytest.raises(ValueError):
+            rope_frequencies(rot, 1e4)
+    with pytest.raises(ClmError) as err:
+        rope_frequencies(-2**32 + 4, 1e4)
+    assert err.value.code == INVALID

@@ -528,11 +528,17 @@ int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t
   const uint64_t kd = (uint64_t)pool->n_kv_heads * pool->head_dim, qd = (uint64_t)n_heads * pool->head_dim;
   CLM_CHECK(ld_k >= kd && ld_v >= kd && (!d_q || ld_q >= qd) && std::max(ld_q, std::max(ld_k, ld_v)) < (1ull << 40),
             CLM_INVALID_ARGUMENT, "a row stride is smaller than a row");
+  CLM_CHECK((uint64_t)n * positions - 1 <= (1ull << 58) / std::max(d_q ? ld_q : 1, std::max(ld_k, ld_v)), CLM_OUT_OF_RANGE,
+            "the rows do not fit into an address space");
   CLM_CHECK(!d_q || (reinterpret_cast<uintptr_t>(d_q_out) & 15) == 0, CLM_INVALID_ARGUMENT,
             "the rotated queries must be 16-byte aligned");
-  if (d_q) {  // rotated pairs are read by several threads
-    const uint64_t rows = (uint64_t)n * positions, q = reinterpret_cast<uintptr_t>(d_q), o = reinterpret_cast<uintptr_t>(d_q_out);
-    CLM_CHECK(o >= q + ((rows - 1) * ld_q + qd) * dtype_size(src_dtype) || q >= o + rows * qd * 2, CLM_INVALID_ARGUMENT,
+  if (d_q) {  // rotated pairs are read by several threads, and the kv heads' CTAs write while others read
+    const uint64_t rows = (uint64_t)n * positions, o = reinterpret_cast<uintptr_t>(d_q_out);
+    auto apart = [&](const void* p, uint64_t ld, uint64_t row) {
+      const uint64_t at = reinterpret_cast<uintptr_t>(p);
+      return o >= at + ((rows - 1) * ld + row) * dtype_size(src_dtype) || at >= o + rows * qd * 2;
+    };
+    CLM_CHECK(apart(d_q, ld_q, qd) && apart(d_k, ld_k, kd) && apart(d_v, ld_v, kd), CLM_INVALID_ARGUMENT,
               "the rotated queries must not overlap the rows");
   }
   AppendArgs a{};

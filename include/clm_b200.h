@@ -236,11 +236,11 @@ enum { CLM_ROPE_PLAIN = 0, CLM_ROPE_LINEAR = 1, CLM_ROPE_BANDS = 2, CLM_ROPE_YAR
 CLM_API int clm_b200_rope_frequencies(int kind, uint32_t rot, double theta, double factor, double low, double high,
                                       double original, double* h_inv_freq, float* h_scale);
 /* Rows enter the cache: for sequences 0..n-1, `positions` rows each, at d_pos[b] + i: k (rotated) and v go to the
- * pages, q (optional) is rotated into d_q_out [n][positions][n_heads][head_dim] in the pool's type (not in place).
- * Row r of q / k / v starts ld elements after row r - 1 (slices of one fused projection).  d_parents (optional, <= 256
- * nodes): a tree window as in clm_b200_run_tree_window; node i is placed at d_pos[b] + i and rotated at d_pos[b] +
- * depth(i).  rope NULL: no rotation.  The positions are not advanced.  Idle sequences: nothing enters, their q rows
- * become 0. */
+ * pages, q (optional) is rotated into d_q_out [n][positions][n_heads][head_dim] in the pool's type (not over q, k or v).
+ * No two sequences of a call have a row in the same place.  Row r of q / k / v starts ld elements after row r - 1 (slices
+ * of one fused projection).  d_parents (optional, <= 256 nodes): a tree window as in clm_b200_run_tree_window; node i is
+ * placed at d_pos[b] + i and rotated at d_pos[b] + depth(i).  rope NULL: no rotation.  The positions are not advanced.
+ * Idle sequences: nothing enters, their q rows become 0. */
 CLM_API int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, uint32_t layer,
                                const clm_b200_kv_seqs* seqs, uint32_t n, uint32_t positions, uint32_t n_heads,
                                int src_dtype, const void* d_q, uint64_t ld_q, const void* d_k, uint64_t ld_k,

@@ -312,3 +312,16 @@ def test_counts_that_no_32_bits_hold():
     with pytest.raises(ClmError) as err:
         rope_frequencies(-2**32 + 4, 1e4)
     assert err.value.code == INVALID
+
+
+@pytest.mark.parametrize("k,v,out", [(A, A + 2**16, A + 2047), (A, A + 2**16, A + 2**16 - 6144 + 16), (A + 2**16, A, A + 16),
+                                     (A + 2**16, A, A + 2**16 + 5 * 512 + 512 - 16)])
+def test_append_refuses_queries_over_keys_or_values(k, v, out):
+    """Six rows of two kv heads of 128 in 16 bits, 256 elements apart: 3,072 bytes each; the result's 6,144 bytes."""
+    assert append(q=A + 2**20, k=k, v=v, out=out & ~15, ld_q=512, ld_k=256, ld_v=256) == INVALID
+    assert b"overlap" in _native.lib.clm_b200_last_error()
+
+
+def test_append_refuses_rows_beyond_any_memory():
+    assert append(n=4, positions=2**24, ld_k=2**39, out=A + 2**40) == RANGE
+    assert append(n=4, positions=2**24, q=0, heads=0, ld_v=2**39) == RANGE

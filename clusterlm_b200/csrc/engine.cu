@@ -69,6 +69,7 @@ struct Session {
   float* d_dprobs = nullptr;   // pipeline tail: draft distributions of the current window [W][V]
   cudaEvent_t queued = nullptr;  // after what the last call queued for it on a caller's stream
   bool has_queued = false;       // such a call was made since the context's stream last waited for it
+  bool in_rounds = false;      // pipeline: rounds have begun, so a message of its next window is on its way
   bool own_links = false;      // pipeline: the session's messages use lin / lout below (clm_b200_pipe_attach_session)
   LinkDev lin, lout;
 };
@@ -1750,11 +1751,7 @@ static int add_session(LlamaEngine* e, uint64_t id, const Session* parent) {
     const size_t win = (size_t)(e->wmax() + 1) * sizeof(int32_t), probs = (size_t)e->wmax() * e->d.V * sizeof(float);
     err = cudaMalloc(&s->d_win, win);
     if (err == cudaSuccess) err = cudaMalloc(&s->d_dprobs, probs);
-    if (err == cudaSuccess)
-      err = parent ? cudaMemcpyAsync(s->d_win, parent->d_win, win, cudaMemcpyDeviceToDevice, st)
-                   : cudaMemsetAsync(s->d_win, 0, win, st);
-    if (err == cudaSuccess && parent)
-      err = cudaMemcpyAsync(s->d_dprobs, parent->d_dprobs, probs, cudaMemcpyDeviceToDevice, st);
+    if (err == cudaSuccess) err = cudaMemsetAsync(s->d_win, 0, win, st);  // (a fork's parent has none yet)
   }
   int rc = err == cudaSuccess ? CLM_OK : cuda_fail(err, "session_open");
   if (rc == CLM_OK && parent && !e->layers.empty() && parent->pos % kPageTokens != 0) {
@@ -1811,6 +1808,8 @@ int llama_session_fork(LlamaEngine* e, uint64_t parent_id, uint64_t id) {
   CLM_CHECK(parent != nullptr, CLM_NOT_FOUND, "session not open");
   CLM_CHECK(find_session(e, id) == nullptr, CLM_ALREADY_EXISTS, "session already open");
   CLM_CHECK(parent->outstanding == 0, CLM_FAILED_PRECONDITION, "a window is outstanding for the parent session");
+  // (stages that have run a round are behind the tail by the window that is on its way, and no message comes for a child)
+  CLM_CHECK(!parent->in_rounds, CLM_FAILED_PRECONDITION, "the parent session's rounds have begun in a pipeline");
   CLM_TRY(e->after_queued(*parent));  // rounds in flight on a caller's stream
   CLM_TRY(sync_pos(e, parent));
   return add_session(e, id, parent);
@@ -2342,6 +2341,7 @@ int llama_pipe_begin(LlamaEngine* e, uint64_t id, uint32_t row, const clm_b200_s
   CLM_CHECK(row < e->spec.max_window, CLM_OUT_OF_RANGE, "row outside the last window");
   cudaStream_t st = pick_stream(e->ctx, stream);
   LlamaEngine::Queued mark(e, st, s);
+  s->in_rounds = true;
   const bool stochastic = p->temperature > 0.0f;
   RoundCtl c{p->temperature, 0u, (unsigned long long)p->seed};
   CLM_CUDA(cudaMemcpyAsync(e->ctl, &c, sizeof(c), cudaMemcpyHostToDevice, st));
@@ -2361,6 +2361,7 @@ int llama_pipe_round(LlamaEngine* e, uint64_t id, const clm_b200_spec_params* p,
   CLM_TRY(pipe_session(e, id, p->q, &s));
   cudaStream_t st = pick_stream(e->ctx, stream);
   LlamaEngine::Queued mark(e, st, s);
+  s->in_rounds = true;
   const bool stochastic = p->temperature > 0.0f;
   if (e->spec.role == CLM_ROLE_TAIL) {
     RoundCtl c{p->temperature, 0u, (unsigned long long)p->seed};

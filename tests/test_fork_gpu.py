@@ -144,3 +144,49 @@ def test_forked_rounds_follow_the_parent_and_part_by_seed(ctx):
                for s, seed in ((1, 5), (2, 5), (3, 6)))
     assert a == b and a != c
     e.close()
+
+
+@pytest.mark.parametrize("length", [64, 100])
+def test_forks_of_a_split_model_equal_the_whole_ones(ctx, length):
+    """Prefix, middle and tail (with its draft head) each fork: their windows chained are the whole engine's, to the bit."""
+    from clusterlm_b200.engine import ROLE_MIDDLE, ROLE_PREFIX, ROLE_TAIL
+
+    geo = small_geo(n_layers=3)
+    kw = dict(max_context=192, max_window=16, sessions=3)
+    whole = make_engine(ctx, geo, **kw)
+    stages = [make_engine(ctx, geo, ROLE_PREFIX, 0, 1, **kw), make_engine(ctx, geo, ROLE_MIDDLE, 1, 2, **kw),
+              make_engine(ctx, geo, ROLE_TAIL, 2, 3, **kw)]
+    rng = np.random.default_rng(length)
+    prompt = rng.integers(0, geo.vocab, length).astype(np.int32)
+
+    def window(s, at, toks, keep):
+        want = whole.run_window(s, at, tokens=toks)
+        rec = stages[0].run_window(s, at, tokens=toks)
+        rec = stages[1].run_window(s, at, records=rec)
+        np.testing.assert_array_equal(stages[2].run_window(s, at, records=rec), want)
+        for e in (whole, *stages):
+            e.commit(s, keep)
+
+    for e in (whole, *stages):
+        e.open_session(1)
+    for at in range(0, length, 16):
+        window(1, at, prompt[at:at + 16], len(prompt[at:at + 16]))
+    for e in (whole, *stages):
+        e.fork_session(1, 2)
+        e.fork_session(2, 3)
+        assert [e.position(s) for s in (1, 2, 3)] == [length] * 3
+    at = {s: length for s in (1, 2, 3)}
+    for q, keep in [(4, 4), (8, 3), (4, 1), (16, 16)]:
+        for s in (2, 1, 3):
+            window(s, at[s], rng.integers(0, geo.vocab, q).astype(np.int32), keep)
+            at[s] += keep
+    drafts = [e.mtp_draft(5, 3) for e in (whole, stages[2])]
+    np.testing.assert_array_equal(*drafts)
+    for e in (whole, *stages):
+        e.close_session(1)
+        e.fork_session(3, 1)  # the place and the pages go round
+        assert e.position(1) == at[3]
+    at[1] = at[3]
+    window(1, at[1], rng.integers(0, geo.vocab, 4).astype(np.int32), 4)
+    for e in (whole, *stages):
+        e.close()

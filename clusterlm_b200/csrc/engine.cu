@@ -1753,6 +1753,11 @@ static int add_session(LlamaEngine* e, uint64_t id, const Session* parent) {
     if (err == cudaSuccess) err = cudaMalloc(&s->d_dprobs, probs);
     if (err == cudaSuccess) err = cudaMemsetAsync(s->d_win, 0, win, st);  // (a fork's parent has none yet)
   }
+  if (parent) {  // its messages take its parent's way
+    s->own_links = parent->own_links;
+    s->lin = parent->lin;
+    s->lout = parent->lout;
+  }
   int rc = err == cudaSuccess ? CLM_OK : cuda_fail(err, "session_open");
   if (rc == CLM_OK && parent && !e->layers.empty() && parent->pos % kPageTokens != 0) {
     // the parent's last page, in every layer

@@ -362,8 +362,9 @@ CLM_API int clm_b200_session_close(clm_b200_engine* e, uint64_t session);
  * continuations of one prompt so prefill it once; clm_b200_run_batch_window reads the pages that consecutive sessions of
  * a batch share once for all of them.  A child takes one of max_sessions.
  * Llama-family engines of any role; the stages of a split model each fork.  In a pipeline (clm_b200_pipe_*) a session is
- * forked after its prefill and before its rounds (later: CLM_FAILED_PRECONDITION) (no
- * reference counterpart: a domain's sequence state is private, reference_domain.cpp:297-329). */
+ * forked after its prefill and before its rounds (later: CLM_FAILED_PRECONDITION); the child's messages take the parent's
+ * links until clm_b200_pipe_attach_session binds others (no reference counterpart: a domain's sequence state is private,
+ * reference_domain.cpp:297-329). */
 CLM_API int clm_b200_session_fork(clm_b200_engine* e, uint64_t parent, uint64_t child);
 /* One verification window of `positions` rows (1..max_window; max_window <= 256: windows of more than 16 rows,
  * prefill chunks and large trees, run on the tensor-core path) at committed position `base`.

@@ -1162,18 +1162,21 @@ struct LlamaEngine : clm_b200_engine {
     Queued(const Queued&) = delete;
     Queued& operator=(const Queued&) = delete;
     ~Queued() {
+      if (st == e->ctx->stream) return;
       cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-      if (st == e->ctx->stream || cudaStreamIsCapturing(st, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone)
-        return;
+      cudaError_t rc = cudaStreamIsCapturing(st, &capture);
+      if (rc == cudaSuccess && capture != cudaStreamCaptureStatusNone) return;  // nothing is queued
       for (int i = 0; i < n; ++i) {
         Session& x = *s[i];
         x.has_queued = true;
-        if (x.queued == nullptr && cudaEventCreateWithFlags(&x.queued, cudaEventDisableTiming) != cudaSuccess) x.queued = nullptr;
-        if (x.queued != nullptr && cudaEventRecord(x.queued, st) != cudaSuccess) {
+        if (rc == cudaSuccess && x.queued == nullptr) rc = cudaEventCreateWithFlags(&x.queued, cudaEventDisableTiming);
+        if (rc == cudaSuccess) rc = cudaEventRecord(x.queued, st);
+        if (rc != cudaSuccess && x.queued != nullptr) {  // after_queued then waits for the device
           cudaEventDestroy(x.queued);
-          x.queued = nullptr;  // (after_queued then waits for the device)
+          x.queued = nullptr;
         }
       }
+      if (rc != cudaSuccess) cudaGetLastError();  // (no launch check is to find it)
     }
   };
   // Orders the context's stream behind the session's work on callers' streams.

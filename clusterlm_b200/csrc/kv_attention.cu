@@ -7,7 +7,7 @@
 // An "entry" is a group's shared pages (rows: all query heads of a kv head of all the group's window rows) or a
 // sequence's own pages (rows: its own).  Entries of up to kStreamRows rows per kv head are bound by reading the
 // pages: the stream kernel, whose warps load the operands of mma.sync straight from global memory.  Entries of more
-// rows are bound by the products: the tile kernel, on the tensor cores' accumulators in TMEM.  All groups of a call
+// rows by products and softmax: the tile kernel, on the tensor cores' accumulators in TMEM.  All groups of a call
 // go to one of the two, and all sequences; so a call is one or two launches and the combining one.
 //
 // Work of a kernel is one line of units: per entry, per item (kv head, and row tile in the tile kernel), its pages
@@ -19,8 +19,8 @@
 // GPU time of a call (fp16, head_dim 128, 32 heads over 8 unless said): 4 sequences of about 1,000 positions 13 us; 8
 // tree windows of 16 rows over 4,096 shared positions 34 us; 64 windows of 4 rows, 16,384 shared and about 500 own
 // positions each, 138 us (tile kernel 83 us, 0.83 PFLOP/s; stream kernel 36 us, 3.7 TB/s; combining kernel 10 us);
-// 256 rows over 8,192 positions (bf16) 101 us (0.72 PFLOP/s in the tile kernel); 64 sequences of 2,048 positions, 8
-// rows a kv head, 94 us (5.7 TB/s).
+// 256 rows over 8,192 positions (bf16) 102 us (0.72 PFLOP/s in the tile kernel); 64 sequences of 2,048 positions, 8
+// rows a kv head, 95 us (5.6 TB/s).
 #include <algorithm>
 #include <cfloat>
 
@@ -47,7 +47,7 @@ constexpr int kStreamSwitch = 2;  // stream kernel: a segment's start and end ta
 constexpr int kSwitch = 12;
 
 struct Plan {
-  uint32_t cum[kMaxEntries + 1];  // work units before entry e (below 2^31, checked by the host)
+  uint32_t cum[kMaxEntries + 1];  // work units before entry e (below 2^32: two per page, which the host counts)
   int pages[kMaxEntries];         // pages of an item of entry e (stream kernel: half pages with a position that is seen)
   uint32_t shares, q, r;          // how the line is cut (below)
   __device__ __forceinline__ struct Shares cut() const;
@@ -509,10 +509,12 @@ struct Walk {
 // Every wait is bounded.  When one gives up, all warps do: the rows whose products are missing become NaN, the caller's
 // flag is raised, and the CTA ends after its products and copies in flight.
 //
-// Bound by the tensor pipe: a page of both streams takes 2,230 clocks, of which 16 score products (M 128, N 64, K 16,
-// both operands in shared memory) take 107 each and 8 products with V 64 each.  (Score products of two pages, N 128,
-// take no longer, but their scores leave no room for a second buffer: a page of both streams then waits for its own
-// softmax, 3,100 clocks.  With half the query in TMEM, one score buffer: 2,750.)
+// A page of both streams takes 2,230 clocks, in which 16 score products (M 128, N 64, K 16, both operands in shared
+// memory) complete every 107 and 8 products with V every 64, and the softmax warps are busy for about 1,900: the chain of
+// scores, softmax and products bounds it, no unit alone (256 rows over 8,192 positions: tensor unit 53% of the active
+// clocks, of which arithmetic 40%, special-function unit 31%, issue slots 41%).  (Score products of two pages, N 128, take
+// no longer, but their scores leave no room for a second buffer: a page of both streams then waits for its own softmax,
+// 3,100 clocks.  With half the query in TMEM, one score buffer: 2,750.)
 //
 // The producer warp copies the pages with 16-byte asynchronous copies, because the cache's chunk order is not the
 // tensor cores' (128-byte swizzle): each chunk goes straight to its place, where a bulk copy would need a reordering
@@ -1024,7 +1026,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
     int i0, i1;
     long long b0, b1;
     bool v0, v1;
-    // (the warp's queries lie in shared memory: with them in registers the loop would spill)
+    // (the warp's queries lie in shared memory: head_dim 128 has no registers left, and spills 40 bytes as it is)
     auto s_q = [&](int which, int u) { return &s_query[warp][which * KW + u][lane]; };
     auto row = [&](int which, int& i, long long& base, bool& valid) {
       const int r = g + 8 * which;

@@ -21,10 +21,11 @@
 //      is left, its lowest indices stay.
 //   3. the cumulative mass over CTAs, then warp segments, then entries locates the token.
 //
-// Bound by instructions, and by the cluster's barriers where there are few rows: 1 row of 128,256 15 us (27,000
-// clocks on eight CTAs, of which eight barriers and what waits for them take half); 64 of 151,936 with top-p 69 us (two
-// rows' slices on an SM at a time: two waves of 52,000 clocks, half the issue slots used); 256 of 128,256 with mixed
-// settings 158 us.
+// One row of 128,256 takes 15 us on sixteen CTAs (on eight 16 us, 27,000 clocks, of which eight barriers and what waits for
+// them take half).  64 of 151,936 with top-p take 69 us: two rows' slices on an SM at a time, two waves of 52,000 clocks
+// with half the issue slots used; ranking and the histogram's merging and scanning, which all CTAs of a row do alike, take
+// twice as long as the first pass over the entries, and two CTAs an SM leave 64 registers a thread, with 168 bytes
+// spilled.  256 of 128,256 with mixed settings take 158 us.
 #include <cooperative_groups.h>
 
 #include <cfloat>

@@ -123,11 +123,6 @@ __device__ __forceinline__ int group_of(const Args& a, int b) {
   return lo;
 }
 
-__device__ __forceinline__ int shared_pages(const Args& a, int b) {
-  const int g = group_of(a, b);
-  return g < 0 ? 0 : min((int)a.groups.pages[g], a.seqs.max_pages);
-}
-
 // Items before entry e, within its kind (groups, sequences).
 __device__ __forceinline__ int items_before(const Args& a, int e) {
   if (e >= a.groups.n) return (e - a.groups.n) * a.kind[1].tiles * a.nkv;
@@ -154,25 +149,28 @@ __device__ __forceinline__ Shares Plan::cut() const { return Shares{shares, q, r
 // of its entries (the other kernel's have none).  first: a sequence's first page of its own; of a group the sequence whose
 // table names its pages, the first that is not idle (an idle one's table may name anything).
 __device__ void make_plan(const Args& a, Plan* plan, int* first, int tile, uint32_t shares) {
-  const int E = a.groups.n + a.seqs.n;
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    const Entry en = entry_of(a, e);
-    const int per = tile ? 1 : 2, unit = kPageTokens / per;
-    int pages = 0, at = 0;
-    if (e < a.groups.n) {
-      for (at = en.s0; at < en.s1 && a.seqs.base(at) < 0; ++at) {
-      }
-      if (at < en.s1) pages = per * min((int)a.groups.pages[e], a.seqs.max_pages);
-    } else {
-      const long long base = a.seqs.base(en.s0);
-      at = shared_pages(a, en.s0);
-      if (base >= 0)
-        pages = max(0, (int)min((base + a.positions + unit - 1) / unit, (long long)per * a.seqs.max_pages) - per * at);
-    }
+  const int G = a.groups.n, E = G + a.seqs.n, per = tile ? 1 : 2, unit = kPageTokens / per;
+  auto put = [&](int e, const Entry& en, int pages) {
     plan->pages[e] = pages;
-    first[e] = at;
     plan->cum[e + 1] = a.kind[en.kind].tile == tile ? units_of(en, pages) * (uint32_t)(en.tiles * a.nkv) : 0u;
+  };
+  for (int e = threadIdx.x; e < G; e += blockDim.x) first[e] = a.seqs.n;
+  __syncthreads();
+  for (int e = G + threadIdx.x; e < E; e += blockDim.x) {
+    const Entry en = entry_of(a, e);
+    const long long base = a.seqs.base(en.s0);
+    const int g = group_of(a, en.s0), at = g < 0 ? 0 : min((int)a.groups.pages[g], a.seqs.max_pages);
+    int pages = 0;
+    if (base >= 0) {
+      pages = max(0, (int)min((base + a.positions + unit - 1) / unit, (long long)per * a.seqs.max_pages) - per * at);
+      if (g >= 0) atomicMin(&first[g], en.s0);
+    }
+    first[e] = at;
+    put(e, en, pages);
   }
+  __syncthreads();
+  for (int e = threadIdx.x; e < G; e += blockDim.x)
+    put(e, entry_of(a, e), first[e] < a.seqs.n ? per * min((int)a.groups.pages[e], a.seqs.max_pages) : 0);
   __syncthreads();
   if (threadIdx.x < 32) {
     uint32_t run = 0;

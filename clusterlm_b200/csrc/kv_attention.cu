@@ -1024,7 +1024,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, 1) kv_stream_kernel(const _
     int i0, i1;
     long long b0, b1;
     bool v0, v1;
-    // (the warp's queries lie in shared memory: head_dim 128 has no registers left, and spills 40 bytes as it is)
+    // (the warp's queries lie in shared memory: head_dim 128 has no registers left, and spills 24 bytes as it is)
     auto s_q = [&](int which, int u) { return &s_query[warp][which * KW + u][lane]; };
     auto row = [&](int which, int& i, long long& base, bool& valid) {
       const int r = g + 8 * which;

@@ -32,8 +32,9 @@ struct KvSeqs {
   int mapped = 0;      // 1: sequence b is slot[b], else slot b
   uint16_t slot[kKvMaxMapped] = {};
   __device__ __forceinline__ int at(int b) const { return mapped ? slot[b] : b; }
+  // (held at 2^62, far behind every table, so that sums with a window's rows do not wrap)
   __device__ __forceinline__ long long base(int b) const {
-    return *reinterpret_cast<const long long*>(pos + (long long)at(b) * pos_stride);
+    return min(*reinterpret_cast<const long long*>(pos + (long long)at(b) * pos_stride), 1ll << 62);
   }
   __device__ __forceinline__ const int32_t* table(int b) const { return tables + (long long)at(b) * table_stride; }
 };

@@ -239,6 +239,22 @@ def test_attention_of_idle_sequences_and_missing_pages(ctx, kv):
     assert bool((room[0] == 9).all()) and bool((room[6] == 9).all())  # rows before and behind stay as they are
 
 
+def test_positions_behind_every_table(ctx, kv):
+    """The largest positions: their rows have no page, are given back all the same, and see every page of the table."""
+    k, v, tables, p, q = make(3, 4, 4, 2, 64, [130, 200, 100], F16)
+    table = tables[:, :2].contiguous()
+    for far in (2**63 - 1, 2**63 - 3, 2**62, 2**40):
+        p[:] = torch.tensor([far, 2**63 - 64, far], device="cuda")
+        K, V = k.clone(), v.clone()
+        kn = torch.randn(3, 4, 2, 64, device="cuda", dtype=F16)
+        room = torch.full((3, 4, 4, 64), math.nan, device="cuda", dtype=F16)
+        assert torch.equal(kv.kv_append(ctx, K, V, table, p, q, kn, kn, out=room), q)
+        assert torch.equal(K, k) and torch.equal(V, v)
+        near = torch.full((3,), 128, dtype=torch.int64, device="cuda")  # as many positions as the tables hold
+        for x in (q, torch.randn(3, 40, 4, 64, device="cuda", dtype=F16)):
+            check(kv.kv_attention(ctx, k, v, table, p, x), *ref.attention(k, v, table, near, x))
+
+
 @pytest.mark.parametrize("positions,nh", [(1, 2), (1, 16), (6, 8), (3, 64)])  # 1, 8, 24 and 96 rows per kv head of a sequence
 def test_attention_of_a_group_whose_first_sequences_are_idle(ctx, kv, positions, nh):
     """The group's pages come from the table of a sequence that is not idle; the idle ones' tables name other pages, or none."""

@@ -253,9 +253,8 @@ CLM_API int clm_b200_kv_append(clm_b200_ctx* ctx, const clm_b200_kv_pool* pool, 
  * sequence's table is not read): these pages are read once for all of the group's rows.  Sequences after the last group
  * share nothing.  Softmax statistics and sums are f32, the weights round to the pool's type for their product with v;
  * scale >= 0.  Rows that see nothing (idle sequences) become 0.  A value that is not finite counts only for the rows that
- * see its position: an infinity gives that infinity, NaN or infinities of both signs give NaN (so does, in a page that is
- * committed to its end, an infinity whose weight rounds to 0).  q rows ld_q elements apart, 16-byte aligned, like d_out;
- * q, pool and out have one type.
+ * see its position: an infinity gives that infinity, NaN or infinities of both signs give NaN (so may an infinity whose
+ * weight is too small to be held).  q rows ld_q elements apart, 16-byte aligned, like d_out; q, pool and out have one type.
  * d_work: clm_b200_kv_attention_workspace bytes, 16-byte aligned, used by this call alone while it runs (a captured
  * graph keeps its own).  The waits inside are bounded: rows whose operands never arrive become NaN (in an engine's window
  * the commit then fails with CLM_DEADLINE_EXCEEDED). */

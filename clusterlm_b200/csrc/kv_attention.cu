@@ -895,10 +895,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(const __grid_const
           uint32_t o[16];
           tc_ld16(to + 16 * c, o);
           tc_wait_ld();
-          if (odd && was_valid)  // values that are not finite, which the row sees, in these pages from the window's first on
+          if (odd && was_valid)  // values that are not finite, which the row sees, in the stream's pages from the window's first
+                                 // on (not another stream's: a row that sees none of this one's pages has no maximum here)
             for (int j = -(int)(was_base % kPageTokens); j < a.positions; ++j) {
               const long long pos = was_base + j, at = pos / kPageTokens - was.page0;
-              if ((j >= 0 && !win.sees(was_i, j)) || at < 0 || at >= was.pages) continue;
+              if ((j >= 0 && !win.sees(was_i, j)) || at < 0 || at >= was.pages || (!was.pair && at % 2 != s)) continue;
               const int32_t page = a.seqs.table(was.s0)[pos / kPageTokens];
               if (page < 0 || page >= a.seqs.pool_pages) continue;
               const int pp = (int)(pos % kPageTokens);

@@ -357,6 +357,32 @@ def test_attention_of_values_that_are_not_finite(ctx, kv, hd, dtype, nh, positio
     assert out[finite].isfinite().all() and bool(((out - want).abs() <= bound)[finite].all())
 
 
+@pytest.mark.parametrize("positions,nh,hd", [(33, 1, 64), (33, 2, 128), (20, 7, 64), (70, 4, 128)])
+def test_attention_of_an_infinity_next_to_pages_that_are_not_seen(ctx, kv, positions, nh, hd):
+    """The window begins in one page and ends in others, so that its first rows see nothing of these: an infinity in the first
+    page reaches them as such, whichever warps have the other pages (enough sequences that a CTA takes several pages)."""
+    n, nkv = 48, 4
+    base = [(57, 2, 63, 50)[b % 4] for b in range(n)]
+    k, v, tables, p, q = make(n, positions, nh * nkv, nkv, hd, base, BF16)
+    ki, vi = (x.cuda() for x in ref.page_index(hd))
+    bad, odd = v.clone(), torch.zeros(n, positions, nkv, hd, dtype=torch.float64, device="cuda")
+    for b in range(n):
+        for slot, d, value in ((base[b], 3, math.inf), (base[b] + 4, 5, -math.inf), (1, 7, math.inf), (base[b] + 1, 7, -math.inf),
+                               (base[b] + positions - 1, 9, math.inf), (0, 11, math.nan)):
+            page, at = int(tables[b, slot // PAGE]), slot % PAGE
+            k[page].view(nkv, -1)[:, ki[at]] = 0
+            v[page].view(nkv, -1)[:, vi[at, d]] = 0
+            bad[page].view(nkv, -1)[:, vi[at, d]] = value
+            odd[b, max(0, slot - base[b]):, :, d] += value
+    want, bound = ref.attention(k, v, tables, p, q)
+    want = want + odd.repeat_interleave(nh, dim=2)
+    out = kv.kv_attention(ctx, k, bad, tables, p, q).double()
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[want.isinf()], want[want.isinf()])
+    finite = want.isfinite()
+    assert bool(((out - want).abs() <= bound)[finite].all())
+
+
 def test_attention_with_large_scores_and_another_scale(ctx, kv):
     k, v, tables, p, q = make(2, 3, 4, 2, 64, [100, 200], BF16)
     q = q * 40  # a softmax that is nearly one-hot
